@@ -163,6 +163,32 @@ int h3_gemm_nvfp4(const uint8_t* a_codes, const uint8_t* a_sf, const H3ScaleSlot
  * tfvideo/minimax_h3.py:296-298).  rope: fp32 [S, rot/2, 2, 2] rotation matrices; rot % 8 == 0, rot <= 128. */
 int h3_qknorm_rope(void* q, void* k, long long ld, int S, int H, int rot, const float* qw, const float* kw,
                    const float* rope, float eps, void* stream);
+/* Positions of a packed sequence over 1..4 axes (time, height, width, ...): element (s, a) at pos + s * ld +
+ * a * axis_stride (elements of `type`; any strides).  Axis a rotates dims[a] (even) dims of a head: pair p of the
+ * rotated span (dims p and p + rot/2, rot = sum of dims <= 128) belongs to the axes one after another, and the j-th
+ * pair of axis a turns by pos[s, a] * theta[a]^(-2j / dims[a]) radians, formed in 64 bits. */
+enum { H3_POS_I32 = 0, H3_POS_I64 = 1, H3_POS_F32 = 2 };
+typedef struct H3Positions {
+  const void* pos;
+  int type;              /* H3_POS_* */
+  long long ld;
+  long long axis_stride;
+  int axes;
+  int dims[4];
+  double theta[4];
+} H3Positions;
+/* The rotation table of those positions, fp32 [S, rot/2, 2, 2] ([[cos, -sin], [sin, cos]] per pair): the `rope`
+ * argument of h3_qknorm_rope and ComfyUI's rope_freqs (in the reference the host model makes it,
+ * tools/profile_block.py:41-45).  out: 16-byte aligned. */
+int h3_rope_axes(const H3Positions* pos, int S, float* out, void* stream);
+/* h3_qknorm_rope straight from positions, with no table: per-head RMSNorm (weights qw, kw [128], 16-byte aligned) and
+ * the split-half rotation of the first rot dims in one pass.  q holds Hq heads and k Hk (they may differ); element
+ * (s, h, d) at s * ld + h * hs + d.  Outputs are the inputs themselves (in place) or memory apart from them.
+ * rot % 8 == 0; strides multiples of 4 elements, pointers 8-byte aligned. */
+int h3_qknorm_rope_axes(const void* q, long long ldq, long long hsq, const void* k, long long ldk, long long hsk,
+                        int S, int Hq, int Hk, const float* qw, const float* kw, const H3Positions* pos, float eps,
+                        void* out_q, long long ldoq, long long hsoq, void* out_k, long long ldok, long long hsok,
+                        void* stream);
 /* Scratch bytes h3_attn_fp8 needs for S tokens and H heads. */
 size_t h3_attn_workspace_bytes(int S, int H);
 /* Non-causal FP8 attention softmax(q k^T / sqrt(128)) v over H heads of head_dim 128 (replaces the attention

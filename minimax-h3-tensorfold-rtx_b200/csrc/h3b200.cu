@@ -2,6 +2,7 @@
 // included here, so the device status word and the kernels live in one module.  Host code validates arguments,
 // builds TMA tensor maps (cuTensorMapEncodeTiled, fetched from the driver at first use) and launches on the
 // caller's stream.  Nothing here allocates device memory.
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -12,6 +13,7 @@
 #include "elementwise.cuh"
 #include "gemm_nvfp4.cuh"
 #include "h3b200.h"
+#include "rope_axes.cuh"
 
 using namespace h3;
 
@@ -547,6 +549,77 @@ int h3_qknorm_rope(void* q, void* k, long long ld, int S, int H, int rot, const 
                eps};
   qknorm_rope_kernel<<<(unsigned)((S + 7) / 8), 256, 0, S_(stream)>>>(a);
   return check_launch("h3_qknorm_rope");
+}
+
+namespace {
+// Checks an H3Positions and lays out each pair's axis and frequency for the kernels.
+int rope_pos(RopePos* r, const H3Positions* p, const char* who) {
+  if (!p || !p->pos) return fail(H3_ERR_ARG, "%s: NULL positions", who);
+  if (p->type != H3_POS_I32 && p->type != H3_POS_I64 && p->type != H3_POS_F32)
+    return fail(H3_ERR_ARG, "%s: position type %d is none of H3_POS_*", who, p->type);
+  if (!aligned(p->pos, p->type == H3_POS_I64 ? 8 : 4)) return fail(H3_ERR_ARG, "%s: misaligned positions", who);
+  if (p->axes < 1 || p->axes > 4) return fail(H3_ERR_SHAPE, "%s: 1..4 position axes, got %d", who, p->axes);
+  r->pos = p->pos;
+  r->ld = p->ld;
+  r->axis_stride = p->axis_stride;
+  r->type = p->type;
+  r->pairs = 0;
+  for (int a = 0; a < p->axes; ++a) {
+    const int d = p->dims[a];
+    if (d <= 0 || d % 2 || r->pairs + d / 2 > kRopeMaxPairs)
+      return fail(H3_ERR_SHAPE, "%s: each axis rotates an even number of dims > 0, together <= %d (axis %d: %d)", who,
+                  2 * kRopeMaxPairs, a, d);
+    if (!(p->theta[a] > 0.0) || !std::isfinite(p->theta[a]))
+      return fail(H3_ERR_ARG, "%s: theta of axis %d must be positive and finite", who, a);
+    const double step = std::pow(p->theta[a], -2.0 / d);
+    double f = 0.15915494309189533577;   // 1 / (2 pi)
+    for (int j = 0; j < d / 2; ++j, f *= step) {
+      r->axis[r->pairs] = (uint8_t)a;
+      r->turns[r->pairs++] = f;
+    }
+  }
+  return H3_OK;
+}
+}  // namespace
+
+int h3_rope_axes(const H3Positions* pos, int S, float* out, void* stream) {
+  RopePos r;
+  int rc = rope_pos(&r, pos, "h3_rope_axes");
+  if (rc) return rc;
+  if (!out || !aligned(out, 16)) return fail(H3_ERR_ARG, "h3_rope_axes: out NULL or not 16-byte aligned");
+  if (S <= 0) return fail(H3_ERR_SHAPE, "h3_rope_axes: S must be positive (S=%d)", S);
+  const int per = 256 / r.pairs;
+  const int need = (int)(((long long)S + per - 1) / per), cap = num_sms() * 8;
+  rope_axes_kernel<<<need < cap ? need : cap, 256, 0, S_(stream)>>>(r, S, reinterpret_cast<float4*>(out));
+  return check_launch("h3_rope_axes");
+}
+
+int h3_qknorm_rope_axes(const void* q, long long ldq, long long hsq, const void* k, long long ldk, long long hsk,
+                        int S, int Hq, int Hk, const float* qw, const float* kw, const H3Positions* pos, float eps,
+                        void* out_q, long long ldoq, long long hsoq, void* out_k, long long ldok, long long hsok,
+                        void* stream) {
+  const char* who = "h3_qknorm_rope_axes";
+  RopePos r;
+  int rc = rope_pos(&r, pos, who);
+  if (rc) return rc;
+  if (!q || !k || !qw || !kw || !out_q || !out_k) return fail(H3_ERR_ARG, "%s: NULL pointer", who);
+  if (S <= 0 || Hq <= 0 || Hk <= 0 || Hq > 65535 || Hk > 65535)
+    return fail(H3_ERR_SHAPE, "%s: need S > 0 and 1..65,535 heads (S=%d Hq=%d Hk=%d)", who, S, Hq, Hk);
+  if (r.pairs % 4) return fail(H3_ERR_SHAPE, "%s: the rotated dims must be a multiple of 8 (rot=%d)", who, 2 * r.pairs);
+  if (ldq % 4 || hsq % 4 || ldk % 4 || hsk % 4 || ldoq % 4 || hsoq % 4 || ldok % 4 || hsok % 4)
+    return fail(H3_ERR_SHAPE, "%s: token and head strides must be multiples of 4 elements", who);
+  if (!aligned(q, 8) || !aligned(k, 8) || !aligned(out_q, 8) || !aligned(out_k, 8) || !aligned(qw, 16) ||
+      !aligned(kw, 16))
+    return fail(H3_ERR_ARG, "%s: q / k / outputs 8-byte and norm weights 16-byte alignment required", who);
+  QkNormAxesArgs a{reinterpret_cast<const __nv_bfloat16*>(q), reinterpret_cast<const __nv_bfloat16*>(k),
+                   reinterpret_cast<__nv_bfloat16*>(out_q), reinterpret_cast<__nv_bfloat16*>(out_k),
+                   ldq, hsq, ldk, hsk, ldoq, hsoq, ldok, hsok, S, Hq, Hk, qw, kw, eps};
+  const int blocks = (int)(((long long)S + 7) / 8), groups = (Hq + Hk + 7) / 8;
+  // groups of one token over several blocks while the tokens alone leave SMs without their six resident blocks
+  int split = (num_sms() * 6 + blocks - 1) / blocks;
+  split = split < groups ? split : groups;
+  qknorm_rope_axes_kernel<<<dim3(blocks, split), 256, 0, S_(stream)>>>(a, r);
+  return check_launch(who);
 }
 
 size_t h3_attn_workspace_bytes(int S, int H) {

@@ -3,6 +3,9 @@
 Same interface as tfvideo/kernels.py of the reference (:31, :56, :76): ``idx`` (int32 [S]) is each row's
 modulation row and ``mod`` (fp32 [R, 6, D]) holds shift_msa, scale_msa, gate_msa, shift_mlp, scale_mlp, gate_mlp.
 fp32 inside, bf16 out.  ``gelu_tanh`` is the FFN activation of BASELINE's H3-shaped configs.
+
+``rope_axes`` and ``qknorm_rope_axes`` take positions over several axes (time, height, width) instead of a ready
+rotation table; ``AxialPositions`` bundles them for ``EngineBlock`` and ``StepGraph``.
 """
 
 from __future__ import annotations
@@ -15,6 +18,107 @@ from . import native as N
 def _check_rows(x: torch.Tensor, name: str) -> None:
     if x.dim() != 2 or x.dtype != torch.bfloat16 or x.stride(1) != 1:
         raise ValueError(f"{name}: expected a row-major bf16 [S, D] tensor, got {tuple(x.shape)} {x.dtype}")
+
+
+HEAD_DIM = 128
+
+
+def _check_positions(what: str, pos: torch.Tensor, dims, theta) -> tuple[tuple[int, ...], tuple[float, ...]]:
+    dims = tuple(int(d) for d in dims)
+    theta = (float(theta),) * len(dims) if isinstance(theta, (int, float)) else tuple(float(t) for t in theta)
+    if pos.dim() != 2 or pos.dtype not in N.POS_TYPES:
+        raise ValueError(f"{what}: pos must be an int32, int64 or fp32 [S, axes] tensor, got {tuple(pos.shape)} "
+                         f"{pos.dtype}")
+    if not 1 <= len(dims) <= 4 or len(dims) != pos.shape[1] or len(theta) != len(dims):
+        raise ValueError(f"{what}: pos has {pos.shape[1]} axes, dims {len(dims)}, theta {len(theta)} (1 to 4 of each)")
+    if any(d <= 0 or d % 2 for d in dims) or sum(dims) > HEAD_DIM:
+        raise ValueError(f"{what}: each axis rotates an even number of dims, together at most {HEAD_DIM}, got {dims}")
+    if any(not 0.0 < t < float("inf") for t in theta):
+        raise ValueError(f"{what}: theta must be positive and finite, got {theta}")
+    return dims, theta
+
+
+def rope_axes(pos: torch.Tensor, dims, theta=10000.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The rotation table fp32 [S, rot/2, 2, 2] ([[cos, -sin], [sin, cos]]) of ``pos`` [S, axes] (int32, int64 or
+    fp32, any strides).  Axis a rotates ``dims[a]`` dims (rot = their sum): its j-th pair turns by
+    pos[s, a] * theta^(-2j / dims[a]), formed in 64 bits; pairs of the axes one after another.  ``theta``: one number,
+    or one per axis."""
+
+    dims, theta = _check_positions("rope_axes", pos, dims, theta)
+    shape = (pos.shape[0], sum(dims) // 2, 2, 2)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.float32, device=pos.device)
+    elif tuple(out.shape) != shape or out.dtype != torch.float32 or not out.is_contiguous():
+        raise ValueError(f"rope_axes: out must be a contiguous fp32 {shape} tensor, got {tuple(out.shape)} {out.dtype}")
+    with N.on_device("rope_axes", pos, out) as stream:
+        if shape[0]:
+            N.rope_axes(N.positions(pos, dims, theta), shape[0], out, stream)
+    return out
+
+
+def qknorm_rope_axes(q: torch.Tensor, k: torch.Tensor, qw: torch.Tensor, kw: torch.Tensor, pos: torch.Tensor, dims,
+                     theta=10000.0, eps: float = 1e-5, out_q: torch.Tensor | None = None,
+                     out_k: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Per-head RMSNorm of q [S, Hq, 128] and k [S, Hk, 128] (bf16, head dim contiguous, weights ``qw`` / ``kw``
+    [128]) and the split-half rotation of their first rot dims by ``rope_axes``'s angles, in one pass with no table.
+    In place, unless ``out_q`` / ``out_k`` name other memory (apart from the inputs).  rot % 8 == 0."""
+
+    dims, theta = _check_positions("qknorm_rope_axes", pos, dims, theta)
+    oq, ok = q if out_q is None else out_q, k if out_k is None else out_k
+    for name, t, like in (("q", q, q), ("k", k, k), ("out_q", oq, q), ("out_k", ok, k)):
+        if t.dim() != 3 or t.shape[2] != HEAD_DIM or t.shape != like.shape or t.dtype != torch.bfloat16 \
+                or t.stride(2) != 1:
+            raise ValueError(f"qknorm_rope_axes: {name} must be bf16 [S, H, {HEAD_DIM}] with a contiguous head dim, got "
+                             f"{tuple(t.shape)} {t.dtype} strides {t.stride()}")
+        if t.stride(0) % 4 or t.stride(1) % 4 or t.data_ptr() % 8:
+            raise ValueError(f"qknorm_rope_axes: {name} needs 8-byte aligned rows, got strides {t.stride()}")
+    if not q.shape[0] == k.shape[0] == pos.shape[0]:
+        raise ValueError(f"qknorm_rope_axes: q has {q.shape[0]} tokens, k {k.shape[0]}, pos {pos.shape[0]}")
+    if sum(dims) % 8:
+        raise ValueError(f"qknorm_rope_axes: the rotated dims must be a multiple of 8, got {dims}")
+    if qw.numel() != HEAD_DIM or kw.numel() != HEAD_DIM:
+        raise ValueError(f"qknorm_rope_axes: norm weights have {HEAD_DIM} elements")
+    qw, kw = _norm_weight(qw), _norm_weight(kw)
+    with N.on_device("qknorm_rope_axes", q, k, oq, ok, qw, kw, pos) as stream:
+        if q.shape[0] and q.shape[1] and k.shape[1]:
+            N.qknorm_rope_axes(q, k, qw, kw, N.positions(pos, dims, theta), eps, oq, ok, stream)
+        elif q.shape[0] and q.shape[1] + k.shape[1]:
+            raise ValueError("qknorm_rope_axes: q and k need at least one head each")
+    return oq, ok
+
+
+def _norm_weight(w: torch.Tensor) -> torch.Tensor:
+    w = w.reshape(-1).float().contiguous()
+    return w if w.data_ptr() % 16 == 0 else w.clone()
+
+
+class AxialPositions:
+    """Positions of a packed sequence over several axes, in place of a rotation table: ``pos`` [S, axes], the dims
+    each axis rotates and theta, as for ``rope_axes``.  ``EngineBlock`` takes one as its ``rope_freqs``."""
+
+    def __init__(self, pos: torch.Tensor, dims, theta=10000.0):
+        self.dims, self.theta = _check_positions("AxialPositions", pos, dims, theta)
+        self.pos = pos
+
+    def __len__(self) -> int:
+        return self.pos.shape[0]
+
+    @property
+    def rot(self) -> int:
+        return sum(self.dims)
+
+    def rows(self, a: int, b: int) -> "AxialPositions":
+        """The positions of tokens [a, b) (a view)."""
+
+        return AxialPositions(self.pos[a:b], self.dims, self.theta)
+
+    def to(self, device) -> "AxialPositions":
+        return AxialPositions(self.pos.to(device), self.dims, self.theta)
+
+    def table(self) -> torch.Tensor:
+        """ComfyUI's rope_freqs of these positions: fp32 [1, S, 1, rot/2, 2, 2]."""
+
+        return rope_axes(self.pos, self.dims, self.theta)[None, :, None]
 
 
 def norm_mod(x: torch.Tensor, w: torch.Tensor, mod: torch.Tensor, part: int, idx: torch.Tensor, eps: float,

@@ -33,6 +33,11 @@ class H3PeerCopy(C.Structure):
     _fields_ = [("src", vp), ("dst", vp), ("bytes", sz)]
 
 
+class H3Positions(C.Structure):
+    _fields_ = [("pos", vp), ("type", i32), ("ld", i64), ("axis_stride", i64), ("axes", i32), ("dims", i32 * 4),
+                ("theta", C.c_double * 4)]
+
+
 # name -> argtypes (restype int unless noted)
 _SIGS = {
     "h3_version": [],
@@ -50,6 +55,9 @@ _SIGS = {
     "h3_modulation": [vp, i32, i32, vp, vp, i32, vp, vp],
     "h3_gemm_nvfp4": [vp, vp, vp, vp, vp, f32, vp, i32, i32, i32, C.POINTER(H3Epilogue), vp],
     "h3_qknorm_rope": [vp, vp, i64, i32, i32, i32, vp, vp, vp, f32, vp],
+    "h3_rope_axes": [C.POINTER(H3Positions), i32, vp, vp],
+    "h3_qknorm_rope_axes": [vp, i64, i64, vp, i64, i64, i32, i32, i32, vp, vp, C.POINTER(H3Positions), f32, vp, i64,
+                            i64, vp, i64, i64, vp],
     "h3_attn_workspace_bytes": ([i32, i32], sz),
     "h3_attn_fp8": [vp, vp, vp, i64, i64, i32, i32, vp, i64, vp, sz, vp],
     "h3_attn_fp8_noalloc": [vp, vp, vp, i64, i64, i32, i32, vp, i64, vp],
@@ -132,6 +140,27 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return t.data_ptr()
 
 
+class on_device:
+    """The device all the given tensors are on, made current for a launch, and its current stream:
+    ``with on_device(what, a, b, ...) as stream``.  ValueError when one is not a CUDA tensor or they are apart."""
+
+    def __init__(self, what: str, *tensors: torch.Tensor):
+        dev = tensors[0].device
+        if any(t.device != dev for t in tensors) or dev.type != "cuda":
+            raise ValueError(f"{what}: all tensors must be on one CUDA device, got "
+                             f"{', '.join(sorted({str(t.device) for t in tensors}))}")
+        self._guard = torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else None
+
+    def __enter__(self) -> int:
+        if self._guard is not None:
+            self._guard.__enter__()
+        return stream()
+
+    def __exit__(self, *exc) -> None:
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
+
+
 def sf_tiled_bytes(rows: int, cols: int) -> int:
     return int(lib().h3_sf_tiled_bytes(rows, cols))
 
@@ -212,6 +241,34 @@ def qknorm_rope(q, k, ld, S, H, rot, qw, kw, rope, eps) -> None:
     _count(1)
     check(lib().h3_qknorm_rope(ptr(q), ptr(k), ld, S, H, rot, ptr(qw), ptr(kw), ptr(rope), eps, stream()),
           "h3_qknorm_rope")
+
+
+POS_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+
+
+def positions(pos: torch.Tensor, dims, theta) -> H3Positions:
+    """The H3Positions of a [S, axes] position tensor (``theta``: one per axis)."""
+
+    p = H3Positions(pos=pos.data_ptr(), type=POS_TYPES[pos.dtype], ld=pos.stride(0), axis_stride=pos.stride(1),
+                    axes=len(dims))
+    p.dims[:len(dims)] = dims
+    p.theta[:len(dims)] = theta
+    return p
+
+
+def rope_axes(pos: H3Positions, S: int, out: torch.Tensor, stream_handle: int) -> None:
+    _count(1)
+    check(lib().h3_rope_axes(C.byref(pos), S, ptr(out), stream_handle), "h3_rope_axes")
+
+
+def qknorm_rope_axes(q, k, qw, kw, pos: H3Positions, eps, out_q, out_k, stream_handle: int) -> None:
+    """q, out_q [S, Hq, 128], k, out_k [S, Hk, 128]."""
+
+    _count(1)
+    check(lib().h3_qknorm_rope_axes(ptr(q), q.stride(0), q.stride(1), ptr(k), k.stride(0), k.stride(1), q.shape[0],
+                                    q.shape[1], k.shape[1], ptr(qw), ptr(kw), C.byref(pos), eps, ptr(out_q),
+                                    out_q.stride(0), out_q.stride(1), ptr(out_k), out_k.stride(0), out_k.stride(1),
+                                    stream_handle), "h3_qknorm_rope_axes")
 
 
 def attn_fp8(q, k, v, ld, hstride, S, H, out, ldo, workspace) -> None:

@@ -1,0 +1,92 @@
+"""Argument checks of the packed-batch operators (positions, span masks, adapters): every refusal comes before any CUDA
+call, so they run without a GPU, through the Python entry points and through the C ABI."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+FAKE = 1 << 20   # an aligned address that is never touched
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from tfvideo import native
+    if not native.LIB_PATH.exists():
+        from build import build
+        build()
+    return native.lib()
+
+
+def _pos(**kw):
+    from tfvideo import native as N
+
+    d = dict(pos=FAKE, type=0, ld=3, axis_stride=1, axes=3, dims=(44, 42, 42), theta=(1e4, 1e4, 1e4))
+    d.update(kw)
+    p = N.H3Positions(pos=d["pos"], type=d["type"], ld=d["ld"], axis_stride=d["axis_stride"], axes=d["axes"])
+    for i, v in enumerate(d["dims"]):
+        p.dims[i] = v
+    for i, v in enumerate(d["theta"]):
+        p.theta[i] = v
+    return p
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(pos=None), "NULL"), (dict(type=3), "type"), (dict(pos=FAKE + 2), "misaligned"), (dict(axes=0), "axes"),
+    (dict(axes=5), "axes"), (dict(dims=(44, 42, 41)), "even"), (dict(dims=(44, 0, 42)), "even"),
+    (dict(dims=(64, 64, 2)), "even"), (dict(theta=(1e4, 0.0, 1e4)), "theta"),
+    (dict(theta=(1e4, float("inf"), 1e4)), "theta"), (dict(theta=(1e4, float("nan"), 1e4)), "theta"),
+])
+def test_positions_refused_by_the_library(lib, kw, word):
+    from tfvideo import native as N
+
+    assert lib.h3_rope_axes(ctypes.byref(_pos(**kw)), 10, FAKE, None) < 0 and word in N.last_error()
+
+
+def test_rope_entry_points_check_their_arguments(lib):
+    from tfvideo import native as N
+
+    p = ctypes.byref(_pos())
+    assert lib.h3_rope_axes(None, 10, FAKE, None) == -1
+    assert lib.h3_rope_axes(p, 0, FAKE, None) == -2 and "S" in N.last_error()
+    assert lib.h3_rope_axes(p, 10, FAKE + 4, None) == -1 and "aligned" in N.last_error()
+
+    def qk(q=FAKE, ldq=384, S=10, Hq=1, Hk=1, qw=FAKE, pos=p, oq=FAKE, hsq=128):
+        return lib.h3_qknorm_rope_axes(q, ldq, hsq, FAKE, 384, 128, S, Hq, Hk, qw, FAKE, pos, 1e-5, oq, 384, 128, FAKE,
+                                       384, 128, None)
+
+    assert qk(q=None) == -1 and qk(oq=None) == -1
+    assert qk(S=0) == -2 and qk(Hq=0) == -2 and qk(Hk=0) == -2
+    assert qk(ldq=386) == -2 and "strides" in N.last_error()
+    assert qk(q=FAKE + 4) == -1 and qk(qw=FAKE + 8) == -1
+    assert qk(pos=ctypes.byref(_pos(dims=(44, 42, 40)))) == -2 and "multiple of 8" in N.last_error()   # rot 126
+
+
+def test_rope_functions_refuse_bad_arguments():
+    from tfvideo import kernels as K
+
+    pos = torch.zeros((10, 3), dtype=torch.int32)
+    for bad, dims, theta in ((pos[0], (32, 32, 32), 1e4), (pos.to(torch.int16), (32, 32, 32), 1e4),
+                             (pos.double(), (32, 32, 32), 1e4), (pos, (32, 32), 1e4), (pos, (32, 31, 33), 1e4),
+                             (pos, (64, 64, 64), 1e4), (pos, (32, 32, 32), 0.0), (pos, (32, 32, 32), (1e4, 1e4)),
+                             (torch.zeros((10, 5), dtype=torch.int32), (8,) * 5, 1e4), (pos, (32, -2, 32), 1e4)):
+        with pytest.raises(ValueError):
+            K.rope_axes(bad, dims, theta)
+        with pytest.raises(ValueError):
+            K.AxialPositions(bad, dims, theta)
+    with pytest.raises(ValueError, match="CUDA device"):
+        K.rope_axes(pos, (32, 32, 32))
+    with pytest.raises(ValueError, match="out"):
+        K.rope_axes(pos, (32, 32, 32), out=torch.empty((10, 48, 2, 2), dtype=torch.float64))
+    q = torch.zeros((10, 4, 128), dtype=torch.bfloat16)
+    w = torch.ones(128)
+    ok = dict(q=q, k=q, qw=w, kw=w, pos=pos, dims=(32, 32, 32))
+    for change in (dict(q=q.float()), dict(q=q[:, :, :64]), dict(q=q[0]), dict(k=q[:9]), dict(pos=pos[:9]),
+                   dict(dims=(32, 32, 30)), dict(qw=w[:64]), dict(out_q=q[:, :2]), dict(out_k=q.float()),
+                   dict(q=torch.zeros((10, 128, 4), dtype=torch.bfloat16).transpose(1, 2)),
+                   dict(q=torch.zeros(10 * 4 * 130, dtype=torch.bfloat16).as_strided((10, 4, 128), (520, 130, 1))),
+                   dict()):                                                  # the last: CPU tensors
+        with pytest.raises(ValueError):
+            K.qknorm_rope_axes(**{**ok, **change})
