@@ -221,6 +221,18 @@ int h3_attn_fp8_peers(const void* q, const void* k, const void* v, long long ld,
                       const int* kv_ptr, const int* kv_idx, void* const* peer, int ranks, int rank, long long ldo,
                       void* workspace, size_t workspace_bytes, void* stream);
 
+/* bf16 attention under per-token key spans: token i attends to the keys [span_lo[i], span_hi[i]) of its head, softmax
+ * over those alone (device int32 [S], clipped to [0, S); both NULL: every key).  Packed requests, a prefix with causal
+ * or frame-causal tokens behind it and windows are all spans.  A token with an empty span gets zeros.  Keys and values
+ * outside a token's span never reach its row, whatever they hold (NaN and infinities included).  Hq query heads share
+ * Hk key heads in groups of Hq / Hk.  q, k and v are bf16 views with their own token and head strides (multiples of 8
+ * elements, 16-byte aligned), element (t, h, d) at t * ld + h * hs + d; out (t, h, d) at out + t * ldo + h * 128 + d.
+ * scores scaled by 1 / sqrt(128).  No workspace.  S <= 262,144.  The reference's backends (tfvideo/attention.py:29-54)
+ * attend to the whole sequence. */
+int h3_attn_bf16(const void* q, long long ldq, long long hsq, const void* k, long long ldk, long long hsk,
+                 const void* v, long long ldv, long long hsv, int S, int Hq, int Hk, const int* span_lo,
+                 const int* span_hi, void* out, long long ldo, void* stream);
+
 /* The same attention as h3_attn_fp8 for callers that cannot allocate device memory -- for example code running
  * inside a host framework that owns every device allocation (ComfyUI records and replays a block's allocations under
  * its dynamic-VRAM mode), or a plugin handed only input and output buffers.  Its scratch is a fixed 64 MiB device

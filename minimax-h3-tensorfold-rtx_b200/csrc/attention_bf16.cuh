@@ -1,0 +1,492 @@
+// bf16 flash attention for sm_100a in which token i sees the keys [lo_i, hi_i): packed requests (documents), a prefix
+// with causal or frame-causal tokens behind it, windows.  QK^T and PV are tcgen05 kind::f16 MMAs with S, P and O in
+// TMEM; Q, K and V are read by TMA straight from the caller's rows (no preparation pass), key heads may be shared by
+// groups of query heads.  No counterpart in the reference, whose backends attend to the whole sequence
+// (tfvideo/attention.py:29-54).
+//
+// o_i = sum_j p_ij v_j / sum_j p_ij, p_ij = exp(q_i k_j / sqrt(128) - m_i), one pass over the keys with the running
+// maximum m and sum l in 32 bits.  A row without keys gives zeros.  P is rounded to bf16 for the PV MMA (both operands
+// of that MMA have one type, V's); l sums the unrounded P.
+//
+// One CTA = two 128-row query tiles (A, B) of one head over the same 128-key steps.  TMEM: S_A, S_B, O_A, O_B of 128
+// columns each, P written over S.  Warps 0-3: softmax of A, 4-7: of B, a thread per query row with its 128 scores in
+// registers; warp 8: TMA; warp 9: all MMAs, alternating A and B, so that one tile's MMAs run under the other's
+// softmax; warp 10: guards masked V rows (below).  A step of both tiles is 4 x 512 cycles of MMA at the bf16 rate and
+// 2 x 1,024 cycles of exponentials at 16 a cycle, of which 5 pairs in 16 go to the FMA pipe (exp2_poly_clamped).
+//
+// Masked keys.  Steps run over the union of the CTA's spans and start at its first key, so documents begin on a step.
+// Scores of masked keys become -inf before the maximum, whatever K holds there.  V needs more: 0 x NaN is NaN inside
+// the MMA, and another request's rows or the memory behind the last one may hold anything.  In a step that hides some
+// key from some row, warp 10 sets non-finite elements of the V tile to zero and notes the step; the epilogue adds
+// them back, from global memory, to the rows that do see them.
+#pragma once
+
+#include <climits>
+
+#include "attention.cuh"
+#include "common.cuh"
+#include "h3b200.h"
+
+namespace h3 {
+
+// warp-wide: one tile of a 3-D tensor map into shared memory, completing on `bar`
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t.reg .b32 rx;\n\t" H3_ELECT
+      "@e cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+      "[%5];\n\t}" ::"r"(smem_u32(smem_dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+// warp-wide: D[tmem] (+)= A[smem] x B[smem], bf16 x bf16 -> fp32
+__device__ __forceinline__ void mma_bf16_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b32 rx;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t" H3_ELECT
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// warp-wide: A from TMEM (lane = row, two consecutive K elements a column)
+__device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b32 rx;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t" H3_ELECT
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// kind::f16 with bf16 operands and an fp32 accumulator: C format F32 = 1 in bits 4-5, A / B format BF16 = 1 in bits
+// 7-9 / 10-12, bit 16 = B is MN-major (its N elements contiguous in shared memory).
+__host__ __device__ constexpr uint32_t idesc_bf16(int M, int N, bool b_mn_major) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(N >> 3) << 17) |
+         ((uint32_t)(M >> 4) << 24);
+}
+
+struct AttnBf16Args {
+  __nv_bfloat16* out;        // element (t, h, d) at out + t * ldo + h * 128 + d
+  long long ldo;
+  const __nv_bfloat16* v;    // element (t, h, d) at v + t * ldv + h * hsv + d (the epilogue's repair of masked steps)
+  long long ldv, hsv;
+  const int* lo;             // spans, or NULL: every key
+  const int* hi;
+  int S, group;              // group: query heads that share a key head
+};
+
+struct AttnBf16Smem {
+  static constexpr int SUB = 128 * 128;            // 128 rows x 64 dims of bf16 (128-byte rows, 128-byte swizzle)
+  static constexpr int TILE = 2 * SUB;             // 128 rows x 128 dims
+  static constexpr int KST = 2, VST = 3;           // ring depths
+  static constexpr int Q_OFF = 0;                  // tiles A, B
+  static constexpr int K_OFF = 2 * TILE;
+  static constexpr int V_OFF = K_OFF + KST * TILE;
+  static constexpr int BAR_OFF = V_OFF + VST * TILE;
+  static constexpr int MAX_S = 262144;
+  static constexpr int BAD_WORDS = MAX_S / 128 / 32 + 1;   // a bit per step whose V tile held masked non-finite values
+  static constexpr int BAD_OFF = BAR_OFF + 256;
+  static constexpr int RED_OFF = BAD_OFF + (BAD_WORDS + 3) / 4 * 16;   // span reductions: 8 warps x 4 ints
+  static constexpr int TOTAL = RED_OFF + 128 + 16 + 1024;
+};
+static_assert(AttnBf16Smem::TOTAL <= 232448, "shared memory of one SM");
+
+constexpr int kAttnBf16Threads = 352;
+// Lag of the running maximum (log2 units) before O and l are rescaled: P <= 2^8 is far inside bf16's range, and its
+// relative rounding does not depend on the factor.
+constexpr float kTauBf16 = 8.0f;
+// pairs of each 32-key chunk whose exp2 runs on the FMA pipe (bit i: keys 2i, 2i + 1)
+constexpr uint32_t kPolyPairsBf16 = 0x2492u;
+
+__device__ __forceinline__ float max_nan(float a, float b) {   // NaN when either is
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1u); }
+
+// 32 scores of one row -> 16 words of bf16 P = exp2(s * scale + nbias) (key 2w in the low half of word w); l2 += the
+// unrounded P.  MASKED: every exponential on the MUFU, whose exp2(-inf) is exactly 0 (the polynomial's is 2^-126).
+template <bool MASKED>
+__device__ __forceinline__ void p_chunk_bf16(const uint32_t (&s)[32], uint64_t scale2, uint64_t nbias2,
+                                             uint32_t (&pw)[16], uint64_t& l2a, uint64_t& l2b) {
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    const uint64_t x = fma2(f32x2_pack(__uint_as_float(s[2 * w]), __uint_as_float(s[2 * w + 1])), scale2, nbias2);
+    uint64_t y;
+    if (!MASKED && ((kPolyPairsBf16 >> w) & 1u)) {
+      float a, b;
+      f32x2_unpack(x, a, b);   // a NaN score stays NaN through the polynomial's clamp
+      y = exp2_poly_clamped(f32x2_pack(max_nan(a, -126.0f), max_nan(b, -126.0f)));
+    } else {
+      y = exp2_mufu_pair(x);
+    }
+    if (w & 1) l2b = add2(l2b, y);
+    else l2a = add2(l2a, y);
+    float a, b;
+    f32x2_unpack(y, a, b);
+    pw[w] = pack_bf16(a, b);
+  }
+}
+
+__global__ void __launch_bounds__(kAttnBf16Threads, 1)
+    attn_bf16_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                     const __grid_constant__ CUtensorMap tmV, const AttnBf16Args p) {
+  using L = AttnBf16Smem;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
+  uint64_t* q_full = bars;
+  uint64_t* k_full = bars + 1;             // [KST]
+  uint64_t* k_empty = k_full + L::KST;
+  uint64_t* v_full = k_empty + L::KST;     // [VST]
+  uint64_t* v_ok = v_full + L::VST;        // [VST]: landed, and its masked non-finite values are zero
+  uint64_t* v_empty = v_ok + L::VST;
+  uint64_t* s_full = v_empty + L::VST;     // [tile]
+  uint64_t* p_full = s_full + 2;           // [tile][half]: P of keys 0-63 / 64-127 written, by four warps
+  uint64_t* o_done = p_full + 4;           // [tile]
+  uint64_t* drained = o_done + 2;
+  uint32_t* bad = reinterpret_cast<uint32_t*>(smem + L::BAD_OFF);
+  int* red = reinterpret_cast<int*>(smem + L::RED_OFF);      // [warp][lo min, lo max, hi min, hi max]
+  int* any_bad = red + 32;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(red + 33);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = blockIdx.y, hk = h / p.group;
+  // the last tiles first: under causal spans they have the most keys
+  const int q0 = (gridDim.x - 1 - blockIdx.x) * 256;
+
+  // ---- this thread's span (softmax warps: a thread per query row) and the spans' ranges over each query tile
+  int lo = 0, hi = 0;
+  if (warp < 8) {
+    const int query = q0 + threadIdx.x;
+    if (query < p.S) {
+      lo = p.lo ? max(p.lo[query], 0) : 0;
+      hi = p.hi ? min(p.hi[query], p.S) : p.S;
+    }
+    const bool live = lo < hi;
+    const int a = __reduce_min_sync(~0u, live ? lo : INT_MAX), b = __reduce_max_sync(~0u, live ? lo : -1);
+    const int c = __reduce_min_sync(~0u, live ? hi : INT_MAX), d = __reduce_max_sync(~0u, live ? hi : -1);
+    if (lane == 0) {
+      red[warp * 4] = a;
+      red[warp * 4 + 1] = b;
+      red[warp * 4 + 2] = c;
+      red[warp * 4 + 3] = d;
+    }
+  }
+  for (int i = threadIdx.x; i < L::BAD_WORDS; i += kAttnBf16Threads) bad[i] = 0;
+  if (threadIdx.x == 0) {
+    *any_bad = 0;
+    mbar_init(q_full, 1);
+    for (int s = 0; s < L::KST; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+    }
+    for (int s = 0; s < L::VST; ++s) {
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_ok[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[2 * t], 4);
+      mbar_init(&p_full[2 * t + 1], 4);
+      mbar_init(&o_done[t], 1);
+    }
+    mbar_init(drained, 1);
+    fence_barrier_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  int lo_min[2], lo_max[2], hi_min[2], hi_max[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    lo_min[t] = hi_min[t] = INT_MAX;
+    lo_max[t] = hi_max[t] = -1;
+    for (int w = 4 * t; w < 4 * t + 4; ++w) {
+      lo_min[t] = min(lo_min[t], red[4 * w]);
+      lo_max[t] = max(lo_max[t], red[4 * w + 1]);
+      hi_min[t] = min(hi_min[t], red[4 * w + 2]);
+      hi_max[t] = max(hi_max[t], red[4 * w + 3]);
+    }
+  }
+  // key steps: step j covers keys base + 128 j ..; tile t takes part in steps [j0[t], j1[t])
+  const int base = min(lo_min[0], lo_min[1]);
+  const int kend = max(hi_max[0], hi_max[1]);
+  const int steps = kend > 0 ? (kend - base + 127) >> 7 : 0;
+  int j0[2], j1[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    j0[t] = hi_max[t] > 0 ? (lo_min[t] - base) >> 7 : 0;
+    j1[t] = hi_max[t] > 0 ? (hi_max[t] - base + 127) >> 7 : 0;
+  }
+  // whether step j hides a key from some live row of tile t
+  auto hides = [&](int t, int j) {
+    const int kb = base + 128 * j;
+    return lo_max[t] > kb || hi_min[t] < kb + 128;
+  };
+
+  if (warp == 8) {
+    // ------------------------------------------------------------------ TMA
+    if (lane == 0) {
+      prefetch_tmap(&tmQ);
+      prefetch_tmap(&tmK);
+      prefetch_tmap(&tmV);
+    }
+    auto load = [&](int off, const CUtensorMap* map, int row, int head, uint64_t* bar) {
+      tma_load_3d(smem + off, map, 0, row, head, bar);
+      tma_load_3d(smem + off + L::SUB, map, 64, row, head, bar);
+    };
+    int nk = 0, nv = 0;   // loads issued
+    if (steps > 0) {
+      mbar_arrive_expect_tx(q_full, 2 * L::TILE);
+      load(L::Q_OFF, &tmQ, q0, h, q_full);
+      load(L::Q_OFF + L::TILE, &tmQ, q0 + 128, h, q_full);
+    }
+    for (int j = 0; j < steps; ++j) {
+      const int ks = j % L::KST, vs = j % L::VST;
+      if (!__all_sync(~0u, mbar_wait(&k_empty[ks], ((j / L::KST) & 1) ^ 1, 301))) break;
+      mbar_arrive_expect_tx(&k_full[ks], L::TILE);
+      load(L::K_OFF + ks * L::TILE, &tmK, base + 128 * j, hk, &k_full[ks]);
+      ++nk;
+      if (!__all_sync(~0u, mbar_wait(&v_empty[vs], ((j / L::VST) & 1) ^ 1, 302))) break;
+      mbar_arrive_expect_tx(&v_full[vs], L::TILE);
+      load(L::V_OFF + vs * L::TILE, &tmV, base + 128 * j, hk, &v_full[vs]);
+      ++nv;
+    }
+    // nothing may still be landing in this CTA's memory when it ends, after a wait that gave up included
+    if (steps > 0) mbar_wait(q_full, 0, 303);
+    for (int j = max(nk - L::KST, 0); j < nk; ++j) mbar_wait(&k_full[j % L::KST], (j / L::KST) & 1, 303);
+    for (int j = max(nv - L::VST, 0); j < nv; ++j) mbar_wait(&v_full[j % L::VST], (j / L::VST) & 1, 303);
+  } else if (warp == 9) {
+    // ------------------------------------------------------------------ MMA
+    constexpr uint32_t idesc_s = idesc_bf16(128, 128, false), idesc_o = idesc_bf16(128, 128, true);
+    auto issue_s = [&](int t, int j) {   // S_t = Q_t K_j^T: 8 MMAs over 16 dims each
+      const uint32_t qa = smem_u32(smem + L::Q_OFF + t * L::TILE);
+      const uint32_t ka = smem_u32(smem + L::K_OFF + (j % L::KST) * L::TILE);
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) {
+        const uint32_t off = (kk >> 2) * L::SUB + (kk & 3) * 32;
+        mma_bf16_ss(tmem + t * 128, sdesc_kmajor_sw128(qa + off), sdesc_kmajor_sw128(ka + off), idesc_s, kk != 0);
+      }
+    };
+    auto issue_pv = [&](int t, int j, int half) {   // O_t (+)= P_t V_j over 64 keys: 4 MMAs over 16 keys each
+      // V rows are keys (the K dimension), 64 dims contiguous: MN-major, 8-key groups 1,024 bytes apart, the two
+      // 64-dim halves SUB apart
+      const uint32_t va = smem_u32(smem + L::V_OFF + (j % L::VST) * L::TILE);
+#pragma unroll
+      for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+        mma_bf16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, make_sdesc(va + kk * 2048, L::SUB, 1024, kLayoutSW128),
+                    idesc_o, j != j0[t] || kk != 0);
+    };
+    bool ok = steps > 0 && __all_sync(~0u, mbar_wait(q_full, 0, 310));
+    for (int j = -1; ok && j < steps; ++j) {
+      if (j >= 0 && !(ok = __all_sync(~0u, mbar_wait(&v_ok[j % L::VST], (j / L::VST) & 1, 311)))) break;
+      const int n = j + 1;
+      if (n < steps && !(ok = __all_sync(~0u, mbar_wait(&k_full[n % L::KST], (n / L::KST) & 1, 312)))) break;
+      tc_fence_after();
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (ok && j >= j0[t] && j < j1[t]) {
+          const uint32_t ph = (j - j0[t]) & 1;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if (ok && (ok = __all_sync(~0u, mbar_wait(&p_full[2 * t + half], ph, 313 + t)))) {
+              tc_fence_after();
+              issue_pv(t, j, half);
+            }
+          }
+          if (ok && j + 1 == j1[t]) tc_commit(&o_done[t]);
+        }
+        if (ok && n >= j0[t] && n < j1[t]) {   // after PV_t(j) in issue order: P_t is read before S_t overwrites it
+          issue_s(t, n);
+          tc_commit(&s_full[t]);
+        }
+      }
+      if (!ok) break;
+      if (j >= 0) tc_commit(&v_empty[j % L::VST]);
+      if (n < steps) tc_commit(&k_empty[n % L::KST]);
+    }
+    if (steps > 0) {   // every MMA has left the tensor core before TMEM and shared memory are given back
+      tc_commit(drained);
+      mbar_wait(drained, 0, 315);
+    }
+  } else if (warp == 10) {
+    // ------------------------------------------------------------------ V guard
+    for (int j = 0; j < steps; ++j) {
+      const int vs = j % L::VST;
+      if (!__all_sync(~0u, mbar_wait(&v_full[vs], (j / L::VST) & 1, 320))) break;
+      if ((j >= j0[0] && j < j1[0] && hides(0, j)) || (j >= j0[1] && j < j1[1] && hides(1, j))) {
+        uint4* vt = reinterpret_cast<uint4*>(smem + L::V_OFF + vs * L::TILE);
+        bool hit = false;
+#pragma unroll 4
+        for (int i = lane; i < L::TILE / 16; i += 32) {
+          uint4 u = vt[i];
+          uint32_t* w = &u.x;
+          bool mine = false;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {   // exponent bits all set: infinity or NaN
+            if ((w[e] & 0x7F80u) == 0x7F80u) { w[e] &= 0xFFFF0000u; mine = true; }
+            if ((w[e] & 0x7F800000u) == 0x7F800000u) { w[e] &= 0x0000FFFFu; mine = true; }
+          }
+          if (mine) vt[i] = u;
+          hit |= mine;
+        }
+        if (__any_sync(~0u, hit)) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMA reads these writes
+          if (lane == 0) {
+            bad[j >> 5] |= 1u << (j & 31);
+            *any_bad = 1;
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&v_ok[vs]);
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax: one thread per query row
+    const int t = warp >> 2;
+    const int first = t ? j0[1] : j0[0], last = t ? j1[1] : j1[0];
+    const int lo_top = t ? lo_max[1] : lo_max[0], hi_low = t ? hi_min[1] : hi_min[0];
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_col = tmem + lane_off + t * 128, o_col = tmem + lane_off + 256 + t * 128;
+    const float scale = kLog2e * 0.08838834764831845f;   // log2(e) / sqrt(128)
+    const uint64_t scale2 = f32x2_splat(scale);
+    const bool live = lo < hi;
+    float m_used = -INFINITY;
+    uint64_t l2a = 0, l2b = 0;
+    bool ok = true;
+    for (int j = first; j < last; ++j) {
+      const int i = j - first, kb = base + 128 * j;
+      ok = __all_sync(~0u, mbar_wait(&s_full[t], i & 1, 330 + t));
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(s_col + 32 * c, s[c]);
+      tmem_ld_wait();
+      const bool masked = lo_top > kb || hi_low < kb + 128;
+      if (masked && live) {   // (a row without keys takes the scores as they are and is zeroed at the end)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t vis = bits_below(hi - kb - 32 * c) & ~bits_below(lo - kb - 32 * c);
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!((vis >> e) & 1u)) s[c][e] = __float_as_uint(-INFINITY);
+        }
+      }
+      const float mx = fmaxf(max_chunk(s[1], max_chunk(s[0], -INFINITY)), max_chunk(s[3], max_chunk(s[2], -INFINITY)));
+      const float mnew = mx * scale;
+      const bool need = mnew > m_used + kTauBf16 || (m_used == -INFINITY && mnew > m_used);
+      float alpha = 1.0f;
+      if (need) {
+        alpha = m_used == -INFINITY ? 0.0f : ex2(m_used - mnew);
+        m_used = mnew;
+        const uint64_t a2 = f32x2_splat(alpha);
+        l2a = mul2(l2a, a2);
+        l2b = mul2(l2b, a2);
+      }
+      // O holds the PV of every earlier step here: those MMAs were issued before S of this step by the same thread,
+      // and s_full counts everything issued before its commit
+      if (i > 0 && __any_sync(~0u, need)) {
+#pragma unroll 1
+        for (int c = 0; c < 8; ++c) {
+          uint32_t o[16];
+          tmem_ld16(o_col + 16 * c, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+          tmem_st16(o_col + 16 * c, o);
+        }
+      }
+      const uint64_t nbias2 = f32x2_splat(m_used == -INFINITY ? 0.0f : -m_used);   // no key yet: P = exp2(-inf) = 0
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t pw[16];
+        if (masked) p_chunk_bf16<true>(s[c], scale2, nbias2, pw, l2a, l2b);
+        else p_chunk_bf16<false>(s[c], scale2, nbias2, pw, l2a, l2b);
+        tmem_st16(s_col + 16 * c, pw);
+        if (c & 1) {
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[2 * t + (c >> 1)]);
+        }
+      }
+    }
+    // ---- epilogue: O / l -> bf16, this thread's row
+    const bool any = last > first;
+    // (the last v_ok: every note of the V guard is visible)
+    if (any)
+      ok = __all_sync(~0u, ok && mbar_wait(&o_done[t], 0, 332) &&
+                               mbar_wait(&v_ok[(steps - 1) % L::VST], ((steps - 1) / L::VST) & 1, 333));
+    if (ok) {
+      tc_fence_after();
+      float la, lb, lc, ld;
+      f32x2_unpack(l2a, la, lb);
+      f32x2_unpack(l2b, lc, ld);
+      const float inv_l = 1.0f / ((la + lb) + (lc + ld));
+      const int query = q0 + threadIdx.x;
+      const bool repair = any && *(volatile int*)any_bad != 0;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t o[32];
+        if (any) {
+          tmem_ld32(o_col + 32 * c, o);
+          tmem_ld_wait();
+        }
+        float f[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) f[e] = live ? __uint_as_float(o[e]) * inv_l : 0.0f;
+        if (repair && live) {   // non-finite V elements this row does see
+          for (int j = first; j < last; ++j) {
+            if (!((bad[j >> 5] >> (j & 31)) & 1u)) continue;
+            const int kb = base + 128 * j;
+            for (int key = max(kb, lo); key < min(kb + 128, hi); ++key) {
+              const __nv_bfloat16* vr = p.v + (long long)key * p.ldv + (long long)hk * p.hsv + 32 * c;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const float x = __bfloat162float(vr[e]);
+                if (!isfinite(x)) f[e] += x;
+              }
+            }
+          }
+        }
+        if (query < p.S) {
+          uint4* d4 = reinterpret_cast<uint4*>(p.out + (long long)query * p.ldo + (long long)h * 128 + 32 * c);
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4)
+            d4[q4] = make_uint4(pack_bf16(f[8 * q4], f[8 * q4 + 1]), pack_bf16(f[8 * q4 + 2], f[8 * q4 + 3]),
+                                pack_bf16(f[8 * q4 + 4], f[8 * q4 + 5]), pack_bf16(f[8 * q4 + 6], f[8 * q4 + 7]));
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace h3

@@ -10,6 +10,7 @@
 #include <string>
 
 #include "attention.cuh"
+#include "attention_bf16.cuh"
 #include "elementwise.cuh"
 #include "gemm_nvfp4.cuh"
 #include "h3b200.h"
@@ -75,6 +76,25 @@ int make_map_u8(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows
   return H3_OK;
 }
 
+// bf16 [heads, tokens, cols] (token stride ld, head stride hs, in elements) read in boxes of 64 columns x box_rows
+// tokens of one head, 128-byte swizzle; tokens and columns past the ends read as zeros, and are not stored.
+int make_map_bf16(CUtensorMap* map, const void* base, uint64_t cols, uint64_t tokens, uint64_t heads, long long ld,
+                  long long hs, uint32_t box_rows, const char* what) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(H3_ERR_CUDA, "%s: cuTensorMapEncodeTiled unavailable from the driver", what);
+  cuuint64_t dims[3] = {cols, tokens, heads};
+  // (the stride of a dimension of one entry is never used, but has to be a valid one)
+  const cuuint64_t row = (cols * 2 + 15) / 16 * 16;
+  cuuint64_t strides[2] = {tokens > 1 ? (cuuint64_t)ld * 2 : row, heads > 1 ? (cuuint64_t)hs * 2 : row};
+  cuuint32_t box[3] = {64, box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(H3_ERR_CUDA, "%s: cuTensorMapEncodeTiled (bf16) failed (%d)", what, (int)r);
+  return H3_OK;
+}
+
 // A tiled scale buffer (h3_sf_tiled_bytes layout) as rows of 2048 bytes -- the scales of 128 matrix rows for one
 // 256-element K tile, contiguous -- read one row per box (256 eight-byte elements, no swizzle).
 int make_map_sf_rows(CUtensorMap* map, const void* base, uint64_t rows, const char* what) {
@@ -104,6 +124,7 @@ int smem_optin(K kernel, int bytes, unsigned* done_mask, const char* what) {
 }
 
 unsigned g_optin_attn[2] = {0, 0};   // [NT - 1]
+unsigned g_optin_attn_bf16 = 0;
 #ifndef H3_GEMM_PAIR
 #define H3_GEMM_PAIR 0
 #endif
@@ -726,6 +747,37 @@ int h3_attn_fp8_sparse(const void* q, const void* k, const void* v, long long ld
   if (!aligned(kv_ptr, 4) || !aligned(kv_idx, 4)) return fail(H3_ERR_ARG, "h3_attn_fp8_sparse: misaligned tile list");
   return attn_run("h3_attn_fp8_sparse", q, k, v, ld, hstride, S, H, kv_ptr, kv_idx, out, ldo, workspace,
                   workspace_bytes, stream);
+}
+
+int h3_attn_bf16(const void* q, long long ldq, long long hsq, const void* k, long long ldk, long long hsk,
+                 const void* v, long long ldv, long long hsv, int S, int Hq, int Hk, const int* span_lo,
+                 const int* span_hi, void* out, long long ldo, void* stream) {
+  const char* who = "h3_attn_bf16";
+  using L = AttnBf16Smem;
+  if (!q || !k || !v || !out) return fail(H3_ERR_ARG, "%s: NULL pointer", who);
+  if ((span_lo == nullptr) != (span_hi == nullptr)) return fail(H3_ERR_ARG, "%s: half a span list", who);
+  if (S <= 0 || S > L::MAX_S || Hk <= 0 || Hq <= 0 || Hq > 65535 || Hq % Hk)
+    return fail(H3_ERR_SHAPE, "%s: need 0 < S <= %d, 0 < Hq <= 65,535 and Hq a multiple of Hk (S=%d Hq=%d Hk=%d)", who,
+                L::MAX_S, S, Hq, Hk);
+  if (ldo % 8 || ldo < (long long)Hq * 128)
+    return fail(H3_ERR_SHAPE, "%s: output rows of %lld elements: a multiple of 8, at least Hq * 128", who, ldo);
+  const struct { long long ld, hs; int heads; } st[3] = {{ldq, hsq, Hq}, {ldk, hsk, Hk}, {ldv, hsv, Hk}};
+  for (const auto& x : st)
+    if ((S > 1 && (x.ld <= 0 || x.ld % 8)) || (x.heads > 1 && (x.hs <= 0 || x.hs % 8)))
+      return fail(H3_ERR_SHAPE, "%s: token and head strides must be positive multiples of 8 elements", who);
+  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) || !aligned(span_lo, 4) ||
+      !aligned(span_hi, 4))
+    return fail(H3_ERR_ARG, "%s: q / k / v / out 16-byte and spans 4-byte alignment required", who);
+  CUtensorMap tq, tk, tv;
+  int rc;
+  if ((rc = make_map_bf16(&tq, q, 128, S, Hq, ldq, hsq, 128, who))) return rc;
+  if ((rc = make_map_bf16(&tk, k, 128, S, Hk, ldk, hsk, 128, who))) return rc;
+  if ((rc = make_map_bf16(&tv, v, 128, S, Hk, ldv, hsv, 128, who))) return rc;
+  if ((rc = smem_optin(attn_bf16_kernel, L::TOTAL, &g_optin_attn_bf16, who))) return rc;
+  AttnBf16Args a{reinterpret_cast<__nv_bfloat16*>(out), ldo, reinterpret_cast<const __nv_bfloat16*>(v), ldv, hsv,
+                 span_lo, span_hi, S, Hq / Hk};
+  attn_bf16_kernel<<<dim3((S + 255) / 256, Hq), kAttnBf16Threads, L::TOTAL, S_(stream)>>>(tq, tk, tv, a);
+  return check_launch(who);
 }
 
 }  // extern "C"

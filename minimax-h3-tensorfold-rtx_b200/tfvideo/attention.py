@@ -7,6 +7,11 @@ fp8            libh3b200's tcgen05 FP8 flash attention (Q/K FP8 per row / per 12
 fp8_sparse(m)  the same kernel under a block-sparse mask ``m`` (a TileMask: per 128-token query tile, the 128-token KV
                tiles it attends to).  ``TileMask.block_sparse`` builds the seeded mask of BASELINE's sharded config
                (25% of tiles per query row, diagonal and text tiles always kept).
+bf16           libh3b200's tcgen05 bf16 flash attention: q, k, v read as they are, no quantisation; key heads may be
+               shared by groups of query heads.
+bf16_spans(m)  the same kernel under a SpanMask ``m``: token i attends to the keys [lo_i, hi_i).  Several requests
+               packed in one sequence (``SpanMask.documents``), or a prompt with frame-causal video behind it
+               (``SpanMask.frames``).
 sdpa / cudnn   PyTorch's bf16 backends, kept as the reference's comparison points (not the fast path).
 The reference's ``int8`` (comfy-kitchen) and ``fp4`` (Triton, sm_120) backends have no B200 build; asking for them
 raises ValueError, like any unknown name.
@@ -94,6 +99,51 @@ class TileMask:
         return cls(lists, S, device)
 
 
+class SpanMask:
+    """The keys each token attends to, as one span [lo, hi) a token: int32 [S] device tensors (clipped to [0, S)).  A
+    token with an empty span attends to nothing and gets zeros.  Read on the device when the kernel runs, so a captured
+    graph follows changes made in place."""
+
+    def __init__(self, lo: torch.Tensor, hi: torch.Tensor):
+        for t in (lo, hi):
+            if t.dim() != 1 or t.dtype != torch.int32 or not t.is_contiguous() or t.shape != lo.shape:
+                raise ValueError("SpanMask: lo and hi must be contiguous int32 [S] tensors, got "
+                                 f"{tuple(lo.shape)} {lo.dtype} and {tuple(hi.shape)} {hi.dtype}")
+        self.lo, self.hi, self.S = lo, hi, lo.shape[0]
+
+    @classmethod
+    def documents(cls, lengths, S: int | None = None, device="cuda") -> "SpanMask":
+        """Requests of the given lengths one after another, each token attending to its own request; tokens behind the
+        last one (up to ``S``) attend to nothing."""
+
+        return cls.frames(lengths, 0, 0, S, device)
+
+    @classmethod
+    def frames(cls, lengths, frame: int, prefix=0, S: int | None = None, device="cuda") -> "SpanMask":
+        """Requests as for ``documents``, each a prefix (``prefix`` tokens, one number or one a request) that attends
+        to itself, then frames of ``frame`` tokens that attend to the prefix and to every frame up to their own
+        (``frame`` 1: causal; 0: no frames, the whole request)."""
+
+        lengths = [int(n) for n in lengths]
+        prefix = [int(prefix)] * len(lengths) if isinstance(prefix, int) else [int(p) for p in prefix]
+        S = sum(lengths) if S is None else int(S)
+        if min(lengths, default=0) < 0 or sum(lengths) > S or frame < 0 or min(prefix, default=0) < 0 \
+                or len(prefix) != len(lengths):
+            raise ValueError(f"SpanMask: lengths {lengths} (prefix {prefix}, frame {frame}) do not fit {S} tokens")
+        lo, hi = torch.zeros(S, dtype=torch.int32), torch.zeros(S, dtype=torch.int32)
+        at = 0
+        for n, p in zip(lengths, prefix):
+            lo[at:at + n] = at
+            if frame:
+                i = torch.arange(n)
+                p = min(p, n)
+                hi[at:at + n] = (at + torch.where(i < p, p, p + ((i - p) // frame + 1) * frame).clamp(max=n)).int()
+            else:
+                hi[at:at + n] = at + n
+            at += n
+        return cls(lo.to(device), hi.to(device))
+
+
 def fp8_tokens(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, S: int, H: int, ld: int, hstride: int,
                out: torch.Tensor, workspace: torch.Tensor | None = None, mask: TileMask | None = None) -> torch.Tensor:
     """Low-level form: element (t, h, d) of q / k / v at base + t * ld + h * hstride + d; out [S, H * 128] bf16.
@@ -129,7 +179,56 @@ def fp8_sparse(mask: TileMask):
     return run
 
 
-BACKENDS = {"sdpa": sdpa_flash, "cudnn": sdpa_cudnn, "fp8": fp8}
+def bf16_tokens(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                mask: SpanMask | None = None) -> torch.Tensor:
+    """Low-level form: q [S, Hq, 128], k and v [S, Hk, 128] bf16 views (token and head strides multiples of 8,
+    16-byte aligned); out [S, Hq * 128] bf16, row stride a multiple of 8."""
+
+    S, Hq, _ = q.shape
+    if mask is not None and mask.S != S:
+        raise ValueError(f"SpanMask is for S={mask.S}, attention has S={S}")
+    lo, hi = (None, None) if mask is None else (mask.lo, mask.hi)
+    with N.on_device("bf16 attention", q, k, v, out, *(() if mask is None else (lo, hi))) as stream:
+        if S and Hq:
+            N.attn_bf16(q, q.stride(0), q.stride(1), k, k.stride(0), k.stride(1), v, v.stride(0), v.stride(1), S, Hq,
+                        k.shape[1], lo, hi, out, out.stride(0), stream)
+    return out
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """t [1, H, S, 128] as [S, H, 128] rows the kernel can read in place, copied when its strides do not allow it."""
+
+    x = t[0].transpose(0, 1)
+    S, H, _ = x.shape
+    if x.stride(2) != 1 or x.data_ptr() % 16 or (S > 1 and (x.stride(0) % 8 or x.stride(0) <= 0)) \
+            or (H > 1 and (x.stride(1) % 8 or x.stride(1) <= 0)):
+        x = x.contiguous()
+    return x
+
+
+def bf16(q, k, v, mask: SpanMask | None = None):
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 4 or t.shape[0] != 1 or t.shape[3] != HEAD_DIM or t.dtype != torch.bfloat16:
+            raise ValueError(f"bf16 attention: {name} must be bf16 [1, H, S, {HEAD_DIM}], got {tuple(t.shape)} {t.dtype}")
+    _, H, S, D = q.shape
+    if k.shape != v.shape or k.shape[2] != S or k.shape[1] == 0 or H % k.shape[1]:
+        raise ValueError(f"bf16 attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: one length, and "
+                         "query heads a multiple of the key heads")
+    out = torch.empty((S, H * D), dtype=torch.bfloat16, device=q.device)
+    bf16_tokens(_rows16(q), _rows16(k), _rows16(v), out, mask)
+    return out.view(1, S, H, D).transpose(1, 2)
+
+
+def bf16_spans(mask: SpanMask):
+    """A backend function (q, k, v) -> o running the bf16 kernel under ``mask``."""
+
+    def run(q, k, v):
+        return bf16(q, k, v, mask)
+
+    return run
+
+
+BACKENDS = {"sdpa": sdpa_flash, "cudnn": sdpa_cudnn, "fp8": fp8, "bf16": bf16}
 BENCH: dict = {}
 DEFAULT = "fp8"
 

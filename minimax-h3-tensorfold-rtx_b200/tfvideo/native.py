@@ -63,6 +63,7 @@ _SIGS = {
     "h3_attn_fp8_noalloc": [vp, vp, vp, i64, i64, i32, i32, vp, i64, vp],
     "h3_attn_fp8_sparse": [vp, vp, vp, i64, i64, i32, i32, vp, vp, vp, i64, vp, sz, vp],
     "h3_attn_fp8_peers": [vp, vp, vp, i64, i64, i32, i32, vp, vp, C.POINTER(vp), i32, i32, i64, vp, sz, vp],
+    "h3_attn_bf16": [vp, i64, i64, vp, i64, i64, vp, i64, i64, i32, i32, i32, vp, vp, vp, i64, vp],
     "h3_peer_alloc": [sz, C.POINTER(vp), vp],
     "h3_peer_open": [vp, C.POINTER(vp)],
     "h3_peer_close": [vp],
@@ -294,6 +295,12 @@ def attn_fp8_peers(q, k, v, ld, hstride, S, H, peers: list[int], rank: int, ldo,
     check(lib().h3_attn_fp8_peers(ptr(q), ptr(k), ptr(v), ld, hstride, S, H, ptr(kv_ptr), ptr(kv_idx), arr,
                                   len(peers), rank, ldo, ptr(workspace), workspace.numel() * workspace.element_size(),
                                   stream()), "h3_attn_fp8_peers")
+
+
+def attn_bf16(q, ldq, hsq, k, ldk, hsk, v, ldv, hsv, S, Hq, Hk, lo, hi, out, ldo, stream_handle: int) -> None:
+    _count(1)
+    check(lib().h3_attn_bf16(ptr(q), ldq, hsq, ptr(k), ldk, hsk, ptr(v), ldv, hsv, S, Hq, Hk, ptr(lo), ptr(hi),
+                             ptr(out), ldo, stream_handle), "h3_attn_bf16")
 
 
 # ---- device buffers shared between the processes of one node (CUDA IPC), for the fused Ulysses exchanges

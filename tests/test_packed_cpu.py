@@ -90,3 +90,53 @@ def test_rope_functions_refuse_bad_arguments():
                    dict()):                                                  # the last: CPU tensors
         with pytest.raises(ValueError):
             K.qknorm_rope_axes(**{**ok, **change})
+
+
+def test_attn_bf16_checks_its_arguments(lib):
+    from tfvideo import native as N
+
+    def call(q=FAKE, ldq=384, hsq=128, ldk=384, S=10, Hq=2, Hk=1, lo=None, hi=None, out=FAKE, ldo=256):
+        return lib.h3_attn_bf16(q, ldq, hsq, FAKE, ldk, 128, FAKE, 384, 128, S, Hq, Hk, lo, hi, out, ldo, None)
+
+    assert call(q=None) == -1 and call(out=None) == -1
+    assert call(lo=FAKE) == -1 and "half" in N.last_error()
+    assert call(lo=FAKE + 2, hi=FAKE) == -1
+    assert call(S=0) == -2 and call(S=262_145) == -2 and call(Hk=0) == -2 and call(Hq=3, Hk=2, ldo=384) == -2
+    assert call(Hq=65_536, Hk=1, ldo=65_536 * 128) == -2
+    assert call(ldo=128) == -2 and call(ldo=260) == -2
+    assert call(ldq=0) == -2 and call(ldq=388) == -2 and call(hsq=-128) == -2 and call(ldk=-8) == -2
+    assert call(q=FAKE + 8) == -1 and "16-byte" in N.last_error()
+
+
+def test_span_masks():
+    from tfvideo import attention as A
+
+    m = A.SpanMask.documents([3, 0, 2], 7, device="cpu")
+    assert m.lo.tolist() == [0, 0, 0, 3, 3, 0, 0] and m.hi.tolist() == [3, 3, 3, 5, 5, 0, 0]
+    m = A.SpanMask.frames([6, 2], 2, [1, 5], device="cpu")
+    assert m.lo.tolist() == [0] * 6 + [6] * 2 and m.hi.tolist() == [1, 3, 3, 5, 5, 6, 8, 8]
+    m = A.SpanMask.frames([4], 1, device="cpu")
+    assert m.hi.tolist() == [1, 2, 3, 4]
+    assert A.SpanMask.documents([], 0, device="cpu").S == 0
+    for bad in (dict(lengths=[3, -1]), dict(lengths=[3], S=2)):
+        with pytest.raises(ValueError):
+            A.SpanMask.documents(**bad, device="cpu")
+    for bad in (dict(lengths=[3], frame=-1), dict(lengths=[3], frame=1, prefix=-1), dict(lengths=[3], frame=1, prefix=[1, 2])):
+        with pytest.raises(ValueError):
+            A.SpanMask.frames(**bad, device="cpu")
+    i = torch.zeros(4, dtype=torch.int32)
+    for lo, hi in ((i.long(), i), (i, i.float()), (i[:3], i), (i[::2], i[::2]), (i[None], i[None])):
+        with pytest.raises(ValueError):
+            A.SpanMask(lo, hi)
+
+
+def test_bf16_attention_refuses_bad_arguments():
+    from tfvideo import attention as A
+
+    q = torch.zeros((1, 4, 10, 128), dtype=torch.bfloat16)
+    m = A.SpanMask.documents([9], device="cpu")
+    for bad in ((q.float(), q, q), (q[0], q, q), (q[..., :64], q[..., :64], q[..., :64]), (q, q[:, :3], q[:, :3]),
+                (q, q[:, :, :9], q[:, :, :9]), (q, q, q[:, :2]), (q, q[:, :0], q[:, :0]), (q, q, q, m),
+                (q.expand(2, 4, 10, 128), q, q), (q, q, q)):                  # the last: CPU tensors
+        with pytest.raises(ValueError):
+            A.bf16(*bad)
