@@ -116,7 +116,7 @@ int h3_nvfp4_quant(const void* x, long long ldx, int cblk, long long blk_stride,
 int h3_gate_add(void* x, int ldx, const void* y, int ldy, const float* mod, const int* idx, int S, int D, int part,
                 void* stream);
 /* act_kind 0: gelu_tanh(u) (u [M, F]); 1: silu(gate) * up (u = [gate | up] [M, 2F]) (replaces kernels.swiglu,
- * tfvideo/kernels.py:66-84); bf16 out [M, F]; amax (nullable) += max |out|.  F % 8 == 0. */
+ * tfvideo/kernels.py:66-84); 2: the same from 16 gate and 16 up columns in turn (F % 16 == 0); bf16 out [M, F]; amax (nullable) += max |out|.  F % 8 == 0. */
 int h3_act(const void* u, int ldu, void* out, int ldo, int M, int F, int act_kind, float* amax, void* stream);
 /* mod[m, j] = ada_b[j] + t_emb[m] . ada_w[j] (fp32 [M, J]) (replaces MiniMaxH3Engine.modulation,
  * tfvideo/minimax_h3.py:265-269). */
@@ -156,6 +156,19 @@ int h3_peer_copy(const H3PeerCopy* copies, int n, void* stream);
 int h3_gemm_nvfp4(const uint8_t* a_codes, const uint8_t* a_sf, const H3ScaleSlot* a_slot, const uint8_t* b_codes,
                   const uint8_t* b_sf, float g_b, const float* bias, int M, int N, int K, const H3Epilogue* epi,
                   void* stream);
+
+/* ---------------------------------------------------------------------------------------------- adapters */
+/* Low-rank adapters of several requests beside a shared projection: out_m = y_m + B_a (scale[a] A_a x_m) with
+ * a = rows[m], for bf16 x [M, K], y and out [M, N] (row strides ldx, ldy, ldo; out may be y itself, and is otherwise
+ * apart from the inputs), A [n, R, K] and B [n, N, R] contiguous (lower ranks padded with zeros), scale fp32 [n] or
+ * NULL (1), rows int32 [M] in any order.  A row whose entry is outside [0, n) has no adapter and is copied bit for bit.
+ * Sums in 32 bits; scale[a] A_a x_m is rounded to bf16 once.  K, N, R multiples of 8, R <= 128; pointers 16-byte
+ * aligned.  workspace: h3_adapter_workspace_bytes(M, R) bytes, one per call in flight.  The reference merges one adapter
+ * set into the weights instead (tfvideo/comfy_nodes.py:95-166). */
+size_t h3_adapter_workspace_bytes(int M, int R);
+int h3_adapter_add(const void* x, long long ldx, const void* y, long long ldy, const void* A, const void* B,
+                   const float* scale, const int* rows, int M, int K, int N, int R, int n, void* out, long long ldo,
+                   void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------------------- attention */
 /* Per-head RMSNorm (weights qw, kw [128]) + split-half RoPE over the first `rot` dims, in place on q and k rows

@@ -1,0 +1,388 @@
+// Low-rank adapters of several requests beside a shared projection: out_m = y_m + B_a (scale_a A_a x_m), a = rows[m]
+// (no adapter outside [0, n)).  No counterpart in the reference, which merges adapters into the weights before they are
+// quantised (tfvideo/comfy_nodes.py:95-166): one set at a time, re-converting the model for each.
+//
+// Two kernels on tcgen05 (kind::f16, fp32 accumulators): shrink, T_m = scale_a A_a x_m, which reads x once, and
+// expand, out = y + T B^T, which reads y and writes out once; T is M x R.  Both are bound by those bytes: a row of
+// y, x and out is 2 (K + 2 N) bytes for 2 R (K + N) FLOP, R FLOP a byte, against about 250 at the measured rates.
+// T is rounded to bf16 once (its sums are in 32 bits): 2^-8 of the adapter's part, which is added to y in 32 bits.
+//
+// Rows come in any order.  A 128-row tile works through the adapters that occur in it, and each row takes only its own
+// adapter's product, from an accumulator of that adapter alone: another request's weights never reach it, non-finite
+// ones included.  Rows without an adapter are copied (or left, in place) bit for bit.
+#pragma once
+
+#include "attention_bf16.cuh"
+#include "common.cuh"
+#include "h3b200.h"
+
+namespace h3 {
+
+struct AdapterArgs {
+  const int* rows;      // [M]
+  const float* scale;   // [n], or NULL: 1
+  __nv_bfloat16* t;     // [M, Rp]
+  int M, K, N, n;
+  int Rp;               // rank rounded up to 16
+  int inplace;          // expand: out is y
+};
+
+// warp-wide store of one box of a 3-D tensor map from shared memory (the part outside the tensor is not written)
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* smem_src, int x, int y, int z) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t.reg .b32 rx;\n\t" H3_ELECT
+      "@e cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];\n\t}" ::"l"(map), "r"(x),
+      "r"(y), "r"(z), "r"(smem_u32(smem_src))
+      : "memory");
+}
+// the elected lane's stores have read their shared memory
+__device__ __forceinline__ void tma_store_wait_read() {
+  asm volatile("{\n\t.reg .pred e;\n\t.reg .b32 rx;\n\t" H3_ELECT
+               "@e cp.async.bulk.commit_group;\n\t@e cp.async.bulk.wait_group.read 0;\n\t}" ::: "memory");
+}
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {   // addr: cluster_addr of another CTA's shared memory
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr));
+  return v;
+}
+
+// One warp: the distinct adapters of rows m0 .. m0 + 127 in rising order; returns how many.
+__device__ __forceinline__ int tile_adapters(const AdapterArgs& a, int m0, int lane, int* list) {
+  int id[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int m = m0 + 32 * i + lane;
+    id[i] = m < a.M ? a.rows[m] : -1;
+    if (id[i] < 0 || id[i] >= a.n) id[i] = INT_MAX;
+  }
+  int count = 0, last = -1;
+  for (;;) {
+    int next = INT_MAX;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (id[i] > last) next = min(next, id[i]);
+    next = __reduce_min_sync(~0u, next);
+    if (next == INT_MAX) break;
+    if (lane == 0) list[count] = next;
+    ++count;
+    last = next;
+  }
+  __syncwarp();
+  return count;
+}
+
+// ------------------------------------------------------------------------------------------------ shrink
+// blockIdx.x: 128-row tile; the CTAs of a cluster (gridDim.y, 1 to 8) share the tile's K range, and add their partial
+// sums over distributed shared memory in a fixed order.  Stages of 64 K elements: the x tile (128 rows of 128 bytes)
+// and, stacked as the MMA's N rows, the A rows of up to G adapters; a tile with more adapters walks x again for the
+// next G (from L2).  Warps 0-3: epilogue, a thread per row; warp 4: TMA; warp 5: MMA.
+struct ShrinkSmem {
+  static constexpr int X = 128 * 128;
+  __host__ __device__ static constexpr int group(int rp) { return rp >= 64 ? 1 : 64 / rp; }
+  __host__ __device__ static constexpr int slot(int rp) { return X + (rp > 64 ? rp : 64) * 128; }
+  __host__ __device__ static constexpr int stages(int rp) { return 98304 / slot(rp); }
+  __host__ __device__ static constexpr int red_row(int rp) { return rp * 4 + 16; }   // padded: threads hold rows
+  __host__ __device__ static constexpr int total(int rp, int splits) {
+    return 1024 + stages(rp) * slot(rp) + (splits > 1 ? 128 * red_row(rp) : 0) + 1024;
+  }
+};
+
+__global__ void __launch_bounds__(192)
+    adapter_shrink_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmA,
+                          const AdapterArgs a) {
+  using L = ShrinkSmem;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int G = L::group(a.Rp), slot = L::slot(a.Rp), stages = L::stages(a.Rp);   // stages: 3 or 4
+  const int splits = gridDim.y;
+  uint8_t* red = smem + stages * slot;
+  uint64_t* full = reinterpret_cast<uint64_t*>(red + (splits > 1 ? 128 * L::red_row(a.Rp) : 0));
+  uint64_t* empty = full + 4;
+  uint64_t* acc_full = empty + 4;
+  uint64_t* acc_empty = acc_full + 1;
+  uint64_t* drained = acc_empty + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+  int* count_s = reinterpret_cast<int*>(tmem_slot + 1);
+  int* list = count_s + 1;   // [128]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int m0 = blockIdx.x * 128;
+  const uint32_t ncols = a.Rp > 64 ? 128 : 64;
+
+  if (threadIdx.x == 32) {
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_init(acc_empty, 4);
+    mbar_init(drained, 1);
+    fence_barrier_init();
+  }
+  if (warp == 0) {
+    const int c = tile_adapters(a, m0, lane, list);
+    if (lane == 0) *count_s = c;
+  }
+  if (warp == 5) {
+    tmem_alloc(tmem_slot, ncols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int count = *count_s;
+  const int chunks = (a.K + 63) >> 6;
+  const int c0 = (int)((long long)chunks * blockIdx.y / splits), c1 = (int)((long long)chunks * (blockIdx.y + 1) / splits);
+  const int passes = (count + G - 1) / G;
+
+  if (warp == 4) {
+    int it = 0;
+    bool ok = true;
+    for (int p = 0; ok && p < passes; ++p) {
+      const int cnt = min(G, count - p * G);
+      for (int c = c0; c < c1; ++c, ++it) {
+        const int st = it % stages;
+        ok = __all_sync(~0u, mbar_wait(&empty[st], ((it / stages) & 1) ^ 1, 401));
+        if (!ok) break;
+        uint8_t* s = smem + st * slot;
+        mbar_arrive_expect_tx(&full[st], L::X + cnt * a.Rp * 128);
+        tma_load_3d(s, &tmX, c * 64, m0, 0, &full[st]);
+        for (int g = 0; g < cnt; ++g)
+          tma_load_3d(s + L::X + g * a.Rp * 128, &tmA, c * 64, 0, list[p * G + g], &full[st]);
+      }
+    }
+    for (int j = max(it - stages, 0); j < it; ++j) mbar_drain(&full[j % stages], (j / stages) & 1, 402);
+  } else if (warp == 5) {
+    int it = 0;
+    bool ok = true;
+    for (int p = 0; ok && p < passes; ++p) {
+      const int cnt = min(G, count - p * G);
+      const uint32_t idesc = idesc_bf16(128, cnt * a.Rp, false);
+      if (p > 0 && !(ok = __all_sync(~0u, mbar_wait(acc_empty, (p - 1) & 1, 411)))) break;
+      for (int c = c0; c < c1; ++c, ++it) {
+        const int st = it % stages;
+        ok = __all_sync(~0u, mbar_wait(&full[st], (it / stages) & 1, 412));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t xa = smem_u32(smem + st * slot), wa = xa + L::X;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          mma_bf16_ss(tmem, sdesc_kmajor_sw128(xa + kk * 32), sdesc_kmajor_sw128(wa + kk * 32), idesc, c != c0 || kk != 0);
+        tc_commit(&empty[st]);
+      }
+      if (ok) tc_commit(acc_full);
+    }
+    tc_commit(drained);   // every MMA has left the tensor core before TMEM is given back
+    mbar_drain(drained, 0, 413);
+  } else {
+    const int row = threadIdx.x, m = m0 + row;
+    int id = m < a.M ? a.rows[m] : -1;
+    if (id >= a.n) id = -1;
+    const float sc = id >= 0 && a.scale ? a.scale[id] : 1.0f;
+    const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+    for (int p = 0; p < passes; ++p) {
+      const int cnt = min(G, count - p * G);
+      if (!__all_sync(~0u, mbar_wait(acc_full, p & 1, 420))) break;
+      tc_fence_after();
+      for (int g = 0; g < cnt; ++g) {
+        const bool mine = id == list[p * G + g];
+        if (!__any_sync(~0u, mine)) continue;
+        for (int c = 0; c < a.Rp; c += 16) {
+          uint32_t v[16];
+          tmem_ld16(tmem + lane_off + g * a.Rp + c, v);
+          tmem_ld_wait();
+          if (mine && splits > 1) {
+            float4* d = reinterpret_cast<float4*>(red + row * L::red_row(a.Rp) + c * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              d[e] = make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]), __uint_as_float(v[4 * e + 2]),
+                                 __uint_as_float(v[4 * e + 3]));
+          } else if (mine) {
+            uint32_t w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              w[e] = pack_bf16(__uint_as_float(v[2 * e]) * sc, __uint_as_float(v[2 * e + 1]) * sc);
+            uint4* d = reinterpret_cast<uint4*>(a.t + (size_t)m * a.Rp + c);
+            d[0] = make_uint4(w[0], w[1], w[2], w[3]);
+            d[1] = make_uint4(w[4], w[5], w[6], w[7]);
+          }
+          __syncwarp();
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty);
+    }
+  }
+  if (splits > 1) {
+    __syncwarp();
+    cluster_sync();
+    const int per = 128 / splits, pieces = a.Rp >> 3;   // this CTA's rows, eight columns a thread at a time
+    for (int i = threadIdx.x; i < per * pieces; i += 192) {
+      const int row = blockIdx.y * per + i / pieces, c = (i % pieces) * 8, m = m0 + row;
+      const int id = m < a.M ? a.rows[m] : -1;
+      if (id < 0 || id >= a.n) continue;
+      float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      for (int s = 0; s < splits; ++s) {
+        const uint32_t at = cluster_addr(red + row * L::red_row(a.Rp) + c * 4, s);
+        const float4 u = ld_cluster_f4(at), v = ld_cluster_f4(at + 16);
+        f[0] += u.x; f[1] += u.y; f[2] += u.z; f[3] += u.w;
+        f[4] += v.x; f[5] += v.y; f[6] += v.z; f[7] += v.w;
+      }
+      const float sc = a.scale ? a.scale[id] : 1.0f;
+      *reinterpret_cast<uint4*>(a.t + (size_t)m * a.Rp + c) =
+          make_uint4(pack_bf16(f[0] * sc, f[1] * sc), pack_bf16(f[2] * sc, f[3] * sc), pack_bf16(f[4] * sc, f[5] * sc),
+                     pack_bf16(f[6] * sc, f[7] * sc));
+    }
+    __syncwarp();
+    cluster_sync();   // no CTA ends while another still reads its partial sums
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 5) tmem_dealloc(tmem, ncols);
+}
+
+// ------------------------------------------------------------------------------------------------ expand
+// A CTA per 128 rows x 128 columns: y, T and B tiles by TMA, one accumulator of 128 columns, out by TMA from where y
+// landed.  Several CTAs an SM keep loads and stores in flight.  Warps 0-3: epilogue, a thread per row; warp 4: the rest.
+struct ExpandSmem {
+  static constexpr int SUB = 128 * 128;   // 128 rows x 64 elements
+  __host__ __device__ static constexpr int kc(int rp) { return rp > 64 ? 2 : 1; }
+  __host__ __device__ static constexpr int total(int rp) { return 1024 + 2 * SUB + 2 * kc(rp) * SUB + 1024; }
+};
+
+__global__ void __launch_bounds__(160)
+    adapter_expand_kernel(const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmT,
+                          const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmO,
+                          const AdapterArgs a) {
+  using L = ExpandSmem;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int kc = L::kc(a.Rp);
+  uint8_t* ys = smem;
+  uint8_t* ts = ys + 2 * L::SUB;
+  uint8_t* bs = ts + kc * L::SUB;
+  uint64_t* y_full = reinterpret_cast<uint64_t*>(bs + kc * L::SUB);
+  uint64_t* t_full = y_full + 1;
+  uint64_t* b_full = t_full + 1;
+  uint64_t* acc_full = b_full + 1;
+  uint64_t* acc_empty = acc_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 1);
+  int* count_s = reinterpret_cast<int*>(tmem_slot + 1);
+  int* list = count_s + 1;   // [128]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int ntile = (a.N + 127) >> 7;
+  const int n0 = (blockIdx.x % ntile) * 128, m0 = (blockIdx.x / ntile) * 128;
+
+  if (threadIdx.x == 0) {
+    mbar_init(y_full, 1);
+    mbar_init(t_full, 1);
+    mbar_init(b_full, 1);
+    mbar_init(acc_full, 1);
+    mbar_init(acc_empty, 4);
+    fence_barrier_init();
+  }
+  if (warp == 4) {
+    tmem_alloc(tmem_slot, 128);
+    tmem_relinquish();
+    const int c = tile_adapters(a, m0, lane, list);
+    if (lane == 0) *count_s = c;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int count = *count_s;
+  const bool moves = count > 0 || !a.inplace;   // in place, a tile without adapters stays as it is
+  bool ok = true;
+
+  if (warp == 4) {
+    if (moves) {
+      mbar_arrive_expect_tx(y_full, 2 * L::SUB);
+      tma_load_3d(ys, &tmY, n0, m0, 0, y_full);
+      tma_load_3d(ys + L::SUB, &tmY, n0 + 64, m0, 0, y_full);
+    }
+    if (count > 0) {
+      mbar_arrive_expect_tx(t_full, kc * L::SUB);
+      for (int c = 0; c < kc; ++c) tma_load_3d(ts + c * L::SUB, &tmT, 64 * c, m0, 0, t_full);
+    }
+    constexpr uint32_t idesc = idesc_bf16(128, 128, false);
+    int loads = 0, products = 0;   // B tiles asked for, products committed
+    for (int i = 0; i < count; ++i) {
+      // (the previous product is complete: its B tile may be overwritten)
+      if (i > 0 && !(ok = __all_sync(~0u, mbar_wait(acc_full, (i - 1) & 1, 431)))) break;
+      mbar_arrive_expect_tx(b_full, kc * L::SUB);
+      for (int c = 0; c < kc; ++c) tma_load_3d(bs + c * L::SUB, &tmB, 64 * c, n0, list[i], b_full);
+      ++loads;
+      ok = __all_sync(~0u, mbar_wait(b_full, i & 1, 432)) && __all_sync(~0u, mbar_wait(t_full, 0, 433)) &&
+           (i == 0 || __all_sync(~0u, mbar_wait(acc_empty, (i - 1) & 1, 434)));
+      if (!ok) break;
+      tc_fence_after();
+      for (int kk = 0; kk < a.Rp / 16; ++kk) {
+        const uint32_t off = (kk >> 2) * L::SUB + (kk & 3) * 32;
+        mma_bf16_ss(tmem, sdesc_kmajor_sw128(smem_u32(ts) + off), sdesc_kmajor_sw128(smem_u32(bs) + off), idesc, kk != 0);
+      }
+      tc_commit(acc_full);
+      ++products;
+    }
+    // every copy has landed and every product is complete before the store and the end of the CTA
+    if (moves) mbar_drain(y_full, 0, 435);
+    if (count > 0) mbar_drain(t_full, 0, 435);
+    if (loads > 0) mbar_drain(b_full, (loads - 1) & 1, 435);
+    if (products > 0) mbar_drain(acc_full, (products - 1) & 1, 436);
+  } else {
+    const int row = threadIdx.x, m = m0 + row;
+    int id = m < a.M ? a.rows[m] : -1;
+    if (id >= a.n) id = -1;
+    const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+    ok = count == 0 || __all_sync(~0u, mbar_wait(y_full, 0, 440));
+    for (int i = 0; i < count; ++i) {
+      if (!(ok = ok && __all_sync(~0u, mbar_wait(acc_full, i & 1, 441)))) break;
+      tc_fence_after();
+      const bool mine = id == list[i];
+      if (__any_sync(~0u, mine)) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t d[32];
+          tmem_ld32(tmem + lane_off + 32 * c, d);
+          tmem_ld_wait();
+          if (mine) {
+            uint8_t* sub = ys + (c >> 1) * L::SUB + row * 128;   // 16-byte pieces, swizzled as TMA wrote them
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint4* at = reinterpret_cast<uint4*>(sub + ((((c & 1) * 4 + q) ^ (row & 7)) << 4));
+              uint4 u = *at;
+              uint32_t* w = &u.x;
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                w[e] = pack_bf16(bf16_lo(w[e]) + __uint_as_float(d[8 * q + 2 * e]),
+                                 bf16_hi(w[e]) + __uint_as_float(d[8 * q + 2 * e + 1]));
+              *at = u;
+            }
+          }
+          __syncwarp();
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the store reads these writes
+  }
+  tc_fence_before();
+  const bool good = __syncthreads_and(ok);
+  tc_fence_after();
+  if (warp == 4) {
+    if (moves && good) {
+      tma_store_3d(&tmO, ys, n0, m0, 0);
+      if (n0 + 64 < a.N) tma_store_3d(&tmO, ys + L::SUB, n0 + 64, m0, 0);
+      tma_store_wait_read();
+    }
+    tmem_dealloc(tmem, 128);
+  }
+}
+
+}  // namespace h3

@@ -72,6 +72,17 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+// Waits until a barrier's phase completes whether or not another wait of the grid gave up, for at most the same limit:
+// copies and MMAs in flight end before a CTA gives back its memory.
+__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity, int code) {
+  if (mbar_try_wait(bar, parity)) return;
+  const uint64_t t0 = globaltimer();
+  while (!mbar_try_wait_suspend(bar, parity, kSuspendNs))
+    if (globaltimer() - t0 > kWaitLimitNs) {
+      set_status(code);
+      return;
+    }
+}
 // kind::f16 with bf16 operands and an fp32 accumulator: C format F32 = 1 in bits 4-5, A / B format BF16 = 1 in bits
 // 7-9 / 10-12, bit 16 = B is MN-major (its N elements contiguous in shared memory).
 __host__ __device__ constexpr uint32_t idesc_bf16(int M, int N, bool b_mn_major) {
@@ -276,9 +287,9 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
       ++nv;
     }
     // nothing may still be landing in this CTA's memory when it ends, after a wait that gave up included
-    if (steps > 0) mbar_wait(q_full, 0, 303);
-    for (int j = max(nk - L::KST, 0); j < nk; ++j) mbar_wait(&k_full[j % L::KST], (j / L::KST) & 1, 303);
-    for (int j = max(nv - L::VST, 0); j < nv; ++j) mbar_wait(&v_full[j % L::VST], (j / L::VST) & 1, 303);
+    if (steps > 0) mbar_drain(q_full, 0, 303);
+    for (int j = max(nk - L::KST, 0); j < nk; ++j) mbar_drain(&k_full[j % L::KST], (j / L::KST) & 1, 303);
+    for (int j = max(nv - L::VST, 0); j < nv; ++j) mbar_drain(&v_full[j % L::VST], (j / L::VST) & 1, 303);
   } else if (warp == 9) {
     // ------------------------------------------------------------------ MMA
     constexpr uint32_t idesc_s = idesc_bf16(128, 128, false), idesc_o = idesc_bf16(128, 128, true);
@@ -330,7 +341,7 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
     }
     if (steps > 0) {   // every MMA has left the tensor core before TMEM and shared memory are given back
       tc_commit(drained);
-      mbar_wait(drained, 0, 315);
+      mbar_drain(drained, 0, 315);
     }
   } else if (warp == 10) {
     // ------------------------------------------------------------------ V guard
@@ -452,6 +463,7 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t o[32];
+        __syncwarp();
         if (any) {
           tmem_ld32(o_col + 32 * c, o);
           tmem_ld_wait();

@@ -285,8 +285,8 @@ __device__ __forceinline__ float gelu_tanh_f(float u) {
 }
 __device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + expf(-g)) * u; }
 
-// act = gelu_tanh(u) (act_kind 0, u [M, F]) or silu(gate) * up (act_kind 1, u = [gate | up] [M, 2F]); bf16 out
-// [M, F].  `amax` (nullable) receives max |act|.  tfvideo/kernels.py:66-84.
+// act = gelu_tanh(u) (act_kind 0, u [M, F]) or silu(gate) * up (act_kind 1, u = [gate | up] [M, 2F]; act_kind 2,
+// u [M, 2F] alternating 16 gate and 16 up columns, as a 16-interleaved fc1 writes them); bf16 out [M, F].  `amax` (nullable) receives max |act|.  tfvideo/kernels.py:66-84.
 __global__ void __launch_bounds__(256) act_kernel(const __nv_bfloat16* u, int ldu, __nv_bfloat16* out, int ldo, int M,
                                                   int F, int act_kind, float* amax) {
   const int vec = F >> 3;
@@ -294,8 +294,9 @@ __global__ void __launch_bounds__(256) act_kernel(const __nv_bfloat16* u, int ld
   float am = 0.f;
   for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
     int r = (int)(i / vec), c = (int)(i % vec) * 8;
-    uint4 a = *reinterpret_cast<const uint4*>(u + (size_t)r * ldu + c);
-    uint4 b = act_kind ? *reinterpret_cast<const uint4*>(u + (size_t)r * ldu + F + c) : a;
+    const int g = act_kind == 2 ? 2 * c - (c & 15) : c, up = act_kind == 2 ? g + 16 : F + c;
+    uint4 a = *reinterpret_cast<const uint4*>(u + (size_t)r * ldu + g);
+    uint4 b = act_kind ? *reinterpret_cast<const uint4*>(u + (size_t)r * ldu + up) : a;
     const uint32_t* aw = &a.x;
     const uint32_t* bw = &b.x;
     uint4 o;

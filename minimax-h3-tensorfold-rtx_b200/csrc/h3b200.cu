@@ -9,6 +9,7 @@
 #include <mutex>
 #include <string>
 
+#include "adapter.cuh"
 #include "attention.cuh"
 #include "attention_bf16.cuh"
 #include "elementwise.cuh"
@@ -124,7 +125,7 @@ int smem_optin(K kernel, int bytes, unsigned* done_mask, const char* what) {
 }
 
 unsigned g_optin_attn[2] = {0, 0};   // [NT - 1]
-unsigned g_optin_attn_bf16 = 0;
+unsigned g_optin_attn_bf16 = 0, g_optin_shrink = 0, g_optin_expand = 0;
 #ifndef H3_GEMM_PAIR
 #define H3_GEMM_PAIR 0
 #endif
@@ -456,7 +457,8 @@ int h3_gate_add(void* x, int ldx, const void* y, int ldy, const float* mod, cons
 int h3_act(const void* u, int ldu, void* out, int ldo, int M, int F, int act_kind, float* amax, void* stream) {
   if (!u || !out) return fail(H3_ERR_ARG, "h3_act: NULL pointer");
   if (M <= 0 || F <= 0 || F % 8 || ldu % 8 || ldo % 8) return fail(H3_ERR_SHAPE, "h3_act: need F %% 8 == 0");
-  if (act_kind != 0 && act_kind != 1) return fail(H3_ERR_ARG, "h3_act: act_kind must be 0 or 1");
+  if (act_kind < 0 || act_kind > 2) return fail(H3_ERR_ARG, "h3_act: act_kind must be 0, 1 or 2");
+  if (act_kind == 2 && F % 16) return fail(H3_ERR_SHAPE, "h3_act: act_kind 2 needs F %% 16 == 0");
   long long n = (long long)M * (F / 8);
   int blocks = (int)((n + 255) / 256 < 148 * 16 ? (n + 255) / 256 : 148 * 16);
   act_kernel<<<blocks, 256, 0, S_(stream)>>>(reinterpret_cast<const __nv_bfloat16*>(u), ldu,
@@ -777,6 +779,63 @@ int h3_attn_bf16(const void* q, long long ldq, long long hsq, const void* k, lon
   AttnBf16Args a{reinterpret_cast<__nv_bfloat16*>(out), ldo, reinterpret_cast<const __nv_bfloat16*>(v), ldv, hsv,
                  span_lo, span_hi, S, Hq / Hk};
   attn_bf16_kernel<<<dim3((S + 255) / 256, Hq), kAttnBf16Threads, L::TOTAL, S_(stream)>>>(tq, tk, tv, a);
+  return check_launch(who);
+}
+
+// ------------------------------------------------------------------------------------------------ adapters
+size_t h3_adapter_workspace_bytes(int M, int R) {
+  if (M <= 0 || R <= 0) return 0;
+  return (size_t)M * (size_t)((R + 15) / 16 * 16) * 2;
+}
+
+int h3_adapter_add(const void* x, long long ldx, const void* y, long long ldy, const void* A, const void* B,
+                   const float* scale, const int* rows, int M, int K, int N, int R, int n, void* out, long long ldo,
+                   void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "h3_adapter_add";
+  if (!x || !y || !A || !B || !rows || !out || !workspace) return fail(H3_ERR_ARG, "%s: NULL pointer", who);
+  if (M <= 0 || K <= 0 || N <= 0 || n <= 0 || R <= 0 || K % 8 || N % 8 || R % 8 || R > 128)
+    return fail(H3_ERR_SHAPE, "%s: need K, N, R %% 8 == 0 and R <= 128 (M=%d K=%d N=%d R=%d n=%d)", who, M, K, N, R, n);
+  if (ldx % 8 || ldy % 8 || ldo % 8 || ldx < K || ldy < N || ldo < N)
+    return fail(H3_ERR_SHAPE, "%s: row strides must be multiples of 8 elements, at least the row", who);
+  if (!aligned(x, 16) || !aligned(y, 16) || !aligned(A, 16) || !aligned(B, 16) || !aligned(out, 16) ||
+      !aligned(workspace, 16) || !aligned(rows, 4) || !aligned(scale, 4))
+    return fail(H3_ERR_ARG, "%s: x / y / A / B / out / workspace 16-byte alignment required", who);
+  if (workspace_bytes < h3_adapter_workspace_bytes(M, R))
+    return fail(H3_ERR_ARG, "%s: workspace %zu bytes < %zu", who, workspace_bytes, h3_adapter_workspace_bytes(M, R));
+  const int Rp = (R + 15) / 16 * 16;
+  const long long mtiles = ((long long)M + 127) / 128, ntiles = ((long long)N + 127) / 128;
+  if (mtiles * ntiles > 0x7FFFFFFF) return fail(H3_ERR_SHAPE, "%s: M x N too large (M=%d N=%d)", who, M, N);
+  CUtensorMap tx, ta, ty, tt, tb, to;
+  int rc;
+  if ((rc = make_map_bf16(&tx, x, K, M, 1, ldx, 0, 128, who))) return rc;
+  if ((rc = make_map_bf16(&ta, A, K, R, n, K, (long long)R * K, Rp, who))) return rc;
+  if ((rc = make_map_bf16(&ty, y, N, M, 1, ldy, 0, 128, who))) return rc;
+  if ((rc = make_map_bf16(&tt, workspace, Rp, M, 1, Rp, 0, 128, who))) return rc;
+  if ((rc = make_map_bf16(&tb, B, R, N, n, R, (long long)N * R, 128, who))) return rc;
+  if ((rc = make_map_bf16(&to, out, N, M, 1, ldo, 0, 128, who))) return rc;
+  if ((rc = smem_optin(adapter_shrink_kernel, 220 * 1024, &g_optin_shrink, who))) return rc;
+  if ((rc = smem_optin(adapter_expand_kernel, ExpandSmem::total(128), &g_optin_expand, who))) return rc;
+  AdapterArgs a{rows, scale, reinterpret_cast<__nv_bfloat16*>(workspace), M, K, N, n, Rp, out == y && ldo == ldy};
+  // the K range over a cluster of CTAs while the row tiles alone leave SMs idle, at least four 64-element stages each
+  const int chunks = (K + 63) / 64;
+  int splits = 1;
+  while (splits < 8 && mtiles * splits * 2 <= num_sms() && chunks >= splits * 8) splits *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)mtiles, splits);
+  cfg.blockDim = dim3(192);
+  cfg.dynamicSmemBytes = ShrinkSmem::total(Rp, splits);
+  cfg.stream = S_(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = splits;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, adapter_shrink_kernel, tx, ta, a);
+  if (e != cudaSuccess) return fail(H3_ERR_CUDA, "%s: cluster launch: %s", who, cudaGetErrorString(e));
+  if ((rc = check_launch(who))) return rc;
+  adapter_expand_kernel<<<(unsigned)(mtiles * ntiles), 160, ExpandSmem::total(Rp), S_(stream)>>>(ty, tt, tb, to, a);
   return check_launch(who);
 }
 

@@ -7,6 +7,9 @@ them): ``nvfp4_weight`` (:30-38), ``absmax`` (:41-45), ``Linear`` (:48-59), ``Bf
 Activation scales live on the device in H3ScaleSlot records (amax / act / used / margin), so the delayed-scale
 policy runs with no host read: ``MiniMaxH3Engine.begin_forward`` updates every slot in one kernel.  A standalone
 ``Nvfp4Linear`` call quantises under its input's own absmax (the reference's dynamic mode), also without a host sync.
+
+``adapter_add`` / ``AdapterSet`` add low-rank adapters beside a projection, a different one for each row's request (the
+reference merges one adapter set into the weights, comfy_nodes.py:95-166).
 """
 
 from __future__ import annotations
@@ -15,6 +18,7 @@ from functools import lru_cache
 
 import torch
 
+from . import native
 from . import native as N
 
 FP4_MAX, E4M3_MAX = 6.0, 448.0
@@ -198,6 +202,82 @@ class Nvfp4Linear(Linear):
 
     def nbytes(self) -> int:
         return self.codes.numel() + self.sf.numel() + 4
+
+
+def adapter_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor, rows: torch.Tensor,
+                scale: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """y[m] + B[a] (scale[a] A[a] x[m]) with a = rows[m], for bf16 x [M, K], y [M, N], A [n, R, K], B [n, N, R] (lower
+    ranks padded with zeros), scale fp32 [n] (None: 1) and rows int32 [M], in any order; a row whose entry is outside
+    [0, n) has no adapter and keeps y's bits.  In place on y, unless ``out`` names other memory (apart from the
+    inputs).  K, N and R multiples of 8, R <= 128."""
+
+    out = y if out is None else out
+    for name, t, d in (("y", y, 2), ("x", x, 2), ("A", A, 3), ("B", B, 3), ("out", out, 2)):
+        if t.dim() != d or t.dtype != torch.bfloat16:
+            raise ValueError(f"adapter_add: {name} must be a {d}-D bf16 tensor, got {tuple(t.shape)} {t.dtype}")
+    (M, K), (n, R), N = x.shape, A.shape[:2], y.shape[1]
+    if y.shape[0] != M or tuple(A.shape) != (n, R, K) or tuple(B.shape) != (n, N, R) or out.shape != y.shape:
+        raise ValueError(f"adapter_add: x {tuple(x.shape)}, y {tuple(y.shape)}, A {tuple(A.shape)}, B {tuple(B.shape)}, "
+                         f"out {tuple(out.shape)} do not fit together")
+    if tuple(rows.shape) != (M,) or rows.dtype != torch.int32:
+        raise ValueError(f"adapter_add: rows must be int32 [{M}], got {tuple(rows.shape)} {rows.dtype}")
+    if scale is not None and (tuple(scale.shape) != (n,) or scale.dtype != torch.float32):
+        raise ValueError(f"adapter_add: scale must be fp32 [{n}], got {tuple(scale.shape)} {scale.dtype}")
+    if K % 8 or N % 8 or R % 8 or R > 128:
+        raise ValueError(f"adapter_add: K, N and R must be multiples of 8 and R at most 128, got K={K} N={N} R={R}")
+    for name, t in (("y", y), ("out", out)):
+        if (N > 1 and t.stride(1) != 1) or t.stride(0) % 8 or (M > 1 and t.stride(0) < N) or t.data_ptr() % 16:
+            raise ValueError(f"adapter_add: {name} needs 16-byte aligned contiguous rows, got strides {t.stride()}")
+    x = x if x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.stride(0) >= K and x.data_ptr() % 16 == 0 else x.contiguous()
+    A, B, rows = A.contiguous(), B.contiguous(), rows.contiguous()
+    scale = None if scale is None else scale.contiguous()
+    with native.on_device("adapter_add", y, x, A, B, rows, out, *(() if scale is None else (scale,))) as stream:
+        if M and N and n and K and R:
+            ws = torch.empty(native.adapter_workspace_bytes(M, R), dtype=torch.uint8, device=x.device)
+            native.adapter_add(x, y, A, B, scale, rows, out, ws, stream)
+        elif out is not y:
+            out.copy_(y)
+    return out
+
+
+class AdapterSet:
+    """The low-rank adapters of several requests for one linear: ``pairs`` of (A [r, K], B [N, r]), ranks up to 128 and
+    any mix of them, and a ``scale`` for each (None: 1).  ``add(y, x, rows)`` adds each row's own adapter to y."""
+
+    def __init__(self, pairs, scales=None, device="cuda"):
+        if not pairs:
+            raise ValueError("AdapterSet: no adapters")
+        K, N = pairs[0][0].shape[1], pairs[0][1].shape[0]
+        for a, b in pairs:
+            if a.dim() != 2 or b.dim() != 2 or a.shape[1] != K or b.shape[0] != N or a.shape[0] != b.shape[1]:
+                raise ValueError(f"AdapterSet: A {tuple(a.shape)} and B {tuple(b.shape)} are not [r, {K}] and [{N}, r]")
+        R = (max(a.shape[0] for a, _ in pairs) + 7) // 8 * 8
+        if not 0 < R <= 128 or K % 8 or N % 8:
+            raise ValueError(f"AdapterSet: ranks up to 128, K and N multiples of 8, got rank {R}, K={K}, N={N}")
+        scales = [1.0] * len(pairs) if scales is None else [float(s) for s in scales]
+        if len(scales) != len(pairs):
+            raise ValueError(f"AdapterSet: {len(scales)} scales for {len(pairs)} adapters")
+        self.n, self.k, self.count = N, K, len(pairs)
+        self.A = torch.zeros((len(pairs), R, K), dtype=torch.bfloat16, device=device)
+        self.B = torch.zeros((len(pairs), N, R), dtype=torch.bfloat16, device=device)
+        for i, (a, b) in enumerate(pairs):
+            self.A[i, :a.shape[0]] = a.to(device)
+            self.B[i, :, :b.shape[1]] = b.to(device)
+        self.scale = torch.tensor(scales, dtype=torch.float32, device=device)
+
+    def interleaved16(self) -> "AdapterSet":
+        """The set for a [gate | up] linear whose output columns alternate in blocks of 16 (Nvfp4Linear's
+        ``interleave16``)."""
+
+        s = AdapterSet.__new__(AdapterSet)
+        s.n, s.k, s.count, s.A, s.scale = self.n, self.k, self.count, self.A, self.scale
+        if self.n % 32:
+            raise ValueError(f"AdapterSet: a 16-interleaved linear has a multiple of 32 outputs, got {self.n}")
+        s.B = self.B.view(self.count, 2, self.n // 32, 16, -1).transpose(1, 2).reshape(self.B.shape).contiguous()
+        return s
+
+    def add(self, y: torch.Tensor, x: torch.Tensor, rows: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+        return adapter_add(y, x, self.A, self.B, rows, self.scale, out)
 
 
 def update_delayed(lins, margin: float = DELAY_MARGIN) -> int:

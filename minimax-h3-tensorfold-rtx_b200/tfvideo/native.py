@@ -17,7 +17,7 @@ import torch
 LIB_PATH = Path(os.environ.get("H3B200_LIB") or Path(__file__).resolve().parent / "_native" / "libh3b200.so")
 
 H3_EPI_STORE, H3_EPI_GATE_RESID, H3_EPI_ACT_BF16, H3_EPI_ACT_Q, H3_EPI_STORE_PEERS = 0, 1, 2, 3, 4
-ACT_GELU, ACT_SWIGLU = 0, 1
+ACT_GELU, ACT_SWIGLU, ACT_SWIGLU16 = 0, 1, 2   # 2 (h3_act): SwiGLU of 16-column interleaved [gate | up]
 SLOT_FLOATS = 4   # H3ScaleSlot: amax, act, used, margin
 
 vp, i32, i64, f32, sz = C.c_void_p, C.c_int, C.c_longlong, C.c_float, C.c_size_t
@@ -55,6 +55,8 @@ _SIGS = {
     "h3_modulation": [vp, i32, i32, vp, vp, i32, vp, vp],
     "h3_gemm_nvfp4": [vp, vp, vp, vp, vp, f32, vp, i32, i32, i32, C.POINTER(H3Epilogue), vp],
     "h3_qknorm_rope": [vp, vp, i64, i32, i32, i32, vp, vp, vp, f32, vp],
+    "h3_adapter_workspace_bytes": ([i32, i32], sz),
+    "h3_adapter_add": [vp, i64, vp, i64, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, i64, vp, sz, vp],
     "h3_rope_axes": [C.POINTER(H3Positions), i32, vp, vp],
     "h3_qknorm_rope_axes": [vp, i64, i64, vp, i64, i64, i32, i32, i32, vp, vp, C.POINTER(H3Positions), f32, vp, i64,
                             i64, vp, i64, i64, vp],
@@ -170,6 +172,10 @@ def attn_workspace_bytes(S: int, H: int) -> int:
     return int(lib().h3_attn_workspace_bytes(S, H))
 
 
+def adapter_workspace_bytes(M: int, R: int) -> int:
+    return int(lib().h3_adapter_workspace_bytes(M, R))
+
+
 def slot_ptr(slots: torch.Tensor, i: int) -> int:
     """Address of H3ScaleSlot i in a float32 [n, 4] device tensor."""
 
@@ -255,6 +261,15 @@ def positions(pos: torch.Tensor, dims, theta) -> H3Positions:
     p.dims[:len(dims)] = dims
     p.theta[:len(dims)] = theta
     return p
+
+
+def adapter_add(x, y, A, B, scale, rows, out, workspace, stream_handle: int) -> None:
+    M, K = x.shape
+    n, N, R = B.shape
+    _count(2)
+    check(lib().h3_adapter_add(ptr(x), x.stride(0), ptr(y), y.stride(0), ptr(A), ptr(B), ptr(scale), ptr(rows), M, K, N,
+                               R, n, ptr(out), out.stride(0), ptr(workspace), workspace.numel(), stream_handle),
+          "h3_adapter_add")
 
 
 def rope_axes(pos: H3Positions, S: int, out: torch.Tensor, stream_handle: int) -> None:

@@ -140,3 +140,40 @@ def test_bf16_attention_refuses_bad_arguments():
                 (q.expand(2, 4, 10, 128), q, q), (q, q, q)):                  # the last: CPU tensors
         with pytest.raises(ValueError):
             A.bf16(*bad)
+
+
+def test_adapter_add_checks_its_arguments(lib):
+    from tfvideo import native as N
+
+    def call(x=FAKE, ldx=64, y=FAKE, ldy=64, rows=FAKE, M=10, K=64, N=64, R=16, n=2, out=FAKE, ldo=64, ws=FAKE, size=1 << 20):
+        return lib.h3_adapter_add(x, ldx, y, ldy, FAKE, FAKE, None, rows, M, K, N, R, n, out, ldo, ws, size, None)
+
+    for bad in (dict(x=None), dict(y=None), dict(rows=None), dict(out=None), dict(ws=None), dict(x=FAKE + 2),
+                dict(out=FAKE + 8), dict(rows=FAKE + 1), dict(size=10 * 32 - 1)):
+        assert call(**bad) == -1, bad
+    for bad in (dict(M=0), dict(K=0), dict(K=60), dict(N=4), dict(R=0), dict(R=12), dict(R=136), dict(n=0), dict(ldx=56),
+                dict(ldx=68), dict(ldy=56), dict(ldo=66)):
+        assert call(**bad) == -2, bad
+    assert lib.h3_adapter_workspace_bytes(10, 8) == 320 and lib.h3_adapter_workspace_bytes(0, 8) == 0
+    assert lib.h3_act(FAKE, 16, FAKE, 8, 4, 8, 2, None, None) == -2 and lib.h3_act(FAKE, 16, FAKE, 8, 4, 8, 3, None, None) == -1
+
+
+def test_adapters_refuse_bad_arguments():
+    from tfvideo import linear as L
+
+    b = lambda *s: torch.zeros(s, dtype=torch.bfloat16)                     # noqa: E731
+    good = dict(y=b(10, 64), x=b(10, 32), A=b(2, 8, 32), B=b(2, 64, 8), rows=torch.zeros(10, dtype=torch.int32))
+    for bad in (dict(y=b(9, 64)), dict(y=b(10, 64).float()), dict(x=b(10, 40)), dict(A=b(8, 32)), dict(B=b(2, 64, 16)),
+                dict(B=b(3, 64, 8)), dict(rows=torch.zeros(10)), dict(rows=torch.zeros(9, dtype=torch.int32)),
+                dict(scale=torch.zeros(3)), dict(scale=torch.zeros(2, dtype=torch.float64)), dict(out=b(10, 72)),
+                dict(out=b(10, 64).half()), dict(A=b(2, 4, 32), B=b(2, 64, 4)), dict(A=b(2, 136, 32), B=b(2, 64, 136)),
+                dict(y=b(64, 10).t()), dict(y=b(10, 68)[:, :64]), dict(y=b(10, 72)[:, 1:65]),
+                dict(out=b(1, 64).expand(10, 64)), dict()):                 # the last: CPU tensors
+        with pytest.raises(ValueError):
+            L.adapter_add(**{**good, **bad})
+    for pairs, scales in (([], None), ([(b(4, 32), b(64, 5))], None), ([(b(4, 32), b(64, 4)), (b(4, 40), b(64, 4))], None),
+                          ([(b(130, 32), b(64, 130))], None), ([(b(4, 30), b(64, 4))], None), ([(b(4, 32), b(64, 4))], [1, 2])):
+        with pytest.raises(ValueError):
+            L.AdapterSet(pairs, scales, device="cpu")
+    with pytest.raises(ValueError, match="32"):
+        L.AdapterSet([(b(4, 32), b(48, 4))], device="cpu").interleaved16()
