@@ -14,9 +14,11 @@ from __future__ import annotations
 
 import torch
 
+from .kernels import AxialPositions
+
 
 class StepGraph:
-    def __init__(self, engine, x: torch.Tensor, t_emb: torch.Tensor, mod_segments, rope_freqs: torch.Tensor):
+    def __init__(self, engine, x: torch.Tensor, t_emb: torch.Tensor, mod_segments, rope_freqs):
         if engine.sp is not None:
             raise ValueError("StepGraph: sequence-parallel engines are not captured")
         if not engine.delayed_scales:
@@ -24,7 +26,10 @@ class StepGraph:
         self.engine = engine
         self.x = x.detach().clone()
         self.t_emb = t_emb.detach().to(device=x.device, dtype=torch.float32).clone()
-        self.rope = rope_freqs.detach().to(device=x.device, dtype=torch.float32).contiguous()
+        if isinstance(rope_freqs, AxialPositions):
+            self.rope = AxialPositions(rope_freqs.pos.detach().to(x.device).clone(), rope_freqs.dims, rope_freqs.theta)
+        else:
+            self.rope = rope_freqs.detach().to(device=x.device, dtype=torch.float32).contiguous()
         self.mod_segments = mod_segments
         # one eager forward on a scratch copy when the run has none yet, so the captured forward is a delayed-scale
         # one; it also fills the engine's buffers and its row-index cache (nothing is allocated during capture)

@@ -12,6 +12,10 @@ B200 design, against the reference's (RTX 16 GB) one:
   * activation scales stay on the device (H3ScaleSlot): the first forward measures each input's absmax (dynamic),
     later forwards use the previous forward's absmax x margin (delayed) -- the reference's policy, with no host read;
   * with a process group, tokens are sharded over ranks and attention runs Ulysses head-parallel (tfvideo/parallel.py).
+
+Several requests may share one packed sequence: ``rope_freqs`` may be a kernels.AxialPositions (each token's position
+over time, height and width), ``attn_mask`` an attention.SpanMask with ``attn="bf16"`` (each token's keys), and
+``set_adapters`` gives every token its request's low-rank adapters beside the shared NVFP4 projections.
 """
 
 from __future__ import annotations
@@ -118,6 +122,7 @@ class _Buffers:
                 self.qkv_all = torch.empty((S, 3, Hl, cfg.head_dim), dtype=torch.bfloat16, **e)
                 self.o_recv = torch.empty((world, n, Hl * cfg.head_dim), dtype=torch.bfloat16, **e)
         self._dyn = None
+        self._proj = {}
 
     def dynamic(self, cfg: Config, n: int, device):
         """bf16 copies of h and the activation: only the first (dynamic-scale) forward writes them."""
@@ -127,10 +132,18 @@ class _Buffers:
                          torch.empty((n, cfg.ffn), dtype=torch.bfloat16, device=device))
         return self._dyn
 
+    def projection(self, n: int, cols: int, device):
+        """bf16 [n, cols] output of a projection whose epilogue is not fused, as one with adapters."""
+
+        if cols not in self._proj:
+            self._proj[cols] = torch.empty((n, cols), dtype=torch.bfloat16, device=device)
+        return self._proj[cols]
+
 
 class MiniMaxH3Engine:
     """The DiT blocks with NVFP4 linears on B200; ``attn`` picks the attention backend (fp8 by default).
-    ``attn_mask`` (an attention.TileMask for the sequence length) runs the FP8 attention block-sparse."""
+    ``attn_mask`` for the sequence length: an attention.TileMask runs the FP8 attention block-sparse, an
+    attention.SpanMask (``attn="bf16"``) gives every token its own span of keys."""
 
     MLP_CHUNK = None                      # the whole sequence at once (HBM holds it)
 
@@ -156,7 +169,9 @@ class MiniMaxH3Engine:
         self._rope_key = self._rope = None
         self.clipped = torch.zeros((), dtype=torch.int32, device=self.device)
         self.timer = None                  # a profiling.StageTimer to time each stage of each block
-        self.attn_mask = None              # attention.TileMask: block-sparse FP8 attention when set
+        self.attn_mask = None              # attention.TileMask (fp8) or attention.SpanMask (bf16) when set
+        self.adapters = {}                 # (block, linear name) -> linear.AdapterSet (set_adapters)
+        self.adapter_rows = None           # int32 [S]: each token's adapter
         self.qkv_parts = 4                 # Ulysses: row parts of the qkv GEMM (all but the last sent by copy engines)
         self.copy_streams = 7              # Ulysses: side streams for those copies (one per destination rank at 8)
         self.part_sender = "auto"          # Ulysses: "copy" (copy engines), "push" (a push kernel beside the GEMM),
@@ -222,6 +237,37 @@ class MiniMaxH3Engine:
         self.lora_sig = lora_sig
         self.end_run()
 
+    def set_adapters(self, adapters: dict, rows: torch.Tensor) -> None:
+        """Low-rank adapters beside the block linears, a different one for each request of the packed sequence:
+        ``adapters[(block, name)]`` is the linear.AdapterSet of block linear ``name`` (qkv, out, fc1, fc2; fc1 of a SwiGLU
+        model with [gate | up] outputs), ``rows`` int32 [S] each token's adapter in those sets (outside them: none).  They
+        stay until ``set_adapters({}, None)``; ``rows`` is read on the device, so it may be changed in place.  Against
+        merged weights (store.load_or_convert): no re-conversion, and as many sets at once as there are requests."""
+
+        if adapters and self.sp is not None:
+            raise ValueError("set_adapters: sequence-parallel engines run without adapters; merge them instead")
+        if adapters and (not torch.is_tensor(rows) or rows.dim() != 1 or rows.dtype != torch.int32
+                         or not rows.is_contiguous()):
+            raise ValueError("set_adapters: rows must be a contiguous int32 [S] tensor")
+        laid_out = {}
+        for (i, name), ad in adapters.items():
+            if not 0 <= i < len(self.blocks) or name not in LIN_NAMES:
+                raise ValueError(f"set_adapters: no linear {name!r} in block {i}")
+            lin = self.blocks[i].lins[name]
+            if (ad.n, ad.k) != (lin.n, lin.k):
+                raise ValueError(f"set_adapters: block {i} {name} is [{lin.n}, {lin.k}], its adapters [{ad.n}, {ad.k}]")
+            laid_out[(i, name)] = ad.interleaved16() if lin.interleaved else ad
+        self.adapters = laid_out
+        self.adapter_rows = rows.to(self.device) if adapters else None
+
+    def _adapter(self, i: int, name: str, S: int):
+        """The AdapterSet of block i's linear ``name`` (None: it has none), for a sequence of S tokens."""
+
+        ad = self.adapters.get((i, name))
+        if ad is not None and self.adapter_rows.shape[0] != S:
+            raise ValueError(f"adapter rows are for {self.adapter_rows.shape[0]} tokens, the sequence has {S}")
+        return ad
+
     def release_vram(self):
         self._buf = None
         torch.cuda.empty_cache()
@@ -243,14 +289,41 @@ class MiniMaxH3Engine:
         self._idx_key, self._idx_ref = (id(mod_segments), S), mod_segments
         return self._idx
 
-    def rope_table(self, rope_freqs: torch.Tensor, S: int) -> torch.Tensor:
-        """fp32 [S, rot/2, 2, 2] from ComfyUI's [1, S, 1, rot/2, 2, 2] rotation table (cached within a forward)."""
+    def rope_table(self, rope_freqs, S: int) -> torch.Tensor:
+        """fp32 [S, rot/2, 2, 2] from ComfyUI's [1, S, 1, rot/2, 2, 2] rotation table (cached within a forward), or
+        made from a kernels.AxialPositions."""
 
+        if isinstance(rope_freqs, K.AxialPositions):
+            p = self.rope_positions(rope_freqs, S)
+            return K.rope_axes(p.pos, p.dims, p.theta)
         key = (id(rope_freqs), rope_freqs.data_ptr(), rope_freqs._version)
         if key != self._rope_key:
             self._rope = rope_freqs.reshape(S, -1, 2, 2).to(device=self.device, dtype=torch.float32).contiguous()
             self._rope_key = key
         return self._rope
+
+    def rope_positions(self, p: "K.AxialPositions", S: int) -> "K.AxialPositions":
+        """The positions on the engine's device (moved there once a forward)."""
+
+        if len(p) != S:
+            raise ValueError(f"AxialPositions holds {len(p)} tokens, the sequence has {S}")
+        key = (id(p), p.pos.data_ptr(), p.pos._version)
+        if key != self._rope_key:
+            self._rope, self._rope_ref = p.to(self.device), p
+            self._rope_key = key
+        return self._rope
+
+    def _qknorm_rope(self, b: Block, q, k, ld: int, n: int, H: int, rope_freqs, S: int, t0: int) -> None:
+        """q, k RMSNorm + RoPE in place for tokens t0 .. t0 + n (rows of ld elements): from the positions when given,
+        else from the rotation table."""
+
+        if isinstance(rope_freqs, K.AxialPositions):
+            p = self.rope_positions(rope_freqs, S).rows(t0, t0 + n)
+            K.qknorm_rope_axes(q.unflatten(1, (H, -1)), k.unflatten(1, (H, -1)), b.q_norm, b.k_norm, p.pos, p.dims,
+                               p.theta, self.cfg.qk_eps)
+        else:
+            rope = self.rope_table(rope_freqs, S)
+            N.qknorm_rope(q, k, ld, n, H, rope.shape[1] * 2, b.q_norm, b.k_norm, rope[t0:t0 + n], self.cfg.qk_eps)
 
     def modulation(self, b: Block, t_emb: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """fp32 [M * 3, 6, D]: ada_b + t_emb @ ada_w^T viewed as ComfyUI's mod rows."""
@@ -308,28 +381,34 @@ class MiniMaxH3Engine:
         mod = self.modulation(b, t_emb.reshape(-1, t_emb.shape[-1]), buf.mod)
         delayed = self._delayed_now
         lq, lo, l1, l2 = (b.lins[k] for k in LIN_NAMES)
+        ad_qkv, ad_out = self._adapter(i, "qkv", S), self._adapter(i, "out", S)
 
         # ---- norm1 (+ NVFP4 of the qkv input)
-        if attention is not None or not delayed:
+        h = None
+        if attention is not None or not delayed or ad_qkv is not None:
             h = buf.dynamic(cfg, n, self.device)[0]
+        if attention is not None or not delayed:
             N.norm_mod(x, b.norm1, mod, idx, 0, cfg.eps, out=h, slot=self._slot(i, "qkv"))
         if attention is not None:
             # An attention override handed in by ComfyUI (a sparse-attention patch, for instance) owns the whole
             # attention half: given the normed input it computes qkv, q/k norms, RoPE and attention through
             # EngineBlock.attn and returns the out-projection's output, which the gate adds to the residual here.
-            a = attention(h, rope_freqs=rope_freqs, transformer_options=transformer_options or {})
+            if isinstance(rope_freqs, K.AxialPositions):
+                table = self.rope_table(rope_freqs, S)[None, :, None]
+            else:
+                table = rope_freqs
+            a = attention(h, rope_freqs=table, transformer_options=transformer_options or {})
             K.gate_add(x, a, mod, 0, idx)
             return self._mlp_half(i, b, x, mod, idx, buf, delayed)
         T = self.timer
         with maybe(T, "norm_mod+quant"):
             if delayed:
-                N.norm_mod(x, b.norm1, mod, idx, 0, cfg.eps, codes=buf.h4, sf=buf.h4sf, slot=self._slot(i, "qkv"))
+                N.norm_mod(x, b.norm1, mod, idx, 0, cfg.eps, out=h, codes=buf.h4, sf=buf.h4sf,
+                           slot=self._slot(i, "qkv"))
             else:
                 self._dynamic_scale(i, "qkv")
                 N.nvfp4_quant(h, buf.h4, buf.h4sf, g_ptr=self._slot(i, "qkv") + 4)
         # ---- qkv, q/k RMSNorm + RoPE, attention
-        rope_all = self.rope_table(rope_freqs, S)
-        rot = rope_all.shape[1] * 2
         ws = A.aligned_workspace(buf.attn_ws)
         if self.sp is not None and buf.peers is not None and self.attn is A.fp8:
             # Ulysses with the exchanges in the producing kernels: the qkv GEMM's epilogue writes each head's columns
@@ -377,11 +456,9 @@ class MiniMaxH3Engine:
             qa = buf.qkv_all.view(S, 3 * Hl * Dh)
             q, k, v = qa[:, :Hl * Dh], qa[:, Hl * Dh:2 * Hl * Dh], qa[:, 2 * Hl * Dh:]
             with maybe(T, "qknorm_rope"):
-                N.qknorm_rope(q, k, 3 * Hl * Dh, S, Hl, rot, b.q_norm, b.k_norm, rope_all, cfg.qk_eps)
+                self._qknorm_rope(b, q, k, 3 * Hl * Dh, S, Hl, rope_freqs, S, 0)
             with maybe(T, "attention"):
-                m = self.attn_mask
-                if m is not None and m.S != S:
-                    raise ValueError(f"attn_mask is for S={m.S}, the sequence has S={S}")
+                m = self._mask(S)
                 N.attn_fp8_peers(q, k, v, 3 * Hl * Dh, Dh, S, Hl, op.ptrs, rank, Hl * Dh, ws,
                                  kv_ptr=None if m is None else m.kv_ptr, kv_idx=None if m is None else m.kv_idx)
             with maybe(T, "exchange_barrier"):
@@ -390,10 +467,12 @@ class MiniMaxH3Engine:
         else:
             with maybe(T, "gemm_qkv"):
                 lq.gemm(buf.h4, buf.h4sf, n, N.H3Epilogue(kind=N.H3_EPI_STORE, out=buf.qkv.data_ptr(), ldo=3 * HD))
-            rope = rope_all[t0:t0 + n]
+            if ad_qkv is not None:
+                with maybe(T, "adapters"):
+                    ad_qkv.add(buf.qkv, h, self.adapter_rows)
             q, k, v = buf.qkv[:, :HD], buf.qkv[:, HD:2 * HD], buf.qkv[:, 2 * HD:]
             with maybe(T, "qknorm_rope"):
-                N.qknorm_rope(q, k, 3 * HD, n, H, rot, b.q_norm, b.k_norm, rope, cfg.qk_eps)
+                self._qknorm_rope(b, q, k, 3 * HD, n, H, rope_freqs, S, t0)
             if self.sp is None:
                 with maybe(T, "attention"):
                     self._attend(q, k, v, S, H, 3 * HD, buf.o, ws)
@@ -418,9 +497,12 @@ class MiniMaxH3Engine:
                 N.absmax_into(src["x"].reshape(-1, src["x"].shape[-1]), sl)
                 self._dynamic_scale(i, "out")
                 N.nvfp4_quant(codes=buf.o4, sf=buf.o4sf, g_ptr=sl + 4, **src)
-        with maybe(T, "gemm_out+gate"):
-            lo.gemm(buf.o4, buf.o4sf, n, N.H3Epilogue(kind=N.H3_EPI_GATE_RESID, x=x.data_ptr(), ldx=D,
-                                                      mod=mod.data_ptr(), idx=idx.data_ptr(), gate_part=0))
+        if ad_out is not None:
+            self._project_add(lo, buf.o4, buf.o4sf, x, mod, idx, 0, ad_out, buf.o, buf)
+        else:
+            with maybe(T, "gemm_out+gate"):
+                lo.gemm(buf.o4, buf.o4sf, n, N.H3Epilogue(kind=N.H3_EPI_GATE_RESID, x=x.data_ptr(), ldx=D,
+                                                          mod=mod.data_ptr(), idx=idx.data_ptr(), gate_part=0))
         x = self._mlp_half(i, b, x, mod, idx, buf, delayed)
         if buf.peers is not None and i == len(self.blocks) - 1:
             # the last block of a Ulysses forward: every barrier of the forward carried the ranks' device status;
@@ -431,11 +513,38 @@ class MiniMaxH3Engine:
                                    f"{status}); the receive buffers of this forward are incomplete")
         return x
 
-    def _attend(self, q, k, v, S, H, ld, out, ws):
+    def _project_add(self, lin, codes, sf, x, mod, idx, part, ad, src, buf) -> None:
+        """x += (lin(input) + its rows' adapters on the bf16 input ``src``) * gate: the adapters join the projection
+        before the gate, so its epilogue stores instead of gating."""
+
+        n, D = x.shape
+        t = buf.projection(n, D, self.device)
+        with maybe(self.timer, "gemm_store"):
+            lin.gemm(codes, sf, n, N.H3Epilogue(kind=N.H3_EPI_STORE, out=t.data_ptr(), ldo=D))
+        with maybe(self.timer, "adapters"):
+            ad.add(t, src, self.adapter_rows)
+        with maybe(self.timer, "gate_add"):
+            N.gate_add(x, t, mod, idx, part)
+
+    def _mask(self, S: int):
+        """``attn_mask``, checked against the attention backend and the sequence length (library backends take none:
+        they ignore a TileMask, as ever, and are refused with a SpanMask)."""
+
         m = self.attn_mask
-        if self.attn is A.fp8 and m is not None:
-            if m.S != S:
-                raise ValueError(f"attn_mask is for S={m.S}, the sequence has S={S}")
+        if m is None or not (isinstance(m, A.SpanMask) or self.attn in (A.fp8, A.bf16)):
+            return None
+        if m.S != S:
+            raise ValueError(f"attn_mask is for S={m.S}, the sequence has S={S}")
+        if isinstance(m, A.SpanMask) != (self.attn is A.bf16):
+            raise ValueError(f"attn_mask is a {type(m).__name__}: a SpanMask needs attn='bf16', a TileMask attn='fp8' "
+                             f"(the engine has attn={self.attn_name!r})")
+        return m
+
+    def _attend(self, q, k, v, S, H, ld, out, ws):
+        m = self._mask(S)
+        if self.attn is A.bf16:
+            A.bf16_tokens(*(t.unflatten(1, (H, -1)) for t in (q, k, v)), out, m)
+        elif self.attn is A.fp8 and m is not None:
             N.attn_fp8_sparse(q, k, v, ld, self.cfg.head_dim, S, H, m.kv_ptr, m.kv_idx, out, out.stride(0), ws)
         elif self.attn is A.fp8:
             N.attn_fp8(q, k, v, ld, self.cfg.head_dim, S, H, out, out.stride(0), ws)
@@ -452,25 +561,45 @@ class MiniMaxH3Engine:
         act_kind = N.ACT_SWIGLU if cfg.act == "swiglu" else N.ACT_GELU
         s1, s2 = self._slot(i, "fc1"), self._slot(i, "fc2")
         T = self.timer
+        ad1, ad2 = self._adapter(i, "fc1", n), self._adapter(i, "fc2", n)
+        h = a = None
+        if not delayed or ad1 is not None or ad2 is not None:
+            h, a = buf.dynamic(cfg, n, self.device)
         if delayed:
             with maybe(T, "norm_mod+quant"):
-                N.norm_mod(x, b.norm2, mod, idx, 1, cfg.eps, codes=buf.h4, sf=buf.h4sf, slot=s1)
-            with maybe(T, "gemm_fc1+act+quant"):
-                l1.gemm(buf.h4, buf.h4sf, n, N.H3Epilogue(kind=N.H3_EPI_ACT_Q, act_kind=act_kind,
-                                                          qcodes=buf.a4.data_ptr(), qsf=buf.a4sf.data_ptr(),
-                                                          q_slot=s2))
+                N.norm_mod(x, b.norm2, mod, idx, 1, cfg.eps, out=None if ad1 is None else h, codes=buf.h4, sf=buf.h4sf,
+                           slot=s1)
         else:
-            h, a = buf.dynamic(cfg, n, self.device)
             N.norm_mod(x, b.norm2, mod, idx, 1, cfg.eps, out=h, slot=s1)
             self._dynamic_scale(i, "fc1")
             N.nvfp4_quant(h, buf.h4, buf.h4sf, g_ptr=s1 + 4)
+        if ad1 is not None:   # the adapters join fc1 before its activation
+            u = buf.projection(n, cfg.fc1_out, self.device)
+            with maybe(T, "gemm_store"):
+                l1.gemm(buf.h4, buf.h4sf, n, N.H3Epilogue(kind=N.H3_EPI_STORE, out=u.data_ptr(), ldo=cfg.fc1_out))
+            with maybe(T, "adapters"):
+                ad1.add(u, h, self.adapter_rows)
+            with maybe(T, "act+quant"):
+                N.act(u, a, N.ACT_SWIGLU16 if l1.interleaved else act_kind, s2)
+        elif delayed:
+            with maybe(T, "gemm_fc1+act+quant"):
+                l1.gemm(buf.h4, buf.h4sf, n,
+                        N.H3Epilogue(kind=N.H3_EPI_ACT_Q, act_kind=act_kind, qcodes=buf.a4.data_ptr(),
+                                     qsf=buf.a4sf.data_ptr(), q_slot=s2, out=None if ad2 is None else a.data_ptr(),
+                                     ldo=0 if ad2 is None else a.stride(0)))
+        else:
             l1.gemm(buf.h4, buf.h4sf, n, N.H3Epilogue(kind=N.H3_EPI_ACT_BF16, act_kind=act_kind, out=a.data_ptr(),
                                                       ldo=a.stride(0), q_slot=s2))
+        if not delayed:
             self._dynamic_scale(i, "fc2")
+        if ad1 is not None or not delayed:
             N.nvfp4_quant(a, buf.a4, buf.a4sf, g_ptr=s2 + 4)
-        with maybe(T, "gemm_fc2+gate"):
-            l2.gemm(buf.a4, buf.a4sf, n, N.H3Epilogue(kind=N.H3_EPI_GATE_RESID, x=x.data_ptr(), ldx=cfg.dim,
-                                                      mod=mod.data_ptr(), idx=idx.data_ptr(), gate_part=1))
+        if ad2 is not None:
+            self._project_add(l2, buf.a4, buf.a4sf, x, mod, idx, 1, ad2, a, buf)
+        else:
+            with maybe(T, "gemm_fc2+gate"):
+                l2.gemm(buf.a4, buf.a4sf, n, N.H3Epilogue(kind=N.H3_EPI_GATE_RESID, x=x.data_ptr(), ldx=cfg.dim,
+                                                          mod=mod.data_ptr(), idx=idx.data_ptr(), gate_part=1))
         return x
 
     def forward(self, x, t_emb, mod_segments, rope_freqs, transformer_options=None):
@@ -503,7 +632,10 @@ class _Proj:
         self.engine, self.i, self.name = engine, i, name
 
     def __call__(self, x):
-        return self.engine.blocks[self.i].lins[self.name](x.contiguous())
+        x = x.contiguous()
+        y = self.engine.blocks[self.i].lins[self.name](x)
+        ad = self.engine._adapter(self.i, self.name, x.shape[0])
+        return y if ad is None else ad.add(y, x, self.engine.adapter_rows)
 
 
 class _Norm:
