@@ -184,38 +184,47 @@ def bf16_tokens(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Te
     """Low-level form: q [S, Hq, 128], k and v [S, Hk, 128] bf16 views (token and head strides multiples of 8,
     16-byte aligned); out [S, Hq * 128] bf16, row stride a multiple of 8."""
 
-    S, Hq, _ = q.shape
-    if mask is not None and mask.S != S:
-        raise ValueError(f"SpanMask is for S={mask.S}, attention has S={S}")
-    lo, hi = (None, None) if mask is None else (mask.lo, mask.hi)
-    with N.on_device("bf16 attention", q, k, v, out, *(() if mask is None else (lo, hi))) as stream:
-        if S and Hq:
-            N.attn_bf16(q, q.stride(0), q.stride(1), k, k.stride(0), k.stride(1), v, v.stride(0), v.stride(1), S, Hq,
-                        k.shape[1], lo, hi, out, out.stride(0), stream)
+    (S, Hq, _), Hk = q.shape, k.shape[1]
+    _bf16_launch(S, Hq, Hk, [(t, t.stride(0), t.stride(1)) for t in (q, k, v)], out, mask)
     return out
 
 
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """t [1, H, S, 128] as [S, H, 128] rows the kernel can read in place, copied when its strides do not allow it."""
+def _bf16_launch(S: int, Hq: int, Hk: int, rows, out: torch.Tensor, mask: SpanMask | None) -> None:
+    """``rows``: (tensor, token stride, head stride) of q, k and v."""
 
-    x = t[0].transpose(0, 1)
-    S, H, _ = x.shape
-    if x.stride(2) != 1 or x.data_ptr() % 16 or (S > 1 and (x.stride(0) % 8 or x.stride(0) <= 0)) \
-            or (H > 1 and (x.stride(1) % 8 or x.stride(1) <= 0)):
-        x = x.contiguous()
-    return x
+    (q, ldq, hsq), (k, ldk, hsk), (v, ldv, hsv) = rows
+    if mask is None:
+        lo = hi = None
+        dev = N.one_device("bf16 attention", q, k, v, out)
+    else:
+        if mask.S != S:
+            raise ValueError(f"SpanMask is for S={mask.S}, attention has S={S}")
+        lo, hi = mask.lo.data_ptr(), mask.hi.data_ptr()
+        dev = N.one_device("bf16 attention", q, k, v, out, mask.lo, mask.hi)
+    if S and Hq:
+        N.launch(dev, "h3_attn_bf16", 1, q.data_ptr(), ldq, hsq, k.data_ptr(), ldk, hsk, v.data_ptr(), ldv, hsv, S, Hq,
+                 Hk, lo, hi, out.data_ptr(), out.stride(0))
 
 
 def bf16(q, k, v, mask: SpanMask | None = None):
+    rows = []
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 4 or t.shape[0] != 1 or t.shape[3] != HEAD_DIM or t.dtype != torch.bfloat16:
             raise ValueError(f"bf16 attention: {name} must be bf16 [1, H, S, {HEAD_DIM}], got {tuple(t.shape)} {t.dtype}")
+        _, hs, ld, ds = t.stride()
+        # read in place by TMA; copied when the strides do not allow it (a dimension of one entry has any)
+        if ds != 1 or t.data_ptr() % 16 or (t.shape[2] > 1 and (ld % 8 or ld <= 0)) \
+                or (t.shape[1] > 1 and (hs % 8 or hs <= 0)):
+            t = N.aligned16(t)
+            _, hs, ld, ds = t.stride()
+        rows.append((t, ld, hs))
     _, H, S, D = q.shape
-    if k.shape != v.shape or k.shape[2] != S or k.shape[1] == 0 or H % k.shape[1]:
+    Hk = k.shape[1]
+    if k.shape != v.shape or k.shape[2] != S or Hk == 0 or H % Hk:
         raise ValueError(f"bf16 attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: one length, and "
                          "query heads a multiple of the key heads")
     out = torch.empty((S, H * D), dtype=torch.bfloat16, device=q.device)
-    bf16_tokens(_rows16(q), _rows16(k), _rows16(v), out, mask)
+    _bf16_launch(S, H, Hk, rows, out, mask)
     return out.view(1, S, H, D).transpose(1, 2)
 
 

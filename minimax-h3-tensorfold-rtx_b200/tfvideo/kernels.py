@@ -10,6 +10,9 @@ rotation table; ``AxialPositions`` bundles them for ``EngineBlock`` and ``StepGr
 
 from __future__ import annotations
 
+import ctypes as C
+from functools import lru_cache
+
 import torch
 
 from . import native as N
@@ -23,19 +26,32 @@ def _check_rows(x: torch.Tensor, name: str) -> None:
 HEAD_DIM = 128
 
 
-def _check_positions(what: str, pos: torch.Tensor, dims, theta) -> tuple[tuple[int, ...], tuple[float, ...]]:
+@lru_cache(maxsize=64)
+def _axes(what: str, dims: tuple, theta) -> tuple:
+    """Validated (dims, theta per axis, rot, the two as H3Positions holds them)."""
+
     dims = tuple(int(d) for d in dims)
-    theta = (float(theta),) * len(dims) if isinstance(theta, (int, float)) else tuple(float(t) for t in theta)
-    if pos.dim() != 2 or pos.dtype not in N.POS_TYPES:
-        raise ValueError(f"{what}: pos must be an int32, int64 or fp32 [S, axes] tensor, got {tuple(pos.shape)} "
-                         f"{pos.dtype}")
-    if not 1 <= len(dims) <= 4 or len(dims) != pos.shape[1] or len(theta) != len(dims):
-        raise ValueError(f"{what}: pos has {pos.shape[1]} axes, dims {len(dims)}, theta {len(theta)} (1 to 4 of each)")
+    theta = tuple(float(t) for t in theta) if isinstance(theta, tuple) else (float(theta),) * len(dims)
+    if not 1 <= len(dims) <= 4 or len(theta) != len(dims):
+        raise ValueError(f"{what}: 1 to 4 axes and one theta for each or for all, got dims {dims}, theta {theta}")
     if any(d <= 0 or d % 2 for d in dims) or sum(dims) > HEAD_DIM:
         raise ValueError(f"{what}: each axis rotates an even number of dims, together at most {HEAD_DIM}, got {dims}")
     if any(not 0.0 < t < float("inf") for t in theta):
         raise ValueError(f"{what}: theta must be positive and finite, got {theta}")
-    return dims, theta
+    n = len(dims)
+    return dims, theta, sum(dims), (N.i32 * 4)(*dims, *(0,) * (4 - n)), (C.c_double * 4)(*theta, *(1.0,) * (4 - n))
+
+
+def _check_positions(what: str, pos: torch.Tensor, dims, theta) -> tuple:
+    axes = _axes(what, tuple(dims), tuple(theta) if isinstance(theta, (list, tuple)) else theta)
+    if pos.dim() != 2 or pos.dtype not in N.POS_TYPES or pos.shape[1] != len(axes[0]):
+        raise ValueError(f"{what}: pos must be an int32, int64 or fp32 [S, {len(axes[0])}] tensor, got "
+                         f"{tuple(pos.shape)} {pos.dtype}")
+    return axes
+
+
+def _positions(pos: torch.Tensor, axes: tuple) -> N.H3Positions:
+    return N.H3Positions(pos.data_ptr(), N.POS_TYPES[pos.dtype], *pos.stride(), len(axes[0]), axes[3], axes[4])
 
 
 def rope_axes(pos: torch.Tensor, dims, theta=10000.0, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -44,15 +60,16 @@ def rope_axes(pos: torch.Tensor, dims, theta=10000.0, out: torch.Tensor | None =
     pos[s, a] * theta^(-2j / dims[a]), formed in 64 bits; pairs of the axes one after another.  ``theta``: one number,
     or one per axis."""
 
-    dims, theta = _check_positions("rope_axes", pos, dims, theta)
-    shape = (pos.shape[0], sum(dims) // 2, 2, 2)
+    axes = _check_positions("rope_axes", pos, dims, theta)
+    S = pos.shape[0]
+    shape = (S, axes[2] // 2, 2, 2)
     if out is None:
         out = torch.empty(shape, dtype=torch.float32, device=pos.device)
-    elif tuple(out.shape) != shape or out.dtype != torch.float32 or not out.is_contiguous():
+    elif out.shape != shape or out.dtype != torch.float32 or not out.is_contiguous():
         raise ValueError(f"rope_axes: out must be a contiguous fp32 {shape} tensor, got {tuple(out.shape)} {out.dtype}")
-    with N.on_device("rope_axes", pos, out) as stream:
-        if shape[0]:
-            N.rope_axes(N.positions(pos, dims, theta), shape[0], out, stream)
+    dev = N.one_device("rope_axes", pos, out)
+    if S:
+        N.launch(dev, "h3_rope_axes", 1, C.byref(_positions(pos, axes)), S, out.data_ptr())
     return out
 
 
@@ -63,32 +80,39 @@ def qknorm_rope_axes(q: torch.Tensor, k: torch.Tensor, qw: torch.Tensor, kw: tor
     [128]) and the split-half rotation of their first rot dims by ``rope_axes``'s angles, in one pass with no table.
     In place, unless ``out_q`` / ``out_k`` name other memory (apart from the inputs).  rot % 8 == 0."""
 
-    dims, theta = _check_positions("qknorm_rope_axes", pos, dims, theta)
+    axes = _check_positions("qknorm_rope_axes", pos, dims, theta)
     oq, ok = q if out_q is None else out_q, k if out_k is None else out_k
+    st = []
     for name, t, like in (("q", q, q), ("k", k, k), ("out_q", oq, q), ("out_k", ok, k)):
-        if t.dim() != 3 or t.shape[2] != HEAD_DIM or t.shape != like.shape or t.dtype != torch.bfloat16 \
-                or t.stride(2) != 1:
-            raise ValueError(f"qknorm_rope_axes: {name} must be bf16 [S, H, {HEAD_DIM}] with a contiguous head dim, got "
-                             f"{tuple(t.shape)} {t.dtype} strides {t.stride()}")
-        if t.stride(0) % 4 or t.stride(1) % 4 or t.data_ptr() % 8:
-            raise ValueError(f"qknorm_rope_axes: {name} needs 8-byte aligned rows, got strides {t.stride()}")
-    if not q.shape[0] == k.shape[0] == pos.shape[0]:
-        raise ValueError(f"qknorm_rope_axes: q has {q.shape[0]} tokens, k {k.shape[0]}, pos {pos.shape[0]}")
-    if sum(dims) % 8:
-        raise ValueError(f"qknorm_rope_axes: the rotated dims must be a multiple of 8, got {dims}")
+        if t.dim() != 3 or t.shape[2] != HEAD_DIM or t.shape != like.shape or t.dtype != torch.bfloat16:
+            raise ValueError(f"qknorm_rope_axes: {name} must be bf16 [S, H, {HEAD_DIM}], got {tuple(t.shape)} {t.dtype}")
+        ld, hs, ds = t.stride()
+        if ds != 1 or ld % 4 or hs % 4 or t.data_ptr() % 8:
+            raise ValueError(f"qknorm_rope_axes: {name} needs a contiguous head dim and 8-byte aligned rows, got strides "
+                             f"{t.stride()}")
+        st.append((t.data_ptr(), ld, hs))
+    (S, Hq, _), Hk = q.shape, k.shape[1]
+    if k.shape[0] != S or pos.shape[0] != S:
+        raise ValueError(f"qknorm_rope_axes: q has {S} tokens, k {k.shape[0]}, pos {pos.shape[0]}")
+    if axes[2] % 8:
+        raise ValueError(f"qknorm_rope_axes: the rotated dims must be a multiple of 8, got {axes[0]}")
     if qw.numel() != HEAD_DIM or kw.numel() != HEAD_DIM:
         raise ValueError(f"qknorm_rope_axes: norm weights have {HEAD_DIM} elements")
+    if S and (Hq == 0) != (Hk == 0):
+        raise ValueError("qknorm_rope_axes: q and k need at least one head each")
     qw, kw = _norm_weight(qw), _norm_weight(kw)
-    with N.on_device("qknorm_rope_axes", q, k, oq, ok, qw, kw, pos) as stream:
-        if q.shape[0] and q.shape[1] and k.shape[1]:
-            N.qknorm_rope_axes(q, k, qw, kw, N.positions(pos, dims, theta), eps, oq, ok, stream)
-        elif q.shape[0] and q.shape[1] + k.shape[1]:
-            raise ValueError("qknorm_rope_axes: q and k need at least one head each")
+    dev = N.one_device("qknorm_rope_axes", q, k, oq, ok, qw, kw, pos)
+    if S and Hq:
+        N.launch(dev, "h3_qknorm_rope_axes", 1, *st[0], *st[1], S, Hq, Hk, qw.data_ptr(), kw.data_ptr(),
+                 C.byref(_positions(pos, axes)), eps, *st[2], *st[3])
     return oq, ok
 
 
 def _norm_weight(w: torch.Tensor) -> torch.Tensor:
-    w = w.reshape(-1).float().contiguous()
+    """fp32 [128], contiguous, 16-byte aligned."""
+
+    if w.dtype != torch.float32 or not w.is_contiguous():
+        w = w.float().contiguous()
     return w if w.data_ptr() % 16 == 0 else w.clone()
 
 
@@ -97,7 +121,7 @@ class AxialPositions:
     each axis rotates and theta, as for ``rope_axes``.  ``EngineBlock`` takes one as its ``rope_freqs``."""
 
     def __init__(self, pos: torch.Tensor, dims, theta=10000.0):
-        self.dims, self.theta = _check_positions("AxialPositions", pos, dims, theta)
+        self.dims, self.theta = _check_positions("AxialPositions", pos, dims, theta)[:2]
         self.pos = pos
 
     def __len__(self) -> int:

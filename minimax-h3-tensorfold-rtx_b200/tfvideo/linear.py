@@ -18,7 +18,6 @@ from functools import lru_cache
 
 import torch
 
-from . import native
 from . import native as N
 
 FP4_MAX, E4M3_MAX = 6.0, 448.0
@@ -215,28 +214,38 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tens
     for name, t, d in (("y", y, 2), ("x", x, 2), ("A", A, 3), ("B", B, 3), ("out", out, 2)):
         if t.dim() != d or t.dtype != torch.bfloat16:
             raise ValueError(f"adapter_add: {name} must be a {d}-D bf16 tensor, got {tuple(t.shape)} {t.dtype}")
-    (M, K), (n, R), N = x.shape, A.shape[:2], y.shape[1]
-    if y.shape[0] != M or tuple(A.shape) != (n, R, K) or tuple(B.shape) != (n, N, R) or out.shape != y.shape:
+    (M, K), (n, R, Ka), cols = x.shape, A.shape, y.shape[1]
+    if y.shape[0] != M or Ka != K or B.shape != (n, cols, R) or out.shape != y.shape:
         raise ValueError(f"adapter_add: x {tuple(x.shape)}, y {tuple(y.shape)}, A {tuple(A.shape)}, B {tuple(B.shape)}, "
                          f"out {tuple(out.shape)} do not fit together")
-    if tuple(rows.shape) != (M,) or rows.dtype != torch.int32:
+    if rows.shape != (M,) or rows.dtype != torch.int32:
         raise ValueError(f"adapter_add: rows must be int32 [{M}], got {tuple(rows.shape)} {rows.dtype}")
-    if scale is not None and (tuple(scale.shape) != (n,) or scale.dtype != torch.float32):
+    if scale is not None and (scale.shape != (n,) or scale.dtype != torch.float32):
         raise ValueError(f"adapter_add: scale must be fp32 [{n}], got {tuple(scale.shape)} {scale.dtype}")
-    if K % 8 or N % 8 or R % 8 or R > 128:
-        raise ValueError(f"adapter_add: K, N and R must be multiples of 8 and R at most 128, got K={K} N={N} R={R}")
+    if K % 8 or cols % 8 or R % 8 or R > 128:
+        raise ValueError(f"adapter_add: K, N and R must be multiples of 8 and R at most 128, got K={K} N={cols} R={R}")
     for name, t in (("y", y), ("out", out)):
-        if (N > 1 and t.stride(1) != 1) or t.stride(0) % 8 or (M > 1 and t.stride(0) < N) or t.data_ptr() % 16:
+        ld, cs = t.stride()
+        if (cols > 1 and cs != 1) or ld % 8 or (M > 1 and ld < cols) or t.data_ptr() % 16:
             raise ValueError(f"adapter_add: {name} needs 16-byte aligned contiguous rows, got strides {t.stride()}")
-    x = x if x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.stride(0) >= K and x.data_ptr() % 16 == 0 else x.contiguous()
-    A, B, rows = A.contiguous(), B.contiguous(), rows.contiguous()
-    scale = None if scale is None else scale.contiguous()
-    with native.on_device("adapter_add", y, x, A, B, rows, out, *(() if scale is None else (scale,))) as stream:
-        if M and N and n and K and R:
-            ws = torch.empty(native.adapter_workspace_bytes(M, R), dtype=torch.uint8, device=x.device)
-            native.adapter_add(x, y, A, B, scale, rows, out, ws, stream)
-        elif out is not y:
-            out.copy_(y)
+    ldx, cs = x.stride()
+    if cs != 1 or ldx % 8 or ldx < K or x.data_ptr() % 16:
+        x = N.aligned16(x)
+        ldx = x.stride(0)
+    A, B, rows = N.aligned16(A), N.aligned16(B), rows.contiguous()
+    if scale is None:
+        dev = N.one_device("adapter_add", y, x, A, B, rows, out)
+    else:
+        scale = scale.contiguous()
+        dev = N.one_device("adapter_add", y, x, A, B, rows, out, scale)
+    if M and cols and n and K and R:
+        size = N.adapter_workspace_bytes(M, R)
+        ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+        N.launch(dev, "h3_adapter_add", 2, x.data_ptr(), ldx, y.data_ptr(), y.stride(0), A.data_ptr(), B.data_ptr(),
+                 None if scale is None else scale.data_ptr(), rows.data_ptr(), M, K, cols, R, n, out.data_ptr(),
+                 out.stride(0), ws.data_ptr(), size)
+    elif out is not y:
+        out.copy_(y)
     return out
 
 

@@ -143,25 +143,37 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return t.data_ptr()
 
 
-class on_device:
-    """The device all the given tensors are on, made current for a launch, and its current stream:
-    ``with on_device(what, a, b, ...) as stream``.  ValueError when one is not a CUDA tensor or they are apart."""
+def one_device(what: str, *tensors: torch.Tensor) -> int:
+    """The index of the CUDA device all the given tensors are on; ValueError when there is no such device."""
 
-    def __init__(self, what: str, *tensors: torch.Tensor):
-        dev = tensors[0].device
-        if any(t.device != dev for t in tensors) or dev.type != "cuda":
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != dev or dev < 0:
             raise ValueError(f"{what}: all tensors must be on one CUDA device, got "
                              f"{', '.join(sorted({str(t.device) for t in tensors}))}")
-        self._guard = torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else None
+    return dev
 
-    def __enter__(self) -> int:
-        if self._guard is not None:
-            self._guard.__enter__()
-        return stream()
 
-    def __exit__(self, *exc) -> None:
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
+def aligned16(t: torch.Tensor) -> torch.Tensor:
+    """t itself when it is contiguous and 16-byte aligned, else a copy that is."""
+
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def launch(dev: int, name: str, kernels: int, *args) -> None:
+    """Entry point ``name`` with ``args`` and device ``dev``'s current stream, with that device current (it may not be
+    the caller's).  Takes a microsecond or two beside the entry point itself: small calls are bound by their host time."""
+
+    _count(kernels)
+    fn = getattr(_lib or lib(), name)
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        check(rc, name)
 
 
 def sf_tiled_bytes(rows: int, cols: int) -> int:
@@ -253,40 +265,6 @@ def qknorm_rope(q, k, ld, S, H, rot, qw, kw, rope, eps) -> None:
 POS_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 
 
-def positions(pos: torch.Tensor, dims, theta) -> H3Positions:
-    """The H3Positions of a [S, axes] position tensor (``theta``: one per axis)."""
-
-    p = H3Positions(pos=pos.data_ptr(), type=POS_TYPES[pos.dtype], ld=pos.stride(0), axis_stride=pos.stride(1),
-                    axes=len(dims))
-    p.dims[:len(dims)] = dims
-    p.theta[:len(dims)] = theta
-    return p
-
-
-def adapter_add(x, y, A, B, scale, rows, out, workspace, stream_handle: int) -> None:
-    M, K = x.shape
-    n, N, R = B.shape
-    _count(2)
-    check(lib().h3_adapter_add(ptr(x), x.stride(0), ptr(y), y.stride(0), ptr(A), ptr(B), ptr(scale), ptr(rows), M, K, N,
-                               R, n, ptr(out), out.stride(0), ptr(workspace), workspace.numel(), stream_handle),
-          "h3_adapter_add")
-
-
-def rope_axes(pos: H3Positions, S: int, out: torch.Tensor, stream_handle: int) -> None:
-    _count(1)
-    check(lib().h3_rope_axes(C.byref(pos), S, ptr(out), stream_handle), "h3_rope_axes")
-
-
-def qknorm_rope_axes(q, k, qw, kw, pos: H3Positions, eps, out_q, out_k, stream_handle: int) -> None:
-    """q, out_q [S, Hq, 128], k, out_k [S, Hk, 128]."""
-
-    _count(1)
-    check(lib().h3_qknorm_rope_axes(ptr(q), q.stride(0), q.stride(1), ptr(k), k.stride(0), k.stride(1), q.shape[0],
-                                    q.shape[1], k.shape[1], ptr(qw), ptr(kw), C.byref(pos), eps, ptr(out_q),
-                                    out_q.stride(0), out_q.stride(1), ptr(out_k), out_k.stride(0), out_k.stride(1),
-                                    stream_handle), "h3_qknorm_rope_axes")
-
-
 def attn_fp8(q, k, v, ld, hstride, S, H, out, ldo, workspace) -> None:
     _count(4)
     check(lib().h3_attn_fp8(ptr(q), ptr(k), ptr(v), ld, hstride, S, H, ptr(out), ldo, ptr(workspace),
@@ -310,12 +288,6 @@ def attn_fp8_peers(q, k, v, ld, hstride, S, H, peers: list[int], rank: int, ldo,
     check(lib().h3_attn_fp8_peers(ptr(q), ptr(k), ptr(v), ld, hstride, S, H, ptr(kv_ptr), ptr(kv_idx), arr,
                                   len(peers), rank, ldo, ptr(workspace), workspace.numel() * workspace.element_size(),
                                   stream()), "h3_attn_fp8_peers")
-
-
-def attn_bf16(q, ldq, hsq, k, ldk, hsk, v, ldv, hsv, S, Hq, Hk, lo, hi, out, ldo, stream_handle: int) -> None:
-    _count(1)
-    check(lib().h3_attn_bf16(ptr(q), ldq, hsq, ptr(k), ldk, hsk, ptr(v), ldv, hsv, S, Hq, Hk, ptr(lo), ptr(hi),
-                             ptr(out), ldo, stream_handle), "h3_attn_bf16")
 
 
 # ---- device buffers shared between the processes of one node (CUDA IPC), for the fused Ulysses exchanges
