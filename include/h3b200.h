@@ -240,11 +240,14 @@ int h3_attn_fp8_peers(const void* q, const void* k, const void* v, long long ld,
  * outside a token's span never reach its row, whatever they hold (NaN and infinities included).  Hq query heads share
  * Hk key heads in groups of Hq / Hk.  q, k and v are bf16 views with their own token and head strides (multiples of 8
  * elements, 16-byte aligned), element (t, h, d) at t * ld + h * hs + d; out (t, h, d) at out + t * ldo + h * 128 + d.
- * scores scaled by 1 / sqrt(128).  No workspace.  S <= 262,144.  The reference's backends (tfvideo/attention.py:29-54)
- * attend to the whole sequence. */
+ * scores scaled by 1 / sqrt(128).  S <= 262,144.  workspace: h3_attn_bf16_workspace_bytes(S, Hk) bytes, 16-byte aligned
+ * (0, and NULL, for short sequences), one per call in flight: the key norms that let long rows of bounded scores skip
+ * their running maximum; NULL is always accepted and only slower.  The reference's backends
+ * (tfvideo/attention.py:29-54) attend to the whole sequence. */
+size_t h3_attn_bf16_workspace_bytes(int S, int Hk);
 int h3_attn_bf16(const void* q, long long ldq, long long hsq, const void* k, long long ldk, long long hsk,
                  const void* v, long long ldv, long long hsv, int S, int Hq, int Hk, const int* span_lo,
-                 const int* span_hi, void* out, long long ldo, void* stream);
+                 const int* span_hi, void* out, long long ldo, void* workspace, size_t workspace_bytes, void* stream);
 
 /* The same attention as h3_attn_fp8 for callers that cannot allocate device memory -- for example code running
  * inside a host framework that owns every device allocation (ComfyUI records and replays a block's allocations under

@@ -22,6 +22,7 @@
 #pragma once
 
 #include <climits>
+#include <type_traits>
 
 #include "attention.cuh"
 #include "common.cuh"
@@ -97,6 +98,7 @@ struct AttnBf16Args {
   long long ldv, hsv;
   const int* lo;             // spans, or NULL: every key
   const int* hi;
+  const float* knorm;        // [key heads][S / 128 tiles]: largest |k|^2 of each 128 keys, or NULL
   int S, group;              // group: query heads that share a key head
 };
 
@@ -120,8 +122,14 @@ constexpr int kAttnBf16Threads = 352;
 // Lag of the running maximum (log2 units) before O and l are rescaled: P <= 2^8 is far inside bf16's range, and its
 // relative rounding does not depend on the factor.
 constexpr float kTauBf16 = 8.0f;
+// Scores are bounded by |q| |k|; while twice that bound is below this (log2 units), a row keeps the maximum of its
+// first step for good: P and l then stay below 2^98, and no later step looks for a maximum.
+constexpr float kBoundBf16 = 80.0f;
 // pairs of each 32-key chunk whose exp2 runs on the FMA pipe (bit i: keys 2i, 2i + 1)
-constexpr uint32_t kPolyPairsBf16 = 0x2492u;
+#ifndef H3_POLY_BF16
+#define H3_POLY_BF16 0x5292u
+#endif
+constexpr uint32_t kPolyPairsBf16 = H3_POLY_BF16;
 
 __device__ __forceinline__ float max_nan(float a, float b) {   // NaN when either is
   float m;
@@ -130,27 +138,76 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // NaN when eithe
 }
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1u); }
 
-// 32 scores of one row -> 16 words of bf16 P = exp2(s * scale + nbias) (key 2w in the low half of word w); l2 += the
-// unrounded P.  MASKED: every exponential on the MUFU, whose exp2(-inf) is exactly 0 (the polynomial's is 2^-126).
-template <bool MASKED>
-__device__ __forceinline__ void p_chunk_bf16(const uint32_t (&s)[32], uint64_t scale2, uint64_t nbias2,
-                                             uint32_t (&pw)[16], uint64_t& l2a, uint64_t& l2b) {
+// 2^(s * scale - m) for a pair, m an integer: n = round(s * scale - m) from the low bits of the sum with 1.5 * 2^23,
+// then the degree-3 polynomial of exp2_poly_clamped at the remainder, its exponent raised by n.  For results that are
+// normal numbers.
+__device__ __forceinline__ uint64_t exp2_poly_int(uint64_t s, uint64_t scale2, uint64_t nm_magic2) {
+  const uint64_t t = fma2(s, scale2, nm_magic2);                            // 1.5 * 2^23 + n
+  const uint64_t g = fma2(s, scale2, fma2(t, f32x2_splat(-1.0f), nm_magic2));   // s * scale - m - n
+  uint64_t p = fma2(f32x2_splat(0.0551716685295105f), g, f32x2_splat(0.2426111400127411f));
+  p = fma2(p, g, f32x2_splat(0.6932609677314758f));
+  p = fma2(p, g, f32x2_splat(0.9999280571937561f));
+  float t0, t1, p0, p1;
+  f32x2_unpack(t, t0, t1);
+  f32x2_unpack(p, p0, p1);
+  return f32x2_pack(__uint_as_float((__float_as_uint(t0) << 23) + __float_as_uint(p0)),
+                    __uint_as_float((__float_as_uint(t1) << 23) + __float_as_uint(p1)));
+}
+
+// 32 scores of one row -> 16 words of bf16 P = exp2(s * scale - m) (key 2w in the low half of word w); l2 += the
+// unrounded P.  POLY (bounded scores, none masked): part of the exponentials as a polynomial; otherwise all on the
+// MUFU, whose exp2(-inf) is exactly 0 and exp2(NaN) NaN.
+template <bool POLY>
+__device__ __forceinline__ void p_chunk_bf16(const uint32_t (&s)[32], uint64_t scale2, float nm, uint32_t (&pw)[16],
+                                             uint64_t& l2a, uint64_t& l2b) {
+  const uint64_t nm2 = f32x2_splat(nm), nm_magic2 = f32x2_splat(nm + 12582912.0f);
 #pragma unroll
   for (int w = 0; w < 16; ++w) {
-    const uint64_t x = fma2(f32x2_pack(__uint_as_float(s[2 * w]), __uint_as_float(s[2 * w + 1])), scale2, nbias2);
-    uint64_t y;
-    if (!MASKED && ((kPolyPairsBf16 >> w) & 1u)) {
-      float a, b;
-      f32x2_unpack(x, a, b);   // a NaN score stays NaN through the polynomial's clamp
-      y = exp2_poly_clamped(f32x2_pack(max_nan(a, -126.0f), max_nan(b, -126.0f)));
-    } else {
-      y = exp2_mufu_pair(x);
-    }
+    const uint64_t x = f32x2_pack(__uint_as_float(s[2 * w]), __uint_as_float(s[2 * w + 1]));
+    const uint64_t y = POLY && ((kPolyPairsBf16 >> w) & 1u) ? exp2_poly_int(x, scale2, nm_magic2)
+                                                            : exp2_mufu_pair(fma2(x, scale2, nm2));
     if (w & 1) l2b = add2(l2b, y);
     else l2a = add2(l2a, y);
     float a, b;
     f32x2_unpack(y, a, b);
     pw[w] = pack_bf16(a, b);
+  }
+}
+
+// Largest |k|^2 of each 128 keys and head (NaN when one is).  Bound by reading K once: 16 lanes a row.
+struct KnormArgs {
+  const __nv_bfloat16* k;
+  long long ld, hs;
+  int S;
+  float* out;
+};
+__global__ void __launch_bounds__(256) attn_bf16_knorm_kernel(const KnormArgs a) {
+  __shared__ float red[16];
+  const int part = threadIdx.x & 15, row0 = threadIdx.x >> 4;
+  uint4 u[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int t = blockIdx.x * 128 + row0 + 16 * i;
+    u[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (t < a.S) u[i] = *reinterpret_cast<const uint4*>(a.k + (long long)t * a.ld + blockIdx.y * a.hs + part * 8);
+  }
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ss += bf16_lo(w[e]) * bf16_lo(w[e]) + bf16_hi(w[e]) * bf16_hi(w[e]);
+#pragma unroll
+    for (int o = 8; o; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
+    m = max_nan(m, ss);
+  }
+  if (part == 0) red[row0] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = max_nan(m, red[i]);
+    a.out[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = m;
   }
 }
 
@@ -350,21 +407,25 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
       if (!__all_sync(~0u, mbar_wait(&v_full[vs], (j / L::VST) & 1, 320))) break;
       if ((j >= j0[0] && j < j1[0] && hides(0, j)) || (j >= j0[1] && j < j1[1] && hides(1, j))) {
         uint4* vt = reinterpret_cast<uint4*>(smem + L::V_OFF + vs * L::TILE);
-        bool hit = false;
-#pragma unroll 4
+        uint32_t seen = 0;   // adding one to an exponent of all ones carries into the sign's place
+#pragma unroll 16
         for (int i = lane; i < L::TILE / 16; i += 32) {
-          uint4 u = vt[i];
-          uint32_t* w = &u.x;
-          bool mine = false;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {   // exponent bits all set: infinity or NaN
-            if ((w[e] & 0x7F80u) == 0x7F80u) { w[e] &= 0xFFFF0000u; mine = true; }
-            if ((w[e] & 0x7F800000u) == 0x7F800000u) { w[e] &= 0x0000FFFFu; mine = true; }
-          }
-          if (mine) vt[i] = u;
-          hit |= mine;
+          const uint4 u = vt[i];
+          seen |= ((u.x & 0x7F807F80u) + 0x00800080u) | ((u.y & 0x7F807F80u) + 0x00800080u) |
+                  ((u.z & 0x7F807F80u) + 0x00800080u) | ((u.w & 0x7F807F80u) + 0x00800080u);
         }
-        if (__any_sync(~0u, hit)) {
+        const bool hit = __any_sync(~0u, (seen & 0x80008000u) != 0);
+        if (hit) {
+          for (int i = lane; i < L::TILE / 16; i += 32) {
+            uint4 u = vt[i];
+            uint32_t* w = &u.x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if ((w[e] & 0x7F80u) == 0x7F80u) w[e] &= 0xFFFF0000u;
+              if ((w[e] & 0x7F800000u) == 0x7F800000u) w[e] &= 0x0000FFFFu;
+            }
+            vt[i] = u;
+          }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMA reads these writes
           if (lane == 0) {
             bad[j >> 5] |= 1u << (j & 31);
@@ -385,10 +446,29 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
     const float scale = kLog2e * 0.08838834764831845f;   // log2(e) / sqrt(128)
     const uint64_t scale2 = f32x2_splat(scale);
     const bool live = lo < hi;
-    float m_used = -INFINITY;
+    float m_used = -INFINITY;   // an integer once a key was seen
     uint64_t l2a = 0, l2b = 0;
-    bool ok = true;
-    for (int j = first; j < last; ++j) {
+    bool ok = true, bounded = false;
+    if (p.knorm && last > first) {
+      const int ntiles = (p.S + 127) >> 7;
+      const float* kn = p.knorm + (size_t)hk * ntiles;
+      float kk = 0.f;
+      for (int i = (base >> 7) + lane; i <= (kend - 1) >> 7; i += 32) kk = max_nan(kk, kn[i]);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) kk = max_nan(kk, __shfl_xor_sync(~0u, kk, o));
+      ok = __all_sync(~0u, mbar_wait(q_full, 0, 334));
+      float qq = 0.f;
+      const uint8_t* qr = smem + L::Q_OFF + t * L::TILE + (threadIdx.x & 127) * 128;
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {   // (any order of the row's pieces will do)
+        const uint4 u = *reinterpret_cast<const uint4*>(qr + (c >> 3) * L::SUB + (((c ^ lane) & 7) << 4));
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) qq += bf16_lo(w[e]) * bf16_lo(w[e]) + bf16_hi(w[e]) * bf16_hi(w[e]);
+      }
+      bounded = __all_sync(~0u, !live || 2.0f * scale * sqrtf(qq) * sqrtf(kk) < kBoundBf16);
+    }
+    for (int j = first; ok && j < last; ++j) {
       const int i = j - first, kb = base + 128 * j;
       ok = __all_sync(~0u, mbar_wait(&s_full[t], i & 1, 330 + t));
       if (!ok) break;
@@ -407,44 +487,50 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
             if (!((vis >> e) & 1u)) s[c][e] = __float_as_uint(-INFINITY);
         }
       }
-      const float mx = fmaxf(max_chunk(s[1], max_chunk(s[0], -INFINITY)), max_chunk(s[3], max_chunk(s[2], -INFINITY)));
-      const float mnew = mx * scale;
-      const bool need = mnew > m_used + kTauBf16 || (m_used == -INFINITY && mnew > m_used);
-      float alpha = 1.0f;
-      if (need) {
-        alpha = m_used == -INFINITY ? 0.0f : ex2(m_used - mnew);
-        m_used = mnew;
-        const uint64_t a2 = f32x2_splat(alpha);
-        l2a = mul2(l2a, a2);
-        l2b = mul2(l2b, a2);
-      }
-      // O holds the PV of every earlier step here: those MMAs were issued before S of this step by the same thread,
-      // and s_full counts everything issued before its commit
-      if (i > 0 && __any_sync(~0u, need)) {
+      if (!bounded || __any_sync(~0u, m_used == -INFINITY)) {
+        const float mx = fmaxf(fmaxf(max_chunk(s[0], -INFINITY), max_chunk(s[1], -INFINITY)),
+                               fmaxf(max_chunk(s[2], -INFINITY), max_chunk(s[3], -INFINITY)));
+        const float mnew = ceilf(mx * scale);
+        const bool need = m_used == -INFINITY ? mnew > m_used : mnew > m_used + kTauBf16 && !bounded;
+        float alpha = 1.0f;
+        if (need) {
+          alpha = m_used == -INFINITY ? 0.0f : ex2(m_used - mnew);
+          m_used = mnew;
+          const uint64_t a2 = f32x2_splat(alpha);
+          l2a = mul2(l2a, a2);
+          l2b = mul2(l2b, a2);
+        }
+        // O holds the PV of every earlier step here: those MMAs were issued before S of this step by the same thread,
+        // and s_full counts everything issued before its commit
+        if (i > 0 && __any_sync(~0u, need)) {
 #pragma unroll 1
-        for (int c = 0; c < 8; ++c) {
-          uint32_t o[16];
-          tmem_ld16(o_col + 16 * c, o);
-          tmem_ld_wait();
+          for (int c = 0; c < 8; ++c) {
+            uint32_t o[16];
+            tmem_ld16(o_col + 16 * c, o);
+            tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-          tmem_st16(o_col + 16 * c, o);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st16(o_col + 16 * c, o);
+          }
         }
       }
-      const uint64_t nbias2 = f32x2_splat(m_used == -INFINITY ? 0.0f : -m_used);   // no key yet: P = exp2(-inf) = 0
+      const float nm = m_used == -INFINITY ? 0.0f : -m_used;   // no key yet: P = exp2(-inf) = 0
+      auto emit = [&](auto poly) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t pw[16];
-        if (masked) p_chunk_bf16<true>(s[c], scale2, nbias2, pw, l2a, l2b);
-        else p_chunk_bf16<false>(s[c], scale2, nbias2, pw, l2a, l2b);
-        tmem_st16(s_col + 16 * c, pw);
-        if (c & 1) {
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[2 * t + (c >> 1)]);
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pw[16];
+          p_chunk_bf16<decltype(poly)::value>(s[c], scale2, nm, pw, l2a, l2b);
+          tmem_st16(s_col + 16 * c, pw);
+          if (c & 1) {
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[2 * t + (c >> 1)]);
+          }
         }
-      }
+      };
+      if (bounded && !masked) emit(std::true_type{});
+      else emit(std::false_type{});
     }
     // ---- epilogue: O / l -> bf16, this thread's row
     const bool any = last > first;

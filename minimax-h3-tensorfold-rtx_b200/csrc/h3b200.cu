@@ -751,9 +751,14 @@ int h3_attn_fp8_sparse(const void* q, const void* k, const void* v, long long ld
                   workspace_bytes, stream);
 }
 
+size_t h3_attn_bf16_workspace_bytes(int S, int Hk) {
+  if (S < 2048 || Hk <= 0) return 0;
+  return (size_t)Hk * ((S + 127) / 128) * 4;
+}
+
 int h3_attn_bf16(const void* q, long long ldq, long long hsq, const void* k, long long ldk, long long hsk,
                  const void* v, long long ldv, long long hsv, int S, int Hq, int Hk, const int* span_lo,
-                 const int* span_hi, void* out, long long ldo, void* stream) {
+                 const int* span_hi, void* out, long long ldo, void* workspace, size_t workspace_bytes, void* stream) {
   const char* who = "h3_attn_bf16";
   using L = AttnBf16Smem;
   if (!q || !k || !v || !out) return fail(H3_ERR_ARG, "%s: NULL pointer", who);
@@ -770,6 +775,9 @@ int h3_attn_bf16(const void* q, long long ldq, long long hsq, const void* k, lon
   if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) || !aligned(span_lo, 4) ||
       !aligned(span_hi, 4))
     return fail(H3_ERR_ARG, "%s: q / k / v / out 16-byte and spans 4-byte alignment required", who);
+  if (workspace && (!aligned(workspace, 16) || workspace_bytes < h3_attn_bf16_workspace_bytes(S, Hk)))
+    return fail(H3_ERR_ARG, "%s: workspace misaligned, or %zu bytes < %zu", who, workspace_bytes,
+                h3_attn_bf16_workspace_bytes(S, Hk));
   CUtensorMap tq, tk, tv;
   int rc;
   if ((rc = make_map_bf16(&tq, q, 128, S, Hq, ldq, hsq, 128, who))) return rc;
@@ -777,7 +785,12 @@ int h3_attn_bf16(const void* q, long long ldq, long long hsq, const void* k, lon
   if ((rc = make_map_bf16(&tv, v, 128, S, Hk, ldv, hsv, 128, who))) return rc;
   if ((rc = smem_optin(attn_bf16_kernel, L::TOTAL, &g_optin_attn_bf16, who))) return rc;
   AttnBf16Args a{reinterpret_cast<__nv_bfloat16*>(out), ldo, reinterpret_cast<const __nv_bfloat16*>(v), ldv, hsv,
-                 span_lo, span_hi, S, Hq / Hk};
+                 span_lo, span_hi, reinterpret_cast<const float*>(workspace), S, Hq / Hk};
+  if (workspace) {
+    KnormArgs kn{reinterpret_cast<const __nv_bfloat16*>(k), ldk, hsk, S, reinterpret_cast<float*>(workspace)};
+    attn_bf16_knorm_kernel<<<dim3((S + 127) / 128, Hk), 256, 0, S_(stream)>>>(kn);
+    if ((rc = check_launch(who))) return rc;
+  }
   attn_bf16_kernel<<<dim3((S + 255) / 256, Hq), kAttnBf16Threads, L::TOTAL, S_(stream)>>>(tq, tk, tv, a);
   return check_launch(who);
 }

@@ -202,8 +202,10 @@ def _bf16_launch(S: int, Hq: int, Hk: int, rows, out: torch.Tensor, mask: SpanMa
         lo, hi = mask.lo.data_ptr(), mask.hi.data_ptr()
         dev = N.one_device("bf16 attention", q, k, v, out, mask.lo, mask.hi)
     if S and Hq:
-        N.launch(dev, "h3_attn_bf16", 1, q.data_ptr(), ldq, hsq, k.data_ptr(), ldk, hsk, v.data_ptr(), ldv, hsv, S, Hq,
-                 Hk, lo, hi, out.data_ptr(), out.stride(0))
+        size = N.attn_bf16_workspace_bytes(S, Hk)
+        ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+        N.launch(dev, "h3_attn_bf16", 2 if size else 1, q.data_ptr(), ldq, hsq, k.data_ptr(), ldk, hsk, v.data_ptr(), ldv,
+                 hsv, S, Hq, Hk, lo, hi, out.data_ptr(), out.stride(0), ws.data_ptr() if size else None, size)
 
 
 def bf16(q, k, v, mask: SpanMask | None = None):

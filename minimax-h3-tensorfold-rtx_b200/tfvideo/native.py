@@ -65,7 +65,8 @@ _SIGS = {
     "h3_attn_fp8_noalloc": [vp, vp, vp, i64, i64, i32, i32, vp, i64, vp],
     "h3_attn_fp8_sparse": [vp, vp, vp, i64, i64, i32, i32, vp, vp, vp, i64, vp, sz, vp],
     "h3_attn_fp8_peers": [vp, vp, vp, i64, i64, i32, i32, vp, vp, C.POINTER(vp), i32, i32, i64, vp, sz, vp],
-    "h3_attn_bf16": [vp, i64, i64, vp, i64, i64, vp, i64, i64, i32, i32, i32, vp, vp, vp, i64, vp],
+    "h3_attn_bf16_workspace_bytes": ([i32, i32], sz),
+    "h3_attn_bf16": [vp, i64, i64, vp, i64, i64, vp, i64, i64, i32, i32, i32, vp, vp, vp, i64, vp, sz, vp],
     "h3_peer_alloc": [sz, C.POINTER(vp), vp],
     "h3_peer_open": [vp, C.POINTER(vp)],
     "h3_peer_close": [vp],
@@ -182,6 +183,10 @@ def sf_tiled_bytes(rows: int, cols: int) -> int:
 
 def attn_workspace_bytes(S: int, H: int) -> int:
     return int(lib().h3_attn_workspace_bytes(S, H))
+
+
+def attn_bf16_workspace_bytes(S: int, Hk: int) -> int:
+    return int(lib().h3_attn_bf16_workspace_bytes(S, Hk))
 
 
 def adapter_workspace_bytes(M: int, R: int) -> int:

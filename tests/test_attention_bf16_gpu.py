@@ -71,7 +71,7 @@ def packed(S, Hq, Hk, seed, scale=1.0):
 
 
 @pytest.mark.parametrize("S,Hq,Hk", [(1, 1, 1), (2, 3, 3), (63, 2, 1), (64, 1, 1), (127, 4, 2), (128, 2, 2), (129, 2, 2),
-                                     (255, 1, 1), (256, 4, 4), (257, 6, 2), (300, 5, 5), (1000, 8, 1), (2500, 2, 2)])
+                                     (255, 1, 1), (256, 4, 4), (257, 6, 2), (300, 5, 5), (1000, 8, 1), (2500, 2, 2), (4097, 3, 1)])
 def test_every_key(S, Hq, Hk):
     from tfvideo import attention as A
 
@@ -238,6 +238,27 @@ def test_rising_scores_rescale_every_step():
     check(A.bf16(q, k, v), q, k, v)
     m = A.SpanMask.frames([S], 100, 50)
     check(A.bf16(q, k, v, m), q, k, v, m.lo, m.hi)
+
+
+@pytest.mark.parametrize("grow", [1.0, 2.5, 6.0])
+def test_long_rows_with_and_without_bounded_scores(grow):
+    """At 2,048 tokens and more a row of bounded scores keeps its first step's maximum; keys that grow along the
+    sequence raise the scores far above it, up to and past the bound (which sends the row to the running maximum)."""
+
+    from tfvideo import attention as A
+
+    S = 2304
+    q, k, v = (t.clone() for t in packed(S, 2, 2, 24))
+    k = (k.float() * torch.linspace(0.2, grow, S, device="cuda")[None, None, :, None]).to(torch.bfloat16)
+    check(A.bf16(q, k, v), q, k, v)
+    for m in (A.SpanMask.documents([900, 1, 1300], S), A.SpanMask.frames([S], 200, 77)):
+        check(A.bf16(q, k, v, m), q, k, v, m.lo, m.hi)
+    k[:, 0, 2000] = float("nan")
+    m = A.SpanMask.documents([1900, 404])
+    o = A.bf16(q, k, v, m)
+    check(o[:, :, :1900], q[:, :, :1900], k[:, :, :1900], v[:, :, :1900])
+    assert torch.isnan(o[:, 0, 1900:]).all() and torch.isfinite(o[:, 1]).all()
+    device_ok()
 
 
 def test_values_at_the_type_limits():

@@ -95,8 +95,8 @@ def test_rope_functions_refuse_bad_arguments():
 def test_attn_bf16_checks_its_arguments(lib):
     from tfvideo import native as N
 
-    def call(q=FAKE, ldq=384, hsq=128, ldk=384, S=10, Hq=2, Hk=1, lo=None, hi=None, out=FAKE, ldo=256):
-        return lib.h3_attn_bf16(q, ldq, hsq, FAKE, ldk, 128, FAKE, 384, 128, S, Hq, Hk, lo, hi, out, ldo, None)
+    def call(q=FAKE, ldq=384, hsq=128, ldk=384, S=10, Hq=2, Hk=1, lo=None, hi=None, out=FAKE, ldo=256, ws=None, size=0):
+        return lib.h3_attn_bf16(q, ldq, hsq, FAKE, ldk, 128, FAKE, 384, 128, S, Hq, Hk, lo, hi, out, ldo, ws, size, None)
 
     assert call(q=None) == -1 and call(out=None) == -1
     assert call(lo=FAKE) == -1 and "half" in N.last_error()
@@ -106,6 +106,10 @@ def test_attn_bf16_checks_its_arguments(lib):
     assert call(ldo=128) == -2 and call(ldo=260) == -2
     assert call(ldq=0) == -2 and call(ldq=388) == -2 and call(hsq=-128) == -2 and call(ldk=-8) == -2
     assert call(q=FAKE + 8) == -1 and "16-byte" in N.last_error()
+    need = lib.h3_attn_bf16_workspace_bytes(5000, 3)
+    assert need == 3 * 40 * 4 and lib.h3_attn_bf16_workspace_bytes(100, 3) == 0
+    assert call(S=5000, Hq=3, Hk=3, ldo=384, ws=FAKE, size=need - 1) == -1 and "workspace" in N.last_error()
+    assert call(S=5000, Hq=3, Hk=3, ldo=384, ws=FAKE + 4, size=need) == -1
 
 
 def test_span_masks():
