@@ -10,8 +10,9 @@
 //
 // One CTA = two 128-row query tiles (A, B) of one head over the same 128-key steps.  TMEM: S_A, S_B, O_A, O_B of 128
 // columns each, P written over S.  Warps 0-3: softmax of A, 4-7: of B, a thread per query row with its 128 scores in
-// registers; warp 8: TMA; warp 9: all MMAs, alternating A and B, so that one tile's MMAs run under the other's
-// softmax; warp 10: guards masked V rows (below).  A step of both tiles is 4 x 512 cycles of MMA at the bf16 rate and
+// registers; warp 8: TMA; warps 9 and 10: the MMAs of A and of B; warp 11: guards masked V rows (below).  One tile's
+// MMAs run under the other's softmax.  (One warp issuing both tiles' MMAs was the bottleneck itself: a wait and a
+// commit cost it about 200 cycles each, and P lay ready for 700 of a step's 3,260 cycles.)  A step of both tiles is 4 x 512 cycles of MMA at the bf16 rate and
 // 2 x 1,024 cycles of exponentials at 16 a cycle, of which 5 pairs in 16 go to the FMA pipe (exp2_poly_clamped).
 //
 // Masked keys.  Steps run over the union of the CTA's spans and start at its first key, so documents begin on a step.
@@ -118,7 +119,7 @@ struct AttnBf16Smem {
 };
 static_assert(AttnBf16Smem::TOTAL <= 232448, "shared memory of one SM");
 
-constexpr int kAttnBf16Threads = 352;
+constexpr int kAttnBf16Threads = 384;
 // Lag of the running maximum (log2 units) before O and l are rescaled: P <= 2^8 is far inside bf16's range, and its
 // relative rounding does not depend on the factor.
 constexpr float kTauBf16 = 8.0f;
@@ -126,10 +127,7 @@ constexpr float kTauBf16 = 8.0f;
 // first step for good: P and l then stay below 2^98, and no later step looks for a maximum.
 constexpr float kBoundBf16 = 80.0f;
 // pairs of each 32-key chunk whose exp2 runs on the FMA pipe (bit i: keys 2i, 2i + 1)
-#ifndef H3_POLY_BF16
-#define H3_POLY_BF16 0x5292u
-#endif
-constexpr uint32_t kPolyPairsBf16 = H3_POLY_BF16;
+constexpr uint32_t kPolyPairsBf16 = 0x2492u;
 
 __device__ __forceinline__ float max_nan(float a, float b) {   // NaN when either is
   float m;
@@ -227,7 +225,8 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
   uint64_t* s_full = v_empty + L::VST;     // [tile]
   uint64_t* p_full = s_full + 2;           // [tile][half]: P of keys 0-63 / 64-127 written, by four warps
   uint64_t* o_done = p_full + 4;           // [tile]
-  uint64_t* drained = o_done + 2;
+  uint64_t* turn = o_done + 2;             // [tile]: the other tile's MMAs of this round are issued
+  uint64_t* drained = turn + 2;
   uint32_t* bad = reinterpret_cast<uint32_t*>(smem + L::BAD_OFF);
   int* red = reinterpret_cast<int*>(smem + L::RED_OFF);      // [warp][lo min, lo max, hi min, hi max]
   int* any_bad = red + 32;
@@ -262,20 +261,21 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
     mbar_init(q_full, 1);
     for (int s = 0; s < L::KST; ++s) {
       mbar_init(&k_full[s], 1);
-      mbar_init(&k_empty[s], 1);
+      mbar_init(&k_empty[s], 2);   // a commit of each MMA warp
     }
     for (int s = 0; s < L::VST; ++s) {
       mbar_init(&v_full[s], 1);
       mbar_init(&v_ok[s], 1);
-      mbar_init(&v_empty[s], 1);
+      mbar_init(&v_empty[s], 2);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
       mbar_init(&p_full[2 * t], 4);
       mbar_init(&p_full[2 * t + 1], 4);
       mbar_init(&o_done[t], 1);
+      mbar_init(&turn[t], 1);
     }
-    mbar_init(drained, 1);
+    mbar_init(drained, 2);
     fence_barrier_init();
   }
   if (warp == 9) {
@@ -347,52 +347,55 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
     if (steps > 0) mbar_drain(q_full, 0, 303);
     for (int j = max(nk - L::KST, 0); j < nk; ++j) mbar_drain(&k_full[j % L::KST], (j / L::KST) & 1, 303);
     for (int j = max(nv - L::VST, 0); j < nv; ++j) mbar_drain(&v_full[j % L::VST], (j / L::VST) & 1, 303);
-  } else if (warp == 9) {
-    // ------------------------------------------------------------------ MMA
+  } else if (warp == 9 || warp == 10) {
+    // ------------------------------------------------------------------ MMA of one tile
     constexpr uint32_t idesc_s = idesc_bf16(128, 128, false), idesc_o = idesc_bf16(128, 128, true);
-    auto issue_s = [&](int t, int j) {   // S_t = Q_t K_j^T: 8 MMAs over 16 dims each
-      const uint32_t qa = smem_u32(smem + L::Q_OFF + t * L::TILE);
+    const int t = warp - 9;
+    const int first = t ? j0[1] : j0[0], last = t ? j1[1] : j1[0];
+    const uint32_t qa = smem_u32(smem + L::Q_OFF + t * L::TILE), s_tm = tmem + t * 128, o_tm = tmem + 256 + t * 128;
+    auto issue_s = [&](int j) {   // S = Q K_j^T: 8 MMAs over 16 dims each
       const uint32_t ka = smem_u32(smem + L::K_OFF + (j % L::KST) * L::TILE);
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk) {
         const uint32_t off = (kk >> 2) * L::SUB + (kk & 3) * 32;
-        mma_bf16_ss(tmem + t * 128, sdesc_kmajor_sw128(qa + off), sdesc_kmajor_sw128(ka + off), idesc_s, kk != 0);
+        mma_bf16_ss(s_tm, sdesc_kmajor_sw128(qa + off), sdesc_kmajor_sw128(ka + off), idesc_s, kk != 0);
       }
     };
-    auto issue_pv = [&](int t, int j, int half) {   // O_t (+)= P_t V_j over 64 keys: 4 MMAs over 16 keys each
+    auto issue_pv = [&](int j, int half) {   // O (+)= P V_j over 64 keys: 4 MMAs over 16 keys each
       // V rows are keys (the K dimension), 64 dims contiguous: MN-major, 8-key groups 1,024 bytes apart, the two
       // 64-dim halves SUB apart
       const uint32_t va = smem_u32(smem + L::V_OFF + (j % L::VST) * L::TILE);
 #pragma unroll
       for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
-        mma_bf16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, make_sdesc(va + kk * 2048, L::SUB, 1024, kLayoutSW128),
-                    idesc_o, j != j0[t] || kk != 0);
+        mma_bf16_ts(o_tm, s_tm + kk * 8, make_sdesc(va + kk * 2048, L::SUB, 1024, kLayoutSW128), idesc_o,
+                    j != first || kk != 0);
     };
     bool ok = steps > 0 && __all_sync(~0u, mbar_wait(q_full, 0, 310));
     for (int j = -1; ok && j < steps; ++j) {
-      if (j >= 0 && !(ok = __all_sync(~0u, mbar_wait(&v_ok[j % L::VST], (j / L::VST) & 1, 311)))) break;
       const int n = j + 1;
+      // (also for steps this tile has no part in: a ring slot is free once both warps have let go of it)
+      if (j >= 0 && !(ok = __all_sync(~0u, mbar_wait(&v_ok[j % L::VST], (j / L::VST) & 1, 311)))) break;
       if (n < steps && !(ok = __all_sync(~0u, mbar_wait(&k_full[n % L::KST], (n / L::KST) & 1, 312)))) break;
+      const bool pv = j >= first && j < last, qk = n >= first && n < last;
+      // The warps take turns, A first.  Left to themselves the two tiles' MMAs interleave and finish together, and both
+      // softmaxes then wait for both: 4,160 cycles a step, against 2,920 in turns.  (Passing the turn on before the
+      // last MMAs of S are issued, or waiting for P before the turn, settles into unequal halves: 3,220 cycles.)
+      if (t + n > 0 && !(ok = __all_sync(~0u, mbar_wait(&turn[t], (n - 1 + t) & 1, 316 + t)))) break;
+      if (pv && !(ok = __all_sync(~0u, mbar_wait(&p_full[2 * t], (j - first) & 1, 313 + t)))) break;
       tc_fence_after();
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (ok && j >= j0[t] && j < j1[t]) {
-          const uint32_t ph = (j - j0[t]) & 1;
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            if (ok && (ok = __all_sync(~0u, mbar_wait(&p_full[2 * t + half], ph, 313 + t)))) {
-              tc_fence_after();
-              issue_pv(t, j, half);
-            }
-          }
-          if (ok && j + 1 == j1[t]) tc_commit(&o_done[t]);
-        }
-        if (ok && n >= j0[t] && n < j1[t]) {   // after PV_t(j) in issue order: P_t is read before S_t overwrites it
-          issue_s(t, n);
-          tc_commit(&s_full[t]);
-        }
+      if (pv) {
+        issue_pv(j, 0);
+        if (!(ok = __all_sync(~0u, mbar_wait(&p_full[2 * t + 1], (j - first) & 1, 313 + t)))) break;
+        tc_fence_after();
+        issue_pv(j, 1);
+        if (n == last) tc_commit(&o_done[t]);
       }
-      if (!ok) break;
+      if (qk) {   // after PV(j) in issue order: P is read before S overwrites it
+        issue_s(n);
+        tc_commit(&s_full[t]);
+      }
+      if (lane == 0) mbar_arrive(&turn[t ^ 1]);
+      __syncwarp();
       if (j >= 0) tc_commit(&v_empty[j % L::VST]);
       if (n < steps) tc_commit(&k_empty[n % L::KST]);
     }
@@ -400,7 +403,7 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
       tc_commit(drained);
       mbar_drain(drained, 0, 315);
     }
-  } else if (warp == 10) {
+  } else if (warp == 11) {
     // ------------------------------------------------------------------ V guard
     for (int j = 0; j < steps; ++j) {
       const int vs = j % L::VST;
