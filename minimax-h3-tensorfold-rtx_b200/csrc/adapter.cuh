@@ -27,19 +27,6 @@ struct AdapterArgs {
   int inplace;          // expand: out is y
 };
 
-// warp-wide store of one box of a 3-D tensor map from shared memory (the part outside the tensor is not written)
-__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* smem_src, int x, int y, int z) {
-  asm volatile(
-      "{\n\t.reg .pred e;\n\t.reg .b32 rx;\n\t" H3_ELECT
-      "@e cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];\n\t}" ::"l"(map), "r"(x),
-      "r"(y), "r"(z), "r"(smem_u32(smem_src))
-      : "memory");
-}
-// the elected lane's stores have read their shared memory
-__device__ __forceinline__ void tma_store_wait_read() {
-  asm volatile("{\n\t.reg .pred e;\n\t.reg .b32 rx;\n\t" H3_ELECT
-               "@e cp.async.bulk.commit_group;\n\t@e cp.async.bulk.wait_group.read 0;\n\t}" ::: "memory");
-}
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {   // addr: cluster_addr of another CTA's shared memory
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"

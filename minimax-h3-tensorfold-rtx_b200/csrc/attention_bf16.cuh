@@ -92,15 +92,30 @@ __host__ __device__ constexpr uint32_t idesc_bf16(int M, int N, bool b_mn_major)
          ((uint32_t)(M >> 4) << 24);
 }
 
+// warp-wide store of one box of a 3-D tensor map from shared memory (the part outside the tensor is not written)
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* smem_src, int x, int y, int z) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t.reg .b32 rx;\n\t" H3_ELECT
+      "@e cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];\n\t}" ::"l"(map), "r"(x),
+      "r"(y), "r"(z), "r"(smem_u32(smem_src))
+      : "memory");
+}
+// the elected lane's stores have read their shared memory
+__device__ __forceinline__ void tma_store_wait_read() {
+  asm volatile("{\n\t.reg .pred e;\n\t.reg .b32 rx;\n\t" H3_ELECT
+               "@e cp.async.bulk.commit_group;\n\t@e cp.async.bulk.wait_group.read 0;\n\t}" ::: "memory");
+}
+
 struct AttnBf16Args {
-  __nv_bfloat16* out;        // element (t, h, d) at out + t * ldo + h * 128 + d
-  long long ldo;
   const __nv_bfloat16* v;    // element (t, h, d) at v + t * ldv + h * hsv + d (the epilogue's repair of masked steps)
   long long ldv, hsv;
   const int* lo;             // spans, or NULL: every key
   const int* hi;
   const float* knorm;        // [key heads][S / 128 tiles]: largest |k|^2 of each 128 keys, or NULL
+  const int* order;          // [S / 256 tiles]: the query tiles by falling number of key steps, or NULL
   int S, group;              // group: query heads that share a key head
+  int tiles, heads;          // CTAs: query tiles x query heads
+  int tile_major;            // CTAs in order of tiles (every head of one, then the next), else of heads
 };
 
 struct AttnBf16Smem {
@@ -172,15 +187,20 @@ __device__ __forceinline__ void p_chunk_bf16(const uint32_t (&s)[32], uint64_t s
   }
 }
 
-// Largest |k|^2 of each 128 keys and head (NaN when one is).  Bound by reading K once: 16 lanes a row.
-struct KnormArgs {
+// Before the attention, for long sequences: the largest |k|^2 of each 128 keys and head (NaN when one is), and the span
+// range of each 128 query rows.  Bound by reading K once: 16 lanes a row.
+struct AttnBf16Prep {
   const __nv_bfloat16* k;
   long long ld, hs;
   int S;
-  float* out;
+  const int *lo, *hi;
+  float* knorm;
+  int2* range;         // [S / 128 tiles]: first and end key of the tile's rows
+  int* order;
 };
-__global__ void __launch_bounds__(256) attn_bf16_knorm_kernel(const KnormArgs a) {
+__global__ void __launch_bounds__(256) attn_bf16_prep_kernel(const AttnBf16Prep a) {
   __shared__ float red[16];
+  __shared__ int2 rr[4];
   const int part = threadIdx.x & 15, row0 = threadIdx.x >> 4;
   uint4 u[8];
 #pragma unroll
@@ -188,6 +208,15 @@ __global__ void __launch_bounds__(256) attn_bf16_knorm_kernel(const KnormArgs a)
     const int t = blockIdx.x * 128 + row0 + 16 * i;
     u[i] = make_uint4(0u, 0u, 0u, 0u);
     if (t < a.S) u[i] = *reinterpret_cast<const uint4*>(a.k + (long long)t * a.ld + blockIdx.y * a.hs + part * 8);
+  }
+  const bool spans = a.lo && blockIdx.y == 0;
+  if (spans && threadIdx.x < 128) {
+    const int t = blockIdx.x * 128 + threadIdx.x;
+    int lo = t < a.S ? max(a.lo[t], 0) : 0, hi = t < a.S ? min(a.hi[t], a.S) : 0;
+    const bool live = lo < hi;
+    lo = __reduce_min_sync(~0u, live ? lo : INT_MAX);
+    hi = __reduce_max_sync(~0u, live ? hi : 0);
+    if ((threadIdx.x & 31) == 0) rr[threadIdx.x >> 5] = make_int2(lo, hi);
   }
   float m = 0.f;
 #pragma unroll
@@ -205,13 +234,35 @@ __global__ void __launch_bounds__(256) attn_bf16_knorm_kernel(const KnormArgs a)
   if (threadIdx.x == 0) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) m = max_nan(m, red[i]);
-    a.out[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = m;
+    a.knorm[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = m;
+    if (spans)
+      a.range[blockIdx.x] = make_int2(min(min(rr[0].x, rr[1].x), min(rr[2].x, rr[3].x)),
+                                      max(max(rr[0].y, rr[1].y), max(rr[2].y, rr[3].y)));
   }
+}
+// The 256-row query tiles (at most 1,024) by falling number of key steps: the longest CTAs start first, so that the
+// last ones to start are short.  One block; each thread ranks its tile against all.
+__global__ void __launch_bounds__(1024) attn_bf16_order_kernel(const AttnBf16Prep a, int tiles) {
+  __shared__ int w[1024];
+  const int t = threadIdx.x, n128 = (a.S + 127) >> 7;
+  int mine = 0;
+  if (t < tiles) {
+    const int2 x = a.range[2 * t], y = 2 * t + 1 < n128 ? a.range[2 * t + 1] : make_int2(INT_MAX, 0);
+    const int lo = min(x.x, y.x), hi = max(x.y, y.y);
+    mine = hi > lo ? (hi - lo + 127) >> 7 : 0;
+  }
+  w[t] = mine;
+  __syncthreads();
+  if (t >= tiles) return;
+  int rank = 0;
+  for (int i = 0; i < tiles; ++i) rank += w[i] > mine || (w[i] == mine && i < t);
+  a.order[rank] = t;
 }
 
 __global__ void __launch_bounds__(kAttnBf16Threads, 1)
     attn_bf16_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                     const __grid_constant__ CUtensorMap tmV, const AttnBf16Args p) {
+                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
+                     const AttnBf16Args p) {
   using L = AttnBf16Smem;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -233,9 +284,29 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(red + 33);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = blockIdx.y, hk = h / p.group;
-  // the last tiles first: under causal spans they have the most keys
-  const int q0 = (gridDim.x - 1 - blockIdx.x) * 256;
+  // the order of CTAs: long ones first where they are known, else the last tiles, which see most under causal spans
+  const int h = p.tile_major ? blockIdx.x % p.heads : blockIdx.x / p.tiles, hk = h / p.group;
+  const int rank = p.tile_major ? blockIdx.x / p.heads : blockIdx.x % p.tiles;
+  const int q0 = (p.order ? p.order[rank] : p.tiles - 1 - rank) * 256;
+  auto load = [&](int off, const CUtensorMap* map, int row, int head, uint64_t* bar) {
+    tma_load_3d(smem + off, map, 0, row, head, bar);
+    tma_load_3d(smem + off + L::SUB, map, 64, row, head, bar);
+  };
+  if (warp == 8) {   // Q needs nothing else: it is on its way before the rest is set up
+    if (lane == 0) {
+      mbar_init(q_full, 1);
+      fence_barrier_init();
+    }
+    __syncwarp();
+    mbar_arrive_expect_tx(q_full, 2 * L::TILE);
+    load(L::Q_OFF, &tmQ, q0, h, q_full);
+    load(L::Q_OFF + L::TILE, &tmQ, q0 + 128, h, q_full);
+    if (lane == 0) {
+      prefetch_tmap(&tmK);
+      prefetch_tmap(&tmV);
+      prefetch_tmap(&tmO);
+    }
+  }
 
   // ---- this thread's span (softmax warps: a thread per query row) and the spans' ranges over each query tile
   int lo = 0, hi = 0;
@@ -258,7 +329,6 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
   for (int i = threadIdx.x; i < L::BAD_WORDS; i += kAttnBf16Threads) bad[i] = 0;
   if (threadIdx.x == 0) {
     *any_bad = 0;
-    mbar_init(q_full, 1);
     for (int s = 0; s < L::KST; ++s) {
       mbar_init(&k_full[s], 1);
       mbar_init(&k_empty[s], 2);   // a commit of each MMA warp
@@ -317,21 +387,7 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
 
   if (warp == 8) {
     // ------------------------------------------------------------------ TMA
-    if (lane == 0) {
-      prefetch_tmap(&tmQ);
-      prefetch_tmap(&tmK);
-      prefetch_tmap(&tmV);
-    }
-    auto load = [&](int off, const CUtensorMap* map, int row, int head, uint64_t* bar) {
-      tma_load_3d(smem + off, map, 0, row, head, bar);
-      tma_load_3d(smem + off + L::SUB, map, 64, row, head, bar);
-    };
     int nk = 0, nv = 0;   // loads issued
-    if (steps > 0) {
-      mbar_arrive_expect_tx(q_full, 2 * L::TILE);
-      load(L::Q_OFF, &tmQ, q0, h, q_full);
-      load(L::Q_OFF + L::TILE, &tmQ, q0 + 128, h, q_full);
-    }
     for (int j = 0; j < steps; ++j) {
       const int ks = j % L::KST, vs = j % L::VST;
       if (!__all_sync(~0u, mbar_wait(&k_empty[ks], ((j / L::KST) & 1) ^ 1, 301))) break;
@@ -344,7 +400,7 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
       ++nv;
     }
     // nothing may still be landing in this CTA's memory when it ends, after a wait that gave up included
-    if (steps > 0) mbar_drain(q_full, 0, 303);
+    mbar_drain(q_full, 0, 303);
     for (int j = max(nk - L::KST, 0); j < nk; ++j) mbar_drain(&k_full[j % L::KST], (j / L::KST) & 1, 303);
     for (int j = max(nv - L::VST, 0); j < nv; ++j) mbar_drain(&v_full[j % L::VST], (j / L::VST) & 1, 303);
   } else if (warp == 9 || warp == 10) {
@@ -541,14 +597,18 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
     if (any)
       ok = __all_sync(~0u, ok && mbar_wait(&o_done[t], 0, 332) &&
                                mbar_wait(&v_ok[(steps - 1) % L::VST], ((steps - 1) / L::VST) & 1, 333));
-    if (ok) {
+    const int query0 = q0 + warp * 32;
+    if (ok && query0 < p.S) {
       tc_fence_after();
       float la, lb, lc, ld;
       f32x2_unpack(l2a, la, lb);
       f32x2_unpack(l2b, lc, ld);
       const float inv_l = 1.0f / ((la + lb) + (lc + ld));
-      const int query = q0 + threadIdx.x;
       const bool repair = any && *(volatile int*)any_bad != 0;
+      // through the tile's Q rows (its MMAs are complete), swizzled, and out by TMA: 32 rows a warp, whole lines
+      // instead of one row a thread (3.7 us of a CTA)
+      if (!any) ok = __all_sync(~0u, mbar_wait(q_full, 0, 335));   // Q has landed: nothing overwrites these rows
+      uint8_t* rows = smem + L::Q_OFF + t * L::TILE + (warp & 3) * 32 * 128;
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t o[32];
@@ -574,13 +634,19 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
             }
           }
         }
-        if (query < p.S) {
-          uint4* d4 = reinterpret_cast<uint4*>(p.out + (long long)query * p.ldo + (long long)h * 128 + 32 * c);
+        uint8_t* row = rows + (c >> 1) * L::SUB + lane * 128;
 #pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4)
-            d4[q4] = make_uint4(pack_bf16(f[8 * q4], f[8 * q4 + 1]), pack_bf16(f[8 * q4 + 2], f[8 * q4 + 3]),
-                                pack_bf16(f[8 * q4 + 4], f[8 * q4 + 5]), pack_bf16(f[8 * q4 + 6], f[8 * q4 + 7]));
-        }
+        for (int q4 = 0; q4 < 4; ++q4)
+          *reinterpret_cast<uint4*>(row + ((((c & 1) * 4 + q4) ^ (lane & 7)) << 4)) =
+              make_uint4(pack_bf16(f[8 * q4], f[8 * q4 + 1]), pack_bf16(f[8 * q4 + 2], f[8 * q4 + 3]),
+                         pack_bf16(f[8 * q4 + 4], f[8 * q4 + 5]), pack_bf16(f[8 * q4 + 6], f[8 * q4 + 7]));
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the store reads these writes
+      __syncwarp();
+      if (ok) {
+        tma_store_3d(&tmO, rows, 0, query0, h);
+        tma_store_3d(&tmO, rows + L::SUB, 64, query0, h);
+        tma_store_wait_read();
       }
     }
   }

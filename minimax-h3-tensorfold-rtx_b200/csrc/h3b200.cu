@@ -751,10 +751,24 @@ int h3_attn_fp8_sparse(const void* q, const void* k, const void* v, long long ld
                   workspace_bytes, stream);
 }
 
-size_t h3_attn_bf16_workspace_bytes(int S, int Hk) {
-  if (S < 2048 || Hk <= 0) return 0;
-  return (size_t)Hk * ((S + 127) / 128) * 4;
+namespace {
+// workspace of h3_attn_bf16: key norms, span ranges, tile order
+struct AttnBf16Ws {
+  size_t knorm, range, order, total;
+};
+AttnBf16Ws attn_bf16_ws(int S, int Hk) {
+  const size_t n = (S + 127) / 128;
+  AttnBf16Ws w;
+  w.knorm = 0;
+  w.range = align_up((size_t)Hk * n * 4, 16);
+  w.order = w.range + align_up(n * 8, 16);
+  w.total = w.order + align_up((n + 1) / 2 * 4, 16);
+  return w;
 }
+}  // namespace
+
+// (below 2,048 tokens a row has too few key steps to win back the two extra launches)
+size_t h3_attn_bf16_workspace_bytes(int S, int Hk) { return S < 2048 || Hk <= 0 ? 0 : attn_bf16_ws(S, Hk).total; }
 
 int h3_attn_bf16(const void* q, long long ldq, long long hsq, const void* k, long long ldk, long long hsk,
                  const void* v, long long ldv, long long hsv, int S, int Hq, int Hk, const int* span_lo,
@@ -778,20 +792,42 @@ int h3_attn_bf16(const void* q, long long ldq, long long hsq, const void* k, lon
   if (workspace && (!aligned(workspace, 16) || workspace_bytes < h3_attn_bf16_workspace_bytes(S, Hk)))
     return fail(H3_ERR_ARG, "%s: workspace misaligned, or %zu bytes < %zu", who, workspace_bytes,
                 h3_attn_bf16_workspace_bytes(S, Hk));
-  CUtensorMap tq, tk, tv;
+  CUtensorMap tq, tk, tv, to;
   int rc;
   if ((rc = make_map_bf16(&tq, q, 128, S, Hq, ldq, hsq, 128, who))) return rc;
   if ((rc = make_map_bf16(&tk, k, 128, S, Hk, ldk, hsk, 128, who))) return rc;
   if ((rc = make_map_bf16(&tv, v, 128, S, Hk, ldv, hsv, 128, who))) return rc;
+  if ((rc = make_map_bf16(&to, out, 128, S, Hq, ldo, 128, 32, who))) return rc;
   if ((rc = smem_optin(attn_bf16_kernel, L::TOTAL, &g_optin_attn_bf16, who))) return rc;
-  AttnBf16Args a{reinterpret_cast<__nv_bfloat16*>(out), ldo, reinterpret_cast<const __nv_bfloat16*>(v), ldv, hsv,
-                 span_lo, span_hi, reinterpret_cast<const float*>(workspace), S, Hq / Hk};
+  AttnBf16Args a{};
+  a.v = reinterpret_cast<const __nv_bfloat16*>(v);
+  a.ldv = ldv;
+  a.hsv = hsv;
+  a.lo = span_lo;
+  a.hi = span_hi;
+  a.S = S;
+  a.group = Hq / Hk;
+  a.tiles = (S + 255) / 256;
+  a.heads = Hq;
+  // Tiles before heads lets the longest CTAs of all heads start first, but has every head's K and V in use at once:
+  // only while those fit L2 beside the rest
+  a.tile_major = (long long)Hk * S * 512 <= 96ll << 20;
   if (workspace) {
-    KnormArgs kn{reinterpret_cast<const __nv_bfloat16*>(k), ldk, hsk, S, reinterpret_cast<float*>(workspace)};
-    attn_bf16_knorm_kernel<<<dim3((S + 127) / 128, Hk), 256, 0, S_(stream)>>>(kn);
+    const AttnBf16Ws w = attn_bf16_ws(S, Hk);
+    uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+    AttnBf16Prep pr{reinterpret_cast<const __nv_bfloat16*>(k), ldk, hsk, S, span_lo, span_hi,
+                    reinterpret_cast<float*>(ws + w.knorm), reinterpret_cast<int2*>(ws + w.range),
+                    reinterpret_cast<int*>(ws + w.order)};
+    attn_bf16_prep_kernel<<<dim3((S + 127) / 128, Hk), 256, 0, S_(stream)>>>(pr);
     if ((rc = check_launch(who))) return rc;
+    a.knorm = pr.knorm;
+    if (span_lo && a.tile_major) {
+      attn_bf16_order_kernel<<<1, 1024, 0, S_(stream)>>>(pr, a.tiles);
+      if ((rc = check_launch(who))) return rc;
+      a.order = pr.order;
+    }
   }
-  attn_bf16_kernel<<<dim3((S + 255) / 256, Hq), kAttnBf16Threads, L::TOTAL, S_(stream)>>>(tq, tk, tv, a);
+  attn_bf16_kernel<<<(unsigned)((long long)a.tiles * Hq), kAttnBf16Threads, L::TOTAL, S_(stream)>>>(tq, tk, tv, to, a);
   return check_launch(who);
 }
 

@@ -107,7 +107,7 @@ def test_attn_bf16_checks_its_arguments(lib):
     assert call(ldq=0) == -2 and call(ldq=388) == -2 and call(hsq=-128) == -2 and call(ldk=-8) == -2
     assert call(q=FAKE + 8) == -1 and "16-byte" in N.last_error()
     need = lib.h3_attn_bf16_workspace_bytes(5000, 3)
-    assert need == 3 * 40 * 4 and lib.h3_attn_bf16_workspace_bytes(100, 3) == 0
+    assert need >= 3 * 40 * 4 and lib.h3_attn_bf16_workspace_bytes(100, 3) == 0
     assert call(S=5000, Hq=3, Hk=3, ldo=384, ws=FAKE, size=need - 1) == -1 and "workspace" in N.last_error()
     assert call(S=5000, Hq=3, Hk=3, ldo=384, ws=FAKE + 4, size=need) == -1
 
