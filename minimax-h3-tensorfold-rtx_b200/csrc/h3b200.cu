@@ -594,13 +594,12 @@ int rope_pos(RopePos* r, const H3Positions* p, const char* who) {
                   2 * kRopeMaxPairs, a, d);
     if (!(p->theta[a] > 0.0) || !std::isfinite(p->theta[a]))
       return fail(H3_ERR_ARG, "%s: theta of axis %d must be positive and finite", who, a);
-    const double step = std::pow(p->theta[a], -2.0 / d);
-    double f = 0.15915494309189533577;   // 1 / (2 pi)
-    for (int j = 0; j < d / 2; ++j, f *= step) {
-      r->axis[r->pairs] = (uint8_t)a;
-      r->turns[r->pairs++] = f;
-    }
+    double f = std::pow(p->theta[a], -2.0 / d);
+    for (int b = 0; b < 6; ++b, f *= f) r->power[a][b] = f;
+    r->pairs += d / 2;
+    r->end[a] = r->pairs;
   }
+  for (int a = p->axes; a < 4; ++a) r->end[a] = r->pairs;
   return H3_OK;
 }
 }  // namespace
@@ -613,7 +612,9 @@ int h3_rope_axes(const H3Positions* pos, int S, float* out, void* stream) {
   if (S <= 0) return fail(H3_ERR_SHAPE, "h3_rope_axes: S must be positive (S=%d)", S);
   const int per = 256 / r.pairs;
   const int need = (int)(((long long)S + per - 1) / per), cap = num_sms() * 8;
-  rope_axes_kernel<<<need < cap ? need : cap, 256, 0, S_(stream)>>>(r, S, reinterpret_cast<float4*>(out));
+  const auto kernel = r.type == H3_POS_I32 ? rope_axes_kernel<H3_POS_I32>
+                      : r.type == H3_POS_I64 ? rope_axes_kernel<H3_POS_I64> : rope_axes_kernel<H3_POS_F32>;
+  kernel<<<need < cap ? need : cap, 256, 0, S_(stream)>>>(r, S, reinterpret_cast<float4*>(out));
   return check_launch("h3_rope_axes");
 }
 
@@ -637,11 +638,17 @@ int h3_qknorm_rope_axes(const void* q, long long ldq, long long hsq, const void*
   QkNormAxesArgs a{reinterpret_cast<const __nv_bfloat16*>(q), reinterpret_cast<const __nv_bfloat16*>(k),
                    reinterpret_cast<__nv_bfloat16*>(out_q), reinterpret_cast<__nv_bfloat16*>(out_k),
                    ldq, hsq, ldk, hsk, ldoq, hsoq, ldok, hsok, S, Hq, Hk, qw, kw, eps};
-  const int blocks = (int)(((long long)S + 7) / 8), groups = (Hq + Hk + 7) / 8;
-  // groups of one token over several blocks while the tokens alone leave SMs without their six resident blocks
-  int split = (num_sms() * 6 + blocks - 1) / blocks;
-  split = split < groups ? split : groups;
-  qknorm_rope_axes_kernel<<<dim3(blocks, split), 256, 0, S_(stream)>>>(a, r);
+  const int blocks = (int)(((long long)S + 7) / 8), groups = ((Hq < Hk ? Hq : Hk) + 3) / 4;
+  // the groups of a token over several blocks while the tokens alone leave SMs without their three resident blocks
+  int split = num_sms() * 3 / blocks;
+  split = split < 1 ? 1 : split < groups ? split : groups;
+  const bool few = Hq == Hk && Hq < 8;
+  if (few) split = 1;
+  const auto kernel =
+      r.type == H3_POS_I32   ? (few ? qknorm_rope_axes_kernel<H3_POS_I32, true> : qknorm_rope_axes_kernel<H3_POS_I32, false>)
+      : r.type == H3_POS_I64 ? (few ? qknorm_rope_axes_kernel<H3_POS_I64, true> : qknorm_rope_axes_kernel<H3_POS_I64, false>)
+                             : (few ? qknorm_rope_axes_kernel<H3_POS_F32, true> : qknorm_rope_axes_kernel<H3_POS_F32, false>);
+  kernel<<<dim3(blocks, split), 256, 0, S_(stream)>>>(a, r);
   return check_launch(who);
 }
 

@@ -97,6 +97,8 @@ def check_norm_rope(got, x, w, a, eps):
 @pytest.mark.parametrize("S,Hq,Hk,dims,kind", [
     (1, 1, 1, (128,), "far"), (7, 4, 4, (32, 32, 32), "grid"), (333, 5, 5, (44, 42, 42), "frac"), (130, 20, 5, (64, 64), "grid"),
     (129, 1, 9, (8,), "grid"), (65, 40, 40, (44, 42, 42), "far"), (2049, 3, 2, (16, 24, 24), "frac"),
+    (20, 6, 6, (64, 64), "grid"), (19, 7, 7, (32, 32, 32), "far"), (9, 3, 3, (16, 24, 24), "frac"), (4000, 8, 8, (128,), "far"),
+    (3, 23, 23, (44, 42, 42), "grid"), (700, 17, 4, (64, 64), "frac"), (77, 2, 31, (32, 32, 32), "grid"),
 ])
 def test_qknorm_rope_axes(S, Hq, Hk, dims, kind):
     from tfvideo import kernels as K
