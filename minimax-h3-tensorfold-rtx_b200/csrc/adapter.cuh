@@ -35,6 +35,22 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {   // addr: clus
   return v;
 }
 
+// warp-wide: transaction bytes expected on a barrier without an arrival
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("{\n\t.reg .pred e;\n\t.reg .b32 rx;\n\t" H3_ELECT
+               "@e mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;\n\t}" ::"r"(smem_u32(bar)), "r"(bytes)
+               : "memory");
+}
+// warp-wide: one arrival
+__device__ __forceinline__ void mbar_arrive_warp(uint64_t* bar) {
+  asm volatile("{\n\t.reg .pred e;\n\t.reg .b32 rx;\n\t" H3_ELECT
+               "@e mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(smem_u32(bar)) : "memory");
+}
+// Programmatic dependent launch: the next kernel of the stream may start its blocks once every block of this one got
+// here, and waits in wait_primary for this one's end (memory included) before it touches what this one wrote.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // One warp: the distinct adapters of rows m0 .. m0 + 127 in rising order; returns how many.
 __device__ __forceinline__ int tile_adapters(const AdapterArgs& a, int m0, int lane, int* list) {
   int id[4];
@@ -66,13 +82,13 @@ __device__ __forceinline__ int tile_adapters(const AdapterArgs& a, int m0, int l
 // and, stacked as the MMA's N rows, the A rows of up to G adapters; a tile with more adapters walks x again for the
 // next G (from L2).  Warps 0-3: epilogue, a thread per row; warp 4: TMA; warp 5: MMA.
 struct ShrinkSmem {
-  static constexpr int X = 128 * 128;
-  __host__ __device__ static constexpr int group(int rp) { return rp >= 64 ? 1 : 64 / rp; }
-  __host__ __device__ static constexpr int slot(int rp) { return X + (rp > 64 ? rp : 64) * 128; }
-  __host__ __device__ static constexpr int stages(int rp) { return 98304 / slot(rp); }
+  static constexpr int X = 128 * 128, SLOT = 2 * X;
+  __host__ __device__ static constexpr int group(int rp) { return 128 / rp; }
+  // two CTAs an SM when there are many, one deeper one when a tile is split
+  __host__ __device__ static constexpr int stages(int splits) { return splits > 1 ? 4 : 3; }
   __host__ __device__ static constexpr int red_row(int rp) { return rp * 4 + 16; }   // padded: threads hold rows
   __host__ __device__ static constexpr int total(int rp, int splits) {
-    return 1024 + stages(rp) * slot(rp) + (splits > 1 ? 128 * red_row(rp) : 0) + 1024;
+    return 1024 + stages(splits) * SLOT + (splits > 1 ? 128 * red_row(rp) : 0) + 1024;
   }
 };
 
@@ -82,8 +98,9 @@ __global__ void __launch_bounds__(192)
   using L = ShrinkSmem;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int G = L::group(a.Rp), slot = L::slot(a.Rp), stages = L::stages(a.Rp);   // stages: 3 or 4
+  constexpr int slot = L::SLOT;
   const int splits = gridDim.y;
+  const int G = L::group(a.Rp), stages = L::stages(splits);
   uint8_t* red = smem + stages * slot;
   uint64_t* full = reinterpret_cast<uint64_t*>(red + (splits > 1 ? 128 * L::red_row(a.Rp) : 0));
   uint64_t* empty = full + 4;
@@ -95,17 +112,27 @@ __global__ void __launch_bounds__(192)
   int* list = count_s + 1;   // [128]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int m0 = blockIdx.x * 128;
-  const uint32_t ncols = a.Rp > 64 ? 128 : 64;
+  constexpr uint32_t ncols = 128;
+  const int chunks = (a.K + 63) >> 6;
+  const int c0 = (int)((long long)chunks * blockIdx.y / splits), c1 = (int)((long long)chunks * (blockIdx.y + 1) / splits);
+  const int ahead = min(stages, c1 - c0);   // x tiles asked for before the tile's adapters are known
 
-  if (threadIdx.x == 32) {
-    for (int s = 0; s < 4; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+  if (warp == 4) {
+    if (lane == 0) {
+      for (int s = 0; s < 4; ++s) {
+        mbar_init(&full[s], 1);
+        mbar_init(&empty[s], 1);
+      }
+      mbar_init(acc_full, 1);
+      mbar_init(acc_empty, 4);
+      mbar_init(drained, 1);
+      fence_barrier_init();
     }
-    mbar_init(acc_full, 1);
-    mbar_init(acc_empty, 4);
-    mbar_init(drained, 1);
-    fence_barrier_init();
+    __syncwarp();
+    for (int i = 0; i < ahead; ++i) {
+      mbar_expect_tx(&full[i], L::X);
+      tma_load_3d(smem + i * slot, &tmX, (c0 + i) * 64, m0, 0, &full[i]);
+    }
   }
   if (warp == 0) {
     const int c = tile_adapters(a, m0, lane, list);
@@ -120,9 +147,8 @@ __global__ void __launch_bounds__(192)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int count = *count_s;
-  const int chunks = (a.K + 63) >> 6;
-  const int c0 = (int)((long long)chunks * blockIdx.y / splits), c1 = (int)((long long)chunks * (blockIdx.y + 1) / splits);
   const int passes = (count + G - 1) / G;
+  launch_dependents();   // (the next kernel's blocks wait for this one to end before they read T)
 
   if (warp == 4) {
     int it = 0;
@@ -134,12 +160,14 @@ __global__ void __launch_bounds__(192)
         ok = __all_sync(~0u, mbar_wait(&empty[st], ((it / stages) & 1) ^ 1, 401));
         if (!ok) break;
         uint8_t* s = smem + st * slot;
-        mbar_arrive_expect_tx(&full[st], L::X + cnt * a.Rp * 128);
-        tma_load_3d(s, &tmX, c * 64, m0, 0, &full[st]);
+        mbar_arrive_expect_tx(&full[st], (it < ahead ? 0 : L::X) + cnt * a.Rp * 128);
+        if (it >= ahead) tma_load_3d(s, &tmX, c * 64, m0, 0, &full[st]);
         for (int g = 0; g < cnt; ++g)
           tma_load_3d(s + L::X + g * a.Rp * 128, &tmA, c * 64, 0, list[p * G + g], &full[st]);
       }
     }
+    // what is still landing: the last stages, and x tiles that no adapter asked for
+    for (; it < ahead; ++it) mbar_arrive_warp(&full[it]);
     for (int j = max(it - stages, 0); j < it; ++j) mbar_drain(&full[j % stages], (j / stages) & 1, 402);
   } else if (warp == 5) {
     int it = 0;
@@ -264,15 +292,20 @@ __global__ void __launch_bounds__(160)
   const int ntile = (a.N + 127) >> 7;
   const int n0 = (blockIdx.x % ntile) * 128, m0 = (blockIdx.x / ntile) * 128;
 
-  if (threadIdx.x == 0) {
-    mbar_init(y_full, 1);
-    mbar_init(t_full, 1);
-    mbar_init(b_full, 1);
-    mbar_init(acc_full, 1);
-    mbar_init(acc_empty, 4);
-    fence_barrier_init();
-  }
   if (warp == 4) {
+    if (lane == 0) {
+      mbar_init(y_full, 1);
+      mbar_init(t_full, 1);
+      mbar_init(b_full, 1);
+      mbar_init(acc_full, 1);
+      mbar_init(acc_empty, 4);
+      fence_barrier_init();
+    }
+    __syncwarp();
+    // y is on its way before the tile's adapters are known (in place, a tile without any reads it for nothing)
+    mbar_arrive_expect_tx(y_full, 2 * L::SUB);
+    tma_load_3d(ys, &tmY, n0, m0, 0, y_full);
+    tma_load_3d(ys + L::SUB, &tmY, n0 + 64, m0, 0, y_full);
     tmem_alloc(tmem_slot, 128);
     tmem_relinquish();
     const int c = tile_adapters(a, m0, lane, list);
@@ -287,15 +320,6 @@ __global__ void __launch_bounds__(160)
   bool ok = true;
 
   if (warp == 4) {
-    if (moves) {
-      mbar_arrive_expect_tx(y_full, 2 * L::SUB);
-      tma_load_3d(ys, &tmY, n0, m0, 0, y_full);
-      tma_load_3d(ys + L::SUB, &tmY, n0 + 64, m0, 0, y_full);
-    }
-    if (count > 0) {
-      mbar_arrive_expect_tx(t_full, kc * L::SUB);
-      for (int c = 0; c < kc; ++c) tma_load_3d(ts + c * L::SUB, &tmT, 64 * c, m0, 0, t_full);
-    }
     constexpr uint32_t idesc = idesc_bf16(128, 128, false);
     int loads = 0, products = 0;   // B tiles asked for, products committed
     for (int i = 0; i < count; ++i) {
@@ -303,7 +327,11 @@ __global__ void __launch_bounds__(160)
       if (i > 0 && !(ok = __all_sync(~0u, mbar_wait(acc_full, (i - 1) & 1, 431)))) break;
       mbar_arrive_expect_tx(b_full, kc * L::SUB);
       for (int c = 0; c < kc; ++c) tma_load_3d(bs + c * L::SUB, &tmB, 64 * c, n0, list[i], b_full);
-      ++loads;
+      if (loads++ == 0) {
+        wait_primary();
+        mbar_arrive_expect_tx(t_full, kc * L::SUB);
+        for (int c = 0; c < kc; ++c) tma_load_3d(ts + c * L::SUB, &tmT, 64 * c, m0, 0, t_full);
+      }
       ok = __all_sync(~0u, mbar_wait(b_full, i & 1, 432)) && __all_sync(~0u, mbar_wait(t_full, 0, 433)) &&
            (i == 0 || __all_sync(~0u, mbar_wait(acc_empty, (i - 1) & 1, 434)));
       if (!ok) break;
@@ -316,9 +344,10 @@ __global__ void __launch_bounds__(160)
       ++products;
     }
     // every copy has landed and every product is complete before the store and the end of the CTA
-    if (moves) mbar_drain(y_full, 0, 435);
-    if (count > 0) mbar_drain(t_full, 0, 435);
+    mbar_drain(y_full, 0, 435);
+    if (loads > 0) mbar_drain(t_full, 0, 435);
     if (loads > 0) mbar_drain(b_full, (loads - 1) & 1, 435);
+    if (loads == 0) wait_primary();   // (a call ends after both its kernels)
     if (products > 0) mbar_drain(acc_full, (products - 1) & 1, 436);
   } else {
     const int row = threadIdx.x, m = m0 + row;

@@ -891,7 +891,13 @@ int h3_adapter_add(const void* x, long long ldx, const void* y, long long ldy, c
   cudaError_t e = cudaLaunchKernelEx(&cfg, adapter_shrink_kernel, tx, ta, a);
   if (e != cudaSuccess) return fail(H3_ERR_CUDA, "%s: cluster launch: %s", who, cudaGetErrorString(e));
   if ((rc = check_launch(who))) return rc;
-  adapter_expand_kernel<<<(unsigned)(mtiles * ntiles), 160, ExpandSmem::total(Rp), S_(stream)>>>(ty, tt, tb, to, a);
+  cfg.gridDim = dim3((unsigned)(mtiles * ntiles));
+  cfg.blockDim = dim3(160);
+  cfg.dynamicSmemBytes = ExpandSmem::total(Rp);
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  e = cudaLaunchKernelEx(&cfg, adapter_expand_kernel, ty, tt, tb, to, a);
+  if (e != cudaSuccess) return fail(H3_ERR_CUDA, "%s: launch: %s", who, cudaGetErrorString(e));
   return check_launch(who);
 }
 
