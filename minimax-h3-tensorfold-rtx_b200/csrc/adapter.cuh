@@ -25,6 +25,8 @@ struct AdapterArgs {
   int M, K, N, n;
   int Rp;               // rank rounded up to 16
   int inplace;          // expand: out is y
+  int* next;            // expand: units handed out beyond each CTA's first; shrink sets it to zero
+  int width;            // expand: 128-column tiles a unit
 };
 
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {   // addr: cluster_addr of another CTA's shared memory
@@ -51,9 +53,10 @@ __device__ __forceinline__ void mbar_arrive_warp(uint64_t* bar) {
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// One warp: the distinct adapters of rows m0 .. m0 + 127 in rising order; returns how many.
-__device__ __forceinline__ int tile_adapters(const AdapterArgs& a, int m0, int lane, int* list) {
-  int id[4];
+// One warp: the distinct adapters of rows m0 .. m0 + 127 in rising order; returns how many.  place (may be NULL): each
+// row's place in that list, 255 without an adapter.
+__device__ __forceinline__ int tile_adapters(const AdapterArgs& a, int m0, int lane, int* list, uint8_t* place) {
+  int id[4], at[4] = {255, 255, 255, 255};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int m = m0 + 32 * i + lane;
@@ -68,9 +71,16 @@ __device__ __forceinline__ int tile_adapters(const AdapterArgs& a, int m0, int l
       if (id[i] > last) next = min(next, id[i]);
     next = __reduce_min_sync(~0u, next);
     if (next == INT_MAX) break;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (id[i] == next) at[i] = count;
     if (lane == 0) list[count] = next;
     ++count;
     last = next;
+  }
+  if (place) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) place[32 * i + lane] = (uint8_t)at[i];
   }
   __syncwarp();
   return count;
@@ -85,10 +95,11 @@ struct ShrinkSmem {
   static constexpr int X = 128 * 128, SLOT = 2 * X;
   __host__ __device__ static constexpr int group(int rp) { return 128 / rp; }
   // two CTAs an SM when there are many, one deeper one when a tile is split
-  __host__ __device__ static constexpr int stages(int splits) { return splits > 1 ? 4 : 3; }
+  __host__ __device__ static constexpr int stages(int rp, int splits) { return splits > 1 ? (rp > 64 ? 4 : 5) : 3; }
+  static constexpr int MAX_STAGES = 5;
   __host__ __device__ static constexpr int red_row(int rp) { return rp * 4 + 16; }   // padded: threads hold rows
   __host__ __device__ static constexpr int total(int rp, int splits) {
-    return 1024 + stages(splits) * SLOT + (splits > 1 ? 128 * red_row(rp) : 0) + 1024;
+    return 1024 + stages(rp, splits) * SLOT + (splits > 1 ? 128 * red_row(rp) : 0) + 1024;
   }
 };
 
@@ -100,11 +111,11 @@ __global__ void __launch_bounds__(192)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   constexpr int slot = L::SLOT;
   const int splits = gridDim.y;
-  const int G = L::group(a.Rp), stages = L::stages(splits);
+  const int G = L::group(a.Rp), stages = L::stages(a.Rp, splits);
   uint8_t* red = smem + stages * slot;
   uint64_t* full = reinterpret_cast<uint64_t*>(red + (splits > 1 ? 128 * L::red_row(a.Rp) : 0));
-  uint64_t* empty = full + 4;
-  uint64_t* acc_full = empty + 4;
+  uint64_t* empty = full + L::MAX_STAGES;
+  uint64_t* acc_full = empty + L::MAX_STAGES;
   uint64_t* acc_empty = acc_full + 1;
   uint64_t* drained = acc_empty + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
@@ -119,7 +130,7 @@ __global__ void __launch_bounds__(192)
 
   if (warp == 4) {
     if (lane == 0) {
-      for (int s = 0; s < 4; ++s) {
+      for (int s = 0; s < L::MAX_STAGES; ++s) {
         mbar_init(&full[s], 1);
         mbar_init(&empty[s], 1);
       }
@@ -135,7 +146,7 @@ __global__ void __launch_bounds__(192)
     }
   }
   if (warp == 0) {
-    const int c = tile_adapters(a, m0, lane, list);
+    const int c = tile_adapters(a, m0, lane, list, nullptr);
     if (lane == 0) *count_s = c;
   }
   if (warp == 5) {
@@ -148,6 +159,7 @@ __global__ void __launch_bounds__(192)
   const uint32_t tmem = *tmem_slot;
   const int count = *count_s;
   const int passes = (count + G - 1) / G;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.next = 0;
   launch_dependents();   // (the next kernel's blocks wait for this one to end before they read T)
 
   if (warp == 4) {
@@ -261,144 +273,259 @@ __global__ void __launch_bounds__(192)
 }
 
 // ------------------------------------------------------------------------------------------------ expand
-// A CTA per 128 rows x 128 columns: y, T and B tiles by TMA, one accumulator of 128 columns, out by TMA from where y
-// landed.  Several CTAs an SM keep loads and stores in flight.  Warps 0-3: epilogue, a thread per row; warp 4: the rest.
+// Persistent over units of 128 rows x `width` tiles of 128 columns (T and the list of adapters stay over a unit), the
+// first by block, the others from a counter: SMs get unequal shares of the memory, and equal runs of tiles ended between
+// 371 and 526 us.  y, T and B tiles
+// come by TMA through rings, out goes by TMA from where y landed, 32 rows a warp.  Warps 0-3 and 4-7: epilogue of every other
+// tile, a thread per row (one such group took 2,900 cycles a tile, twice what memory allows); warp 8: TMA and the
+// lists; warp 9: MMA.
 struct ExpandSmem {
   static constexpr int SUB = 128 * 128;   // 128 rows x 64 elements
   __host__ __device__ static constexpr int kc(int rp) { return rp > 64 ? 2 : 1; }
-  __host__ __device__ static constexpr int total(int rp) { return 1024 + 2 * SUB + 2 * kc(rp) * SUB + 1024; }
+  // y tiles in the ring: an even number, so that a slot always belongs to the same epilogue group (a barrier that two
+  // groups took turns to wait on could be a phase behind for one of them)
+  static constexpr int YS = 4;
+  __host__ __device__ static constexpr int ts(int rp) { return rp > 64 ? 1 : 2; }   // T tiles
+  __host__ __device__ static constexpr int total(int rp) {
+    return 1024 + (2 * YS + (ts(rp) + 2) * kc(rp)) * SUB + 2048;
+  }
 };
 
-__global__ void __launch_bounds__(160)
+__global__ void __launch_bounds__(320)
     adapter_expand_kernel(const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmT,
                           const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmO,
                           const AdapterArgs a) {
   using L = ExpandSmem;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int kc = L::kc(a.Rp);
-  uint8_t* ys = smem;
-  uint8_t* ts = ys + 2 * L::SUB;
-  uint8_t* bs = ts + kc * L::SUB;
-  uint64_t* y_full = reinterpret_cast<uint64_t*>(bs + kc * L::SUB);
-  uint64_t* t_full = y_full + 1;
-  uint64_t* b_full = t_full + 1;
-  uint64_t* acc_full = b_full + 1;
-  uint64_t* acc_empty = acc_full + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 1);
-  int* count_s = reinterpret_cast<int*>(tmem_slot + 1);
-  int* list = count_s + 1;   // [128]
+  constexpr int nys = L::YS;
+  const int kc = L::kc(a.Rp), nts = L::ts(a.Rp);
+  uint8_t* ys = smem;                         // [nys][2 SUB]
+  uint8_t* ts = ys + 2 * nys * L::SUB;        // [nts][kc SUB]
+  uint8_t* bs = ts + nts * kc * L::SUB;       // [2][kc SUB]
+  uint64_t* y_full = reinterpret_cast<uint64_t*>(bs + 2 * kc * L::SUB);   // [4]
+  uint64_t* y_empty = y_full + 4;    // [4]: out has been read from the slot, by each epilogue warp
+  uint64_t* t_full = y_empty + 4;    // [2]
+  uint64_t* t_empty = t_full + 2;
+  uint64_t* b_full = t_empty + 2;    // [2]
+  uint64_t* b_empty = b_full + 2;
+  uint64_t* acc_full = b_empty + 2;  // [2]: the product of an epilogue group's tile
+  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* list_full = acc_empty + 2;   // [2]: the adapters of a row tile
+  uint64_t* list_empty = list_full + 2;
+  uint64_t* drained = list_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+  int* unit_s = reinterpret_cast<int*>(tmem_slot + 1);    // [2]: -1 ends
+  int* count_s = unit_s + 2;                              // [2]
+  int* list_s = count_s + 2;                              // [2][128]: adapters of the unit's rows
+  uint8_t* place_s = reinterpret_cast<uint8_t*>(list_s + 256);   // [2][128]: each row's place among them
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int ntile = (a.N + 127) >> 7;
-  const int n0 = (blockIdx.x % ntile) * 128, m0 = (blockIdx.x / ntile) * 128;
-
-  if (warp == 4) {
+  const int strips = (ntile + a.width - 1) / a.width, units = strips * ((a.M + 127) >> 7);
+  if (warp == 8) {
     if (lane == 0) {
-      mbar_init(y_full, 1);
-      mbar_init(t_full, 1);
-      mbar_init(b_full, 1);
-      mbar_init(acc_full, 1);
-      mbar_init(acc_empty, 4);
+      for (int s = 0; s < 4; ++s) {
+        mbar_init(&y_full[s], 1);
+        mbar_init(&y_empty[s], 4);
+      }
+      for (int s = 0; s < 2; ++s) {
+        mbar_init(&t_full[s], 1);
+        mbar_init(&t_empty[s], 1);
+        mbar_init(&b_full[s], 1);
+        mbar_init(&b_empty[s], 1);
+        mbar_init(&acc_full[s], 1);
+        mbar_init(&acc_empty[s], 4);
+        mbar_init(&list_full[s], 1);
+        mbar_init(&list_empty[s], 9);
+      }
+      mbar_init(drained, 1);
       fence_barrier_init();
     }
     __syncwarp();
-    // y is on its way before the tile's adapters are known (in place, a tile without any reads it for nothing)
-    mbar_arrive_expect_tx(y_full, 2 * L::SUB);
-    tma_load_3d(ys, &tmY, n0, m0, 0, y_full);
-    tma_load_3d(ys + L::SUB, &tmY, n0 + 64, m0, 0, y_full);
-    tmem_alloc(tmem_slot, 128);
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, 256);
     tmem_relinquish();
-    const int c = tile_adapters(a, m0, lane, list);
-    if (lane == 0) *count_s = c;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int count = *count_s;
-  const bool moves = count > 0 || !a.inplace;   // in place, a tile without adapters stays as it is
-  bool ok = true;
+  // a unit's first row and its tiles [x0, x1) of columns
+  auto locate = [&](int unit, int& m0, int& x0, int& x1) {
+    m0 = unit / strips * 128;
+    x0 = unit % strips * a.width;
+    x1 = min(x0 + a.width, ntile);
+  };
 
-  if (warp == 4) {
-    constexpr uint32_t idesc = idesc_bf16(128, 128, false);
-    int loads = 0, products = 0;   // B tiles asked for, products committed
-    for (int i = 0; i < count; ++i) {
-      // (the previous product is complete: its B tile may be overwritten)
-      if (i > 0 && !(ok = __all_sync(~0u, mbar_wait(acc_full, (i - 1) & 1, 431)))) break;
-      mbar_arrive_expect_tx(b_full, kc * L::SUB);
-      for (int c = 0; c < kc; ++c) tma_load_3d(bs + c * L::SUB, &tmB, 64 * c, n0, list[i], b_full);
-      if (loads++ == 0) {
-        wait_primary();
-        mbar_arrive_expect_tx(t_full, kc * L::SUB);
-        for (int c = 0; c < kc; ++c) tma_load_3d(ts + c * L::SUB, &tmT, 64 * c, m0, 0, t_full);
+  if (warp == 8) {
+    int ny = 0, nt = 0, nb = 0;   // y, T and B tiles asked for
+    bool ok = true;
+    auto load_y = [&](int m0, int x) {
+      const int st = ny % nys;
+      if (!(ok = __all_sync(~0u, mbar_wait(&y_empty[st], ((ny / nys) & 1) ^ 1, 451)))) return;
+      mbar_arrive_expect_tx(&y_full[st], 2 * L::SUB);
+      tma_load_3d(ys + 2 * st * L::SUB, &tmY, x * 128, m0, 0, &y_full[st]);
+      tma_load_3d(ys + (2 * st + 1) * L::SUB, &tmY, x * 128 + 64, m0, 0, &y_full[st]);
+      ++ny;
+    };
+    bool waited = false;
+    int unit = blockIdx.x;
+    for (int it = 0; ok; ++it) {
+      int m0 = 0, x0 = 0, x1 = 0;
+      if (unit < units) {
+        locate(unit, m0, x0, x1);
+        // out of place every tile of y is needed: the first is on its way before the adapters are known
+        if (!a.inplace) load_y(m0, x0);
       }
-      ok = __all_sync(~0u, mbar_wait(b_full, i & 1, 432)) && __all_sync(~0u, mbar_wait(t_full, 0, 433)) &&
-           (i == 0 || __all_sync(~0u, mbar_wait(acc_empty, (i - 1) & 1, 434)));
-      if (!ok) break;
-      tc_fence_after();
-      for (int kk = 0; kk < a.Rp / 16; ++kk) {
-        const uint32_t off = (kk >> 2) * L::SUB + (kk & 3) * 32;
-        mma_bf16_ss(tmem, sdesc_kmajor_sw128(smem_u32(ts) + off), sdesc_kmajor_sw128(smem_u32(bs) + off), idesc, kk != 0);
+      if (!ok || !(ok = __all_sync(~0u, mbar_wait(&list_empty[it & 1], ((it >> 1) & 1) ^ 1, 450)))) break;
+      int* list = list_s + (it & 1) * 128;
+      const int count = unit < units ? tile_adapters(a, m0, lane, list, place_s + (it & 1) * 128) : 0;
+      if (lane == 0) {
+        unit_s[it & 1] = unit < units ? unit : -1;
+        count_s[it & 1] = count;
+        mbar_arrive(&list_full[it & 1]);
       }
-      tc_commit(acc_full);
-      ++products;
-    }
-    // every copy has landed and every product is complete before the store and the end of the CTA
-    mbar_drain(y_full, 0, 435);
-    if (loads > 0) mbar_drain(t_full, 0, 435);
-    if (loads > 0) mbar_drain(b_full, (loads - 1) & 1, 435);
-    if (loads == 0) wait_primary();   // (a call ends after both its kernels)
-    if (products > 0) mbar_drain(acc_full, (products - 1) & 1, 436);
-  } else {
-    const int row = threadIdx.x, m = m0 + row;
-    int id = m < a.M ? a.rows[m] : -1;
-    if (id >= a.n) id = -1;
-    const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
-    ok = count == 0 || __all_sync(~0u, mbar_wait(y_full, 0, 440));
-    for (int i = 0; i < count; ++i) {
-      if (!(ok = ok && __all_sync(~0u, mbar_wait(acc_full, i & 1, 441)))) break;
-      tc_fence_after();
-      const bool mine = id == list[i];
-      if (__any_sync(~0u, mine)) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t d[32];
-          tmem_ld32(tmem + lane_off + 32 * c, d);
-          tmem_ld_wait();
-          if (mine) {
-            uint8_t* sub = ys + (c >> 1) * L::SUB + row * 128;   // 16-byte pieces, swizzled as TMA wrote them
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              uint4* at = reinterpret_cast<uint4*>(sub + ((((c & 1) * 4 + q) ^ (row & 7)) << 4));
-              uint4 u = *at;
-              uint32_t* w = &u.x;
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                w[e] = pack_bf16(bf16_lo(w[e]) + __uint_as_float(d[8 * q + 2 * e]),
-                                 bf16_hi(w[e]) + __uint_as_float(d[8 * q + 2 * e + 1]));
-              *at = u;
-            }
-          }
-          __syncwarp();
+      __syncwarp();
+      if (unit >= units) break;
+      if (!waited) wait_primary();   // before T and the counter
+      waited = true;
+      if (lane == 0) unit = gridDim.x + atomicAdd(a.next, 1);
+      if (count > 0) {
+        const int st = nt % nts;
+        if (!(ok = __all_sync(~0u, mbar_wait(&t_empty[st], ((nt / nts) & 1) ^ 1, 452)))) break;
+        mbar_arrive_expect_tx(&t_full[st], kc * L::SUB);
+        for (int c = 0; c < kc; ++c) tma_load_3d(ts + (st * kc + c) * L::SUB, &tmT, 64 * c, m0, 0, &t_full[st]);
+        ++nt;
+      }
+      for (int x = x0; ok && x < x1; ++x) {
+        if (a.inplace ? count > 0 : x > x0) load_y(m0, x);   // (in place, a tile without adapters stays as it is)
+        for (int i = 0; ok && i < count; ++i, ++nb) {
+          const int st = nb & 1;
+          if (!(ok = __all_sync(~0u, mbar_wait(&b_empty[st], ((nb >> 1) & 1) ^ 1, 453)))) break;
+          mbar_arrive_expect_tx(&b_full[st], kc * L::SUB);
+          for (int c = 0; c < kc; ++c)
+            tma_load_3d(bs + (st * kc + c) * L::SUB, &tmB, 64 * c, x * 128, list[i], &b_full[st]);
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(acc_empty);
+      unit = __shfl_sync(~0u, unit, 0);
     }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the store reads these writes
+    for (int j = max(ny - nys, 0); j < ny; ++j) mbar_drain(&y_full[j % nys], (j / nys) & 1, 454);
+    for (int j = max(nt - nts, 0); j < nt; ++j) mbar_drain(&t_full[j % nts], (j / nts) & 1, 454);
+    for (int j = max(nb - 2, 0); j < nb; ++j) mbar_drain(&b_full[j & 1], (j >> 1) & 1, 454);
+  } else if (warp == 9) {
+    constexpr uint32_t idesc = idesc_bf16(128, 128, false);
+    int nt = 0, nb = 0, ny = 0;   // T tiles, products and y tiles so far
+    int np[2] = {0, 0};           // products of each group's tiles
+    bool ok = true;
+    for (int it = 0; ok; ++it) {
+      if (!(ok = __all_sync(~0u, mbar_wait(&list_full[it & 1], (it >> 1) & 1, 460)))) break;
+      const int unit = unit_s[it & 1], count = count_s[it & 1];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&list_empty[it & 1]);
+      if (unit < 0) break;
+      int m0, x0, x1;
+      locate(unit, m0, x0, x1);
+      if (count == 0) {
+        if (!a.inplace) ny += x1 - x0;
+        continue;
+      }
+      const int tt = nt % nts;
+      if (!(ok = __all_sync(~0u, mbar_wait(&t_full[tt], (nt / nts) & 1, 461)))) break;
+      const uint32_t ta = smem_u32(ts + tt * kc * L::SUB);
+      for (int x = x0; ok && x < x1; ++x, ++ny) {
+        const int g = ny & 1;
+        for (int i = 0; i < count; ++i, ++nb) {
+          const int st = nb & 1, k = g ? np[1]++ : np[0]++;
+          ok = __all_sync(~0u, mbar_wait(&b_full[st], (nb >> 1) & 1, 462)) &&
+               __all_sync(~0u, mbar_wait(&acc_empty[g], (k & 1) ^ 1, 463));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t ba = smem_u32(bs + st * kc * L::SUB);
+          for (int kk = 0; kk < a.Rp / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * L::SUB + (kk & 3) * 32;
+            mma_bf16_ss(tmem + g * 128, sdesc_kmajor_sw128(ta + off), sdesc_kmajor_sw128(ba + off), idesc, kk != 0);
+          }
+          tc_commit(&acc_full[g]);
+          tc_commit(&b_empty[st]);
+        }
+      }
+      if (!ok) break;
+      tc_commit(&t_empty[tt]);
+      ++nt;
+    }
+    tc_commit(drained);   // every MMA has left the tensor core before TMEM is given back
+    mbar_drain(drained, 0, 464);
+  } else {
+    const int row = threadIdx.x & 127, group = warp >> 2;
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    int ny = 0, np = 0;
+    bool ok = true;
+    for (int it = 0; ok; ++it) {
+      if (!(ok = __all_sync(~0u, mbar_wait(&list_full[it & 1], (it >> 1) & 1, 440)))) break;
+      const int unit = unit_s[it & 1], count = count_s[it & 1];
+      if (unit < 0) break;
+      const int own = place_s[(it & 1) * 128 + row];
+      int m0, x0, x1;
+      locate(unit, m0, x0, x1);
+      const int r0 = m0 + (warp & 3) * 32;
+      for (int x = x0; x < x1 && (count > 0 || !a.inplace); ++x, ++ny) {
+        if ((ny & 1) != group) continue;   // the other group's tile
+        const int st = ny % nys;
+        uint8_t* yt = ys + 2 * st * L::SUB;
+        if (!(ok = __all_sync(~0u, mbar_wait(&y_full[st], (ny / nys) & 1, 441)))) break;
+        for (int i = 0; i < count; ++i, ++np) {
+          if (!(ok = __all_sync(~0u, mbar_wait(&acc_full[group], np & 1, 442)))) break;
+          tc_fence_after();
+          const bool mine = own == i;
+          if (__any_sync(~0u, mine)) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t d[32];
+              tmem_ld32(tmem + lane_off + group * 128 + 32 * c, d);
+              tmem_ld_wait();
+              if (mine) {
+                uint8_t* sub = yt + (c >> 1) * L::SUB + row * 128;   // 16-byte pieces, swizzled as TMA wrote them
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  uint4* at = reinterpret_cast<uint4*>(sub + ((((c & 1) * 4 + q) ^ (row & 7)) << 4));
+                  uint4 u = *at;
+                  uint32_t* w = &u.x;
+#pragma unroll
+                  for (int e = 0; e < 4; ++e)
+                    w[e] = pack_bf16(bf16_lo(w[e]) + __uint_as_float(d[8 * q + 2 * e]),
+                                     bf16_hi(w[e]) + __uint_as_float(d[8 * q + 2 * e + 1]));
+                  *at = u;
+                }
+              }
+              __syncwarp();
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_empty[group]);
+        }
+        if (!ok) break;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the store reads these writes
+        __syncwarp();
+        if (r0 < a.M) {
+          const uint8_t* from = yt + (warp & 3) * 32 * 128;
+          tma_store_3d(&tmO, from, x * 128, r0, 0);
+          if (x * 128 + 64 < a.N) tma_store_3d(&tmO, from + L::SUB, x * 128 + 64, r0, 0);
+        }
+        tma_store_commit();
+        tma_store_wait_read<0>();
+        if (lane == 0) mbar_arrive(&y_empty[st]);
+        __syncwarp();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&list_empty[it & 1]);
+    }
   }
   tc_fence_before();
-  const bool good = __syncthreads_and(ok);
+  __syncthreads();
   tc_fence_after();
-  if (warp == 4) {
-    if (moves && good) {
-      tma_store_3d(&tmO, ys, n0, m0, 0);
-      if (n0 + 64 < a.N) tma_store_3d(&tmO, ys + L::SUB, n0 + 64, m0, 0);
-      tma_store_wait_read();
-    }
-    tmem_dealloc(tmem, 128);
-  }
+  if (warp == 9) tmem_dealloc(tmem, 256);
 }
 
 }  // namespace h3

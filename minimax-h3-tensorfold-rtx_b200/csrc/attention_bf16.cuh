@@ -100,10 +100,14 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void*
       "r"(y), "r"(z), "r"(smem_u32(smem_src))
       : "memory");
 }
-// the elected lane's stores have read their shared memory
+// warp-wide: the elected lane's stores so far become a group; all but its last N groups have read their shared memory
+__device__ __forceinline__ void tma_store_commit() {
+  asm volatile("{\n\t.reg .pred e;\n\t.reg .b32 rx;\n\t" H3_ELECT "@e cp.async.bulk.commit_group;\n\t}" ::: "memory");
+}
+template <int N>
 __device__ __forceinline__ void tma_store_wait_read() {
-  asm volatile("{\n\t.reg .pred e;\n\t.reg .b32 rx;\n\t" H3_ELECT
-               "@e cp.async.bulk.commit_group;\n\t@e cp.async.bulk.wait_group.read 0;\n\t}" ::: "memory");
+  asm volatile("{\n\t.reg .pred e;\n\t.reg .b32 rx;\n\t" H3_ELECT "@e cp.async.bulk.wait_group.read %0;\n\t}" ::"n"(N)
+               : "memory");
 }
 
 struct AttnBf16Args {
@@ -646,7 +650,8 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
       if (ok) {
         tma_store_3d(&tmO, rows, 0, query0, h);
         tma_store_3d(&tmO, rows + L::SUB, 64, query0, h);
-        tma_store_wait_read();
+        tma_store_commit();
+        tma_store_wait_read<0>();
       }
     }
   }

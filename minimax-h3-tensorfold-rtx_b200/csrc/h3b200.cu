@@ -841,7 +841,7 @@ int h3_attn_bf16(const void* q, long long ldq, long long hsq, const void* k, lon
 // ------------------------------------------------------------------------------------------------ adapters
 size_t h3_adapter_workspace_bytes(int M, int R) {
   if (M <= 0 || R <= 0) return 0;
-  return (size_t)M * (size_t)((R + 15) / 16 * 16) * 2;
+  return (size_t)M * (size_t)((R + 15) / 16 * 16) * 2 + 16;   // T, and the counter of units
 }
 
 int h3_adapter_add(const void* x, long long ldx, const void* y, long long ldy, const void* A, const void* B,
@@ -868,10 +868,16 @@ int h3_adapter_add(const void* x, long long ldx, const void* y, long long ldy, c
   if ((rc = make_map_bf16(&ty, y, N, M, 1, ldy, 0, 128, who))) return rc;
   if ((rc = make_map_bf16(&tt, workspace, Rp, M, 1, Rp, 0, 128, who))) return rc;
   if ((rc = make_map_bf16(&tb, B, R, N, n, R, (long long)N * R, 128, who))) return rc;
-  if ((rc = make_map_bf16(&to, out, N, M, 1, ldo, 0, 128, who))) return rc;
+  if ((rc = make_map_bf16(&to, out, N, M, 1, ldo, 0, 32, who))) return rc;
   if ((rc = smem_optin(adapter_shrink_kernel, 220 * 1024, &g_optin_shrink, who))) return rc;
   if ((rc = smem_optin(adapter_expand_kernel, ExpandSmem::total(128), &g_optin_expand, who))) return rc;
-  AdapterArgs a{rows, scale, reinterpret_cast<__nv_bfloat16*>(workspace), M, K, N, n, Rp, out == y && ldo == ldy};
+  AdapterArgs a{rows, scale, reinterpret_cast<__nv_bfloat16*>(workspace), M, K, N, n, Rp, out == y && ldo == ldy,
+                reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(workspace) + (size_t)M * Rp * 2), 1};
+  // units of up to eight column tiles, as long as every SM has four of them (the list of a unit's adapters takes about
+  // as long as one tile)
+  a.width = (int)(mtiles * ntiles / (4ll * num_sms()));
+  a.width = a.width < 1 ? 1 : a.width > 8 ? 8 : a.width;
+  const long long units = mtiles * ((ntiles + a.width - 1) / a.width);
   // the K range over a cluster of CTAs while the row tiles alone leave SMs idle, at least four 64-element stages each
   const int chunks = (K + 63) / 64;
   int splits = 1;
@@ -891,8 +897,8 @@ int h3_adapter_add(const void* x, long long ldx, const void* y, long long ldy, c
   cudaError_t e = cudaLaunchKernelEx(&cfg, adapter_shrink_kernel, tx, ta, a);
   if (e != cudaSuccess) return fail(H3_ERR_CUDA, "%s: cluster launch: %s", who, cudaGetErrorString(e));
   if ((rc = check_launch(who))) return rc;
-  cfg.gridDim = dim3((unsigned)(mtiles * ntiles));
-  cfg.blockDim = dim3(160);
+  cfg.gridDim = dim3((unsigned)(units < num_sms() ? units : num_sms()));
+  cfg.blockDim = dim3(320);
   cfg.dynamicSmemBytes = ExpandSmem::total(Rp);
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;

@@ -158,7 +158,7 @@ def test_adapter_add_checks_its_arguments(lib):
     for bad in (dict(M=0), dict(K=0), dict(K=60), dict(N=4), dict(R=0), dict(R=12), dict(R=136), dict(n=0), dict(ldx=56),
                 dict(ldx=68), dict(ldy=56), dict(ldo=66)):
         assert call(**bad) == -2, bad
-    assert lib.h3_adapter_workspace_bytes(10, 8) == 320 and lib.h3_adapter_workspace_bytes(0, 8) == 0
+    assert lib.h3_adapter_workspace_bytes(10, 8) >= 320 and lib.h3_adapter_workspace_bytes(0, 8) == 0
     assert lib.h3_act(FAKE, 16, FAKE, 8, 4, 8, 2, None, None) == -2 and lib.h3_act(FAKE, 16, FAKE, 8, 4, 8, 3, None, None) == -1
 
 
