@@ -185,14 +185,13 @@ def bf16_tokens(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Te
     16-byte aligned); out [S, Hq * 128] bf16, row stride a multiple of 8."""
 
     (S, Hq, _), Hk = q.shape, k.shape[1]
-    _bf16_launch(S, Hq, Hk, [(t, t.stride(0), t.stride(1)) for t in (q, k, v)], out, mask)
+    _bf16_launch(S, Hq, Hk, q, q.stride(), k, k.stride(), v, v.stride(), out, out.stride(0), mask)
     return out
 
 
-def _bf16_launch(S: int, Hq: int, Hk: int, rows, out: torch.Tensor, mask: SpanMask | None) -> None:
-    """``rows``: (tensor, token stride, head stride) of q, k and v."""
+def _bf16_launch(S, Hq, Hk, q, sq, k, sk, v, sv, out, ldo, mask: SpanMask | None) -> None:
+    """``sq``, ``sk``, ``sv``: (token stride, head stride, ...) of q, k and v."""
 
-    (q, ldq, hsq), (k, ldk, hsk), (v, ldv, hsv) = rows
     if mask is None:
         lo = hi = None
         dev = N.one_device("bf16 attention", q, k, v, out)
@@ -204,30 +203,38 @@ def _bf16_launch(S: int, Hq: int, Hk: int, rows, out: torch.Tensor, mask: SpanMa
     if S and Hq:
         size = N.attn_bf16_workspace_bytes(S, Hk)
         ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-        N.launch(dev, "h3_attn_bf16", 2 if size else 1, q.data_ptr(), ldq, hsq, k.data_ptr(), ldk, hsk, v.data_ptr(), ldv,
-                 hsv, S, Hq, Hk, lo, hi, out.data_ptr(), out.stride(0), ws.data_ptr() if size else None, size)
+        N.launch(dev, "h3_attn_bf16", 1 if ws is None else 2 if mask is None else 3, q.data_ptr(), sq[0], sq[1],
+                 k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0], sv[1], S, Hq, Hk, lo, hi, out.data_ptr(), ldo,
+                 None if ws is None else ws.data_ptr(), size)
+
+
+def _tma_rows(t: torch.Tensor):
+    """t [1, H, S, 128] and its (token stride, head stride); copied when TMA cannot read its rows in place."""
+
+    _, hs, ld, ds = t.stride()
+    if ds != 1 or ld & 7 or hs & 7 or ld <= 0 or hs <= 0 or t.data_ptr() & 15:
+        _, H, S, _ = t.shape     # (a dimension of one entry has any stride)
+        if ds != 1 or t.data_ptr() & 15 or (S > 1 and (ld & 7 or ld <= 0)) or (H > 1 and (hs & 7 or hs <= 0)):
+            t = N.aligned16(t)
+            _, hs, ld, ds = t.stride()
+    return t, (ld, hs)
 
 
 def bf16(q, k, v, mask: SpanMask | None = None):
-    rows = []
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 4 or t.shape[0] != 1 or t.shape[3] != HEAD_DIM or t.dtype != torch.bfloat16:
-            raise ValueError(f"bf16 attention: {name} must be bf16 [1, H, S, {HEAD_DIM}], got {tuple(t.shape)} {t.dtype}")
-        _, hs, ld, ds = t.stride()
-        # read in place by TMA; copied when the strides do not allow it (a dimension of one entry has any)
-        if ds != 1 or t.data_ptr() % 16 or (t.shape[2] > 1 and (ld % 8 or ld <= 0)) \
-                or (t.shape[1] > 1 and (hs % 8 or hs <= 0)):
-            t = N.aligned16(t)
-            _, hs, ld, ds = t.stride()
-        rows.append((t, ld, hs))
-    _, H, S, D = q.shape
-    Hk = k.shape[1]
-    if k.shape != v.shape or k.shape[2] != S or Hk == 0 or H % Hk:
-        raise ValueError(f"bf16 attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: one length, and "
-                         "query heads a multiple of the key heads")
-    out = torch.empty((S, H * D), dtype=torch.bfloat16, device=q.device)
-    _bf16_launch(S, H, Hk, rows, out, mask)
-    return out.view(1, S, H, D).transpose(1, 2)
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or qs[0] != 1 or ks[0] != 1 or qs[3] != HEAD_DIM or ks[3] != HEAD_DIM \
+            or v.shape != ks or not q.dtype == k.dtype == v.dtype == torch.bfloat16:
+        raise ValueError(f"bf16 attention: q, k and v must be bf16 [1, H, S, {HEAD_DIM}], k and v alike, got "
+                         f"{tuple(qs)} {q.dtype}, {tuple(ks)} {k.dtype}, {tuple(v.shape)} {v.dtype}")
+    _, H, S, D = qs
+    Hk = ks[1]
+    if ks[2] != S or Hk == 0 or H % Hk:
+        raise ValueError(f"bf16 attention: q {tuple(qs)}, k and v {tuple(ks)}: one length, and query heads a multiple "
+                         "of the key heads")
+    (q, sq), (k, sk), (v, sv) = _tma_rows(q), _tma_rows(k), _tma_rows(v)
+    out = q.new_empty((1, S, H, D))
+    _bf16_launch(S, H, Hk, q, sq, k, sk, v, sv, out, H * D, mask)
+    return out.transpose(1, 2)
 
 
 def bf16_spans(mask: SpanMask):

@@ -64,7 +64,7 @@ def rope_axes(pos: torch.Tensor, dims, theta=10000.0, out: torch.Tensor | None =
     S = pos.shape[0]
     shape = (S, axes[2] // 2, 2, 2)
     if out is None:
-        out = torch.empty(shape, dtype=torch.float32, device=pos.device)
+        out = pos.new_empty(shape, dtype=torch.float32)
     elif out.shape != shape or out.dtype != torch.float32 or not out.is_contiguous():
         raise ValueError(f"rope_axes: out must be a contiguous fp32 {shape} tensor, got {tuple(out.shape)} {out.dtype}")
     dev = N.one_device("rope_axes", pos, out)
@@ -82,16 +82,22 @@ def qknorm_rope_axes(q: torch.Tensor, k: torch.Tensor, qw: torch.Tensor, kw: tor
 
     axes = _check_positions("qknorm_rope_axes", pos, dims, theta)
     oq, ok = q if out_q is None else out_q, k if out_k is None else out_k
+    qs, ks = q.shape, k.shape
+    if len(qs) != 3 or len(ks) != 3 or qs[2] != HEAD_DIM or ks[2] != HEAD_DIM or oq.shape != qs or ok.shape != ks \
+            or not q.dtype == k.dtype == oq.dtype == ok.dtype == torch.bfloat16:
+        raise ValueError(f"qknorm_rope_axes: q, k and their outputs must be bf16 [S, H, {HEAD_DIM}], got "
+                         + ", ".join(f"{tuple(t.shape)} {t.dtype}" for t in (q, k, oq, ok)))
     st = []
-    for name, t, like in (("q", q, q), ("k", k, k), ("out_q", oq, q), ("out_k", ok, k)):
-        if t.dim() != 3 or t.shape[2] != HEAD_DIM or t.shape != like.shape or t.dtype != torch.bfloat16:
-            raise ValueError(f"qknorm_rope_axes: {name} must be bf16 [S, H, {HEAD_DIM}], got {tuple(t.shape)} {t.dtype}")
+    for t in (q, k) if out_q is None and out_k is None else (q, k, oq, ok):
         ld, hs, ds = t.stride()
-        if ds != 1 or ld % 4 or hs % 4 or t.data_ptr() % 8:
-            raise ValueError(f"qknorm_rope_axes: {name} needs a contiguous head dim and 8-byte aligned rows, got strides "
-                             f"{t.stride()}")
-        st.append((t.data_ptr(), ld, hs))
-    (S, Hq, _), Hk = q.shape, k.shape[1]
+        at = t.data_ptr()
+        if ds != 1 or ld & 3 or hs & 3 or at & 7:
+            raise ValueError("qknorm_rope_axes: q, k and their outputs need a contiguous head dim and 8-byte aligned rows, "
+                             f"got strides {t.stride()}")
+        st += (at, ld, hs)
+    if len(st) == 6:
+        st += st
+    (S, Hq, _), Hk = qs, ks[1]
     if k.shape[0] != S or pos.shape[0] != S:
         raise ValueError(f"qknorm_rope_axes: q has {S} tokens, k {k.shape[0]}, pos {pos.shape[0]}")
     if axes[2] % 8:
@@ -103,8 +109,8 @@ def qknorm_rope_axes(q: torch.Tensor, k: torch.Tensor, qw: torch.Tensor, kw: tor
     qw, kw = _norm_weight(qw), _norm_weight(kw)
     dev = N.one_device("qknorm_rope_axes", q, k, oq, ok, qw, kw, pos)
     if S and Hq:
-        N.launch(dev, "h3_qknorm_rope_axes", 1, *st[0], *st[1], S, Hq, Hk, qw.data_ptr(), kw.data_ptr(),
-                 C.byref(_positions(pos, axes)), eps, *st[2], *st[3])
+        N.launch(dev, "h3_qknorm_rope_axes", 1, *st[:6], S, Hq, Hk, qw.data_ptr(), kw.data_ptr(),
+                 C.byref(_positions(pos, axes)), eps, *st[6:])
     return oq, ok
 
 

@@ -211,25 +211,27 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tens
     inputs).  K, N and R multiples of 8, R <= 128."""
 
     out = y if out is None else out
-    for name, t, d in (("y", y, 2), ("x", x, 2), ("A", A, 3), ("B", B, 3), ("out", out, 2)):
-        if t.dim() != d or t.dtype != torch.bfloat16:
-            raise ValueError(f"adapter_add: {name} must be a {d}-D bf16 tensor, got {tuple(t.shape)} {t.dtype}")
-    (M, K), (n, R, Ka), cols = x.shape, A.shape, y.shape[1]
-    if y.shape[0] != M or Ka != K or B.shape != (n, cols, R) or out.shape != y.shape:
+    bf16 = torch.bfloat16
+    if not (x.dtype == y.dtype == A.dtype == B.dtype == out.dtype == bf16 and x.dim() == y.dim() == 2
+            and A.dim() == B.dim() == 3):
+        raise ValueError("adapter_add: x, y and out must be 2-D, A and B 3-D bf16 tensors, got "
+                         + ", ".join(f"{tuple(t.shape)} {t.dtype}" for t in (x, y, out, A, B)))
+    (M, K), (n, R, Ka), (My, cols) = x.shape, A.shape, y.shape
+    if My != M or Ka != K or B.shape != (n, cols, R) or out.shape != y.shape:
         raise ValueError(f"adapter_add: x {tuple(x.shape)}, y {tuple(y.shape)}, A {tuple(A.shape)}, B {tuple(B.shape)}, "
                          f"out {tuple(out.shape)} do not fit together")
     if rows.shape != (M,) or rows.dtype != torch.int32:
         raise ValueError(f"adapter_add: rows must be int32 [{M}], got {tuple(rows.shape)} {rows.dtype}")
     if scale is not None and (scale.shape != (n,) or scale.dtype != torch.float32):
         raise ValueError(f"adapter_add: scale must be fp32 [{n}], got {tuple(scale.shape)} {scale.dtype}")
-    if K % 8 or cols % 8 or R % 8 or R > 128:
+    if K & 7 or cols & 7 or R & 7 or R > 128:
         raise ValueError(f"adapter_add: K, N and R must be multiples of 8 and R at most 128, got K={K} N={cols} R={R}")
-    for name, t in (("y", y), ("out", out)):
+    for name, t in (("y", y), ("out", out)) if out is not y else (("y", y),):
         ld, cs = t.stride()
-        if (cols > 1 and cs != 1) or ld % 8 or (M > 1 and ld < cols) or t.data_ptr() % 16:
+        if (cols > 1 and cs != 1) or ld & 7 or (M > 1 and ld < cols) or t.data_ptr() & 15:
             raise ValueError(f"adapter_add: {name} needs 16-byte aligned contiguous rows, got strides {t.stride()}")
     ldx, cs = x.stride()
-    if cs != 1 or ldx % 8 or ldx < K or x.data_ptr() % 16:
+    if cs != 1 or ldx & 7 or ldx < K or x.data_ptr() & 15:
         x = N.aligned16(x)
         ldx = x.stride(0)
     A, B, rows = N.aligned16(A), N.aligned16(B), rows.contiguous()
@@ -240,7 +242,7 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tens
         dev = N.one_device("adapter_add", y, x, A, B, rows, out, scale)
     if M and cols and n and K and R:
         size = N.adapter_workspace_bytes(M, R)
-        ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+        ws = x.new_empty(size // 2)
         N.launch(dev, "h3_adapter_add", 2, x.data_ptr(), ldx, y.data_ptr(), y.stride(0), A.data_ptr(), B.data_ptr(),
                  None if scale is None else scale.data_ptr(), rows.data_ptr(), M, K, cols, R, n, out.data_ptr(),
                  out.stride(0), ws.data_ptr(), size)

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+from functools import lru_cache
 from pathlib import Path
 
 import torch
@@ -185,10 +186,12 @@ def attn_workspace_bytes(S: int, H: int) -> int:
     return int(lib().h3_attn_workspace_bytes(S, H))
 
 
+@lru_cache(maxsize=256)
 def attn_bf16_workspace_bytes(S: int, Hk: int) -> int:
     return int(lib().h3_attn_bf16_workspace_bytes(S, Hk))
 
 
+@lru_cache(maxsize=256)
 def adapter_workspace_bytes(M: int, R: int) -> int:
     return int(lib().h3_adapter_workspace_bytes(M, R))
 
