@@ -116,7 +116,8 @@ struct AttnBf16Args {
   const int* lo;             // spans, or NULL: every key
   const int* hi;
   const float* knorm;        // [key heads][S / 128 tiles]: largest |k|^2 of each 128 keys, or NULL
-  const int* order;          // [S / 256 tiles]: the query tiles by falling number of key steps, or NULL
+  const int4* order;         // [S / 256 tiles]: query tiles by falling number of key steps, or NULL; x: tile, y and z:
+                             // first and end key of its rows
   int S, group;              // group: query heads that share a key head
   int tiles, heads;          // CTAs: query tiles x query heads
   int tile_major;            // CTAs in order of tiles (every head of one, then the next), else of heads
@@ -200,7 +201,7 @@ struct AttnBf16Prep {
   const int *lo, *hi;
   float* knorm;
   int2* range;         // [S / 128 tiles]: first and end key of the tile's rows
-  int* order;
+  int4* order;
 };
 __global__ void __launch_bounds__(256) attn_bf16_prep_kernel(const AttnBf16Prep a) {
   __shared__ float red[16];
@@ -249,10 +250,11 @@ __global__ void __launch_bounds__(256) attn_bf16_prep_kernel(const AttnBf16Prep 
 __global__ void __launch_bounds__(1024) attn_bf16_order_kernel(const AttnBf16Prep a, int tiles) {
   __shared__ int w[1024];
   const int t = threadIdx.x, n128 = (a.S + 127) >> 7;
-  int mine = 0;
+  int mine = 0, lo = 0, hi = 0;
   if (t < tiles) {
     const int2 x = a.range[2 * t], y = 2 * t + 1 < n128 ? a.range[2 * t + 1] : make_int2(INT_MAX, 0);
-    const int lo = min(x.x, y.x), hi = max(x.y, y.y);
+    lo = min(x.x, y.x);
+    hi = max(x.y, y.y);
     mine = hi > lo ? (hi - lo + 127) >> 7 : 0;
   }
   w[t] = mine;
@@ -260,7 +262,7 @@ __global__ void __launch_bounds__(1024) attn_bf16_order_kernel(const AttnBf16Pre
   if (t >= tiles) return;
   int rank = 0;
   for (int i = 0; i < tiles; ++i) rank += w[i] > mine || (w[i] == mine && i < t);
-  a.order[rank] = t;
+  a.order[rank] = make_int4(t, lo, hi, 0);
 }
 
 __global__ void __launch_bounds__(kAttnBf16Threads, 1)
@@ -291,24 +293,41 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
   // the order of CTAs: long ones first where they are known, else the last tiles, which see most under causal spans
   const int h = p.tile_major ? blockIdx.x % p.heads : blockIdx.x / p.tiles, hk = h / p.group;
   const int rank = p.tile_major ? blockIdx.x / p.heads : blockIdx.x % p.tiles;
-  const int q0 = (p.order ? p.order[rank] : p.tiles - 1 - rank) * 256;
+  const int4 known = p.order ? p.order[rank] : make_int4(p.tiles - 1 - rank, 0, p.lo ? 0 : p.S, 0);
+  const int q0 = known.x * 256;
   auto load = [&](int off, const CUtensorMap* map, int row, int head, uint64_t* bar) {
+    mbar_arrive_expect_tx(bar, L::TILE);
     tma_load_3d(smem + off, map, 0, row, head, bar);
     tma_load_3d(smem + off + L::SUB, map, 64, row, head, bar);
   };
-  if (warp == 8) {   // Q needs nothing else: it is on its way before the rest is set up
+  auto load_k = [&](int j, int row) {
+    load(L::K_OFF + j % L::KST * L::TILE, &tmK, row + 128 * j, hk, &k_full[j % L::KST]);
+  };
+  auto load_v = [&](int j, int row) {
+    load(L::V_OFF + j % L::VST * L::TILE, &tmV, row + 128 * j, hk, &v_full[j % L::VST]);
+  };
+  int nk = 0, nv = 0;   // (TMA warp) K and V tiles asked for
+  if (warp == 8) {      // Q, and K and V where their range is known, are on their way before the rest is set up
     if (lane == 0) {
-      mbar_init(q_full, 1);
+      mbar_init(q_full, 2);
+      for (int s = 0; s < L::KST; ++s) {
+        mbar_init(&k_full[s], 1);
+        mbar_init(&k_empty[s], 2);   // a commit of each MMA warp
+      }
+      for (int s = 0; s < L::VST; ++s) {
+        mbar_init(&v_full[s], 1);
+        mbar_init(&v_ok[s], 1);
+        mbar_init(&v_empty[s], 2);
+      }
       fence_barrier_init();
     }
     __syncwarp();
-    mbar_arrive_expect_tx(q_full, 2 * L::TILE);
     load(L::Q_OFF, &tmQ, q0, h, q_full);
     load(L::Q_OFF + L::TILE, &tmQ, q0 + 128, h, q_full);
-    if (lane == 0) {
-      prefetch_tmap(&tmK);
-      prefetch_tmap(&tmV);
-      prefetch_tmap(&tmO);
+    const int sure = known.z > known.y ? (known.z - known.y + 127) >> 7 : 0;
+    for (; nv < min(sure, L::VST); ++nv) {
+      if (nk < L::KST) load_k(nk++, known.y);
+      load_v(nv, known.y);
     }
   }
 
@@ -333,15 +352,6 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
   for (int i = threadIdx.x; i < L::BAD_WORDS; i += kAttnBf16Threads) bad[i] = 0;
   if (threadIdx.x == 0) {
     *any_bad = 0;
-    for (int s = 0; s < L::KST; ++s) {
-      mbar_init(&k_full[s], 1);
-      mbar_init(&k_empty[s], 2);   // a commit of each MMA warp
-    }
-    for (int s = 0; s < L::VST; ++s) {
-      mbar_init(&v_full[s], 1);
-      mbar_init(&v_ok[s], 1);
-      mbar_init(&v_empty[s], 2);
-    }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
       mbar_init(&p_full[2 * t], 4);
@@ -391,17 +401,15 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
 
   if (warp == 8) {
     // ------------------------------------------------------------------ TMA
-    int nk = 0, nv = 0;   // loads issued
     for (int j = 0; j < steps; ++j) {
-      const int ks = j % L::KST, vs = j % L::VST;
-      if (!__all_sync(~0u, mbar_wait(&k_empty[ks], ((j / L::KST) & 1) ^ 1, 301))) break;
-      mbar_arrive_expect_tx(&k_full[ks], L::TILE);
-      load(L::K_OFF + ks * L::TILE, &tmK, base + 128 * j, hk, &k_full[ks]);
-      ++nk;
-      if (!__all_sync(~0u, mbar_wait(&v_empty[vs], ((j / L::VST) & 1) ^ 1, 302))) break;
-      mbar_arrive_expect_tx(&v_full[vs], L::TILE);
-      load(L::V_OFF + vs * L::TILE, &tmV, base + 128 * j, hk, &v_full[vs]);
-      ++nv;
+      if (j >= nk) {
+        if (!__all_sync(~0u, mbar_wait(&k_empty[j % L::KST], ((j / L::KST) & 1) ^ 1, 301))) break;
+        load_k(nk++, base);
+      }
+      if (j >= nv) {
+        if (!__all_sync(~0u, mbar_wait(&v_empty[j % L::VST], ((j / L::VST) & 1) ^ 1, 302))) break;
+        load_v(nv++, base);
+      }
     }
     // nothing may still be landing in this CTA's memory when it ends, after a wait that gave up included
     mbar_drain(q_full, 0, 303);
@@ -613,17 +621,17 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
       // instead of one row a thread (3.7 us of a CTA)
       if (!any) ok = __all_sync(~0u, mbar_wait(q_full, 0, 335));   // Q has landed: nothing overwrites these rows
       uint8_t* rows = smem + L::Q_OFF + t * L::TILE + (warp & 3) * 32 * 128;
-#pragma unroll 1
+      uint32_t o[4][32];
+      if (any) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(o_col + 32 * c, o[c]);
+        tmem_ld_wait();
+      }
+#pragma unroll
       for (int c = 0; c < 4; ++c) {
-        uint32_t o[32];
-        __syncwarp();
-        if (any) {
-          tmem_ld32(o_col + 32 * c, o);
-          tmem_ld_wait();
-        }
         float f[32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) f[e] = live ? __uint_as_float(o[e]) * inv_l : 0.0f;
+        for (int e = 0; e < 32; ++e) f[e] = live ? __uint_as_float(o[c][e]) * inv_l : 0.0f;
         if (repair && live) {   // non-finite V elements this row does see
           for (int j = first; j < last; ++j) {
             if (!((bad[j >> 5] >> (j & 31)) & 1u)) continue;

@@ -769,7 +769,7 @@ AttnBf16Ws attn_bf16_ws(int S, int Hk) {
   w.knorm = 0;
   w.range = align_up((size_t)Hk * n * 4, 16);
   w.order = w.range + align_up(n * 8, 16);
-  w.total = w.order + align_up((n + 1) / 2 * 4, 16);
+  w.total = w.order + (n + 1) / 2 * 16;
   return w;
 }
 }  // namespace
@@ -824,7 +824,7 @@ int h3_attn_bf16(const void* q, long long ldq, long long hsq, const void* k, lon
     uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
     AttnBf16Prep pr{reinterpret_cast<const __nv_bfloat16*>(k), ldk, hsk, S, span_lo, span_hi,
                     reinterpret_cast<float*>(ws + w.knorm), reinterpret_cast<int2*>(ws + w.range),
-                    reinterpret_cast<int*>(ws + w.order)};
+                    reinterpret_cast<int4*>(ws + w.order)};
     attn_bf16_prep_kernel<<<dim3((S + 127) / 128, Hk), 256, 0, S_(stream)>>>(pr);
     if ((rc = check_launch(who))) return rc;
     a.knorm = pr.knorm;
