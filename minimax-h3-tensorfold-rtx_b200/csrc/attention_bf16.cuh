@@ -119,7 +119,8 @@ struct AttnBf16Args {
   const int4* order;         // [S / 256 tiles]: query tiles by falling number of key steps, or NULL; x: tile, y and z:
                              // first and end key of its rows
   int S, group;              // group: query heads that share a key head
-  int tiles, heads;          // CTAs: query tiles x query heads
+  int rows;                  // query rows a CTA: 256, or 128 (tile B unused) when that many CTAs still fit at once
+  int tiles, heads;          // CTAs: query tiles of that many rows x query heads
   int tile_major;            // CTAs in order of tiles (every head of one, then the next), else of heads
 };
 
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
   const int h = p.tile_major ? blockIdx.x % p.heads : blockIdx.x / p.tiles, hk = h / p.group;
   const int rank = p.tile_major ? blockIdx.x / p.heads : blockIdx.x % p.tiles;
   const int4 known = p.order ? p.order[rank] : make_int4(p.tiles - 1 - rank, 0, p.lo ? 0 : p.S, 0);
-  const int q0 = known.x * 256;
+  const int q0 = known.x * p.rows, q_end = min(q0 + p.rows, p.S);
   auto load = [&](int off, const CUtensorMap* map, int row, int head, uint64_t* bar) {
     mbar_arrive_expect_tx(bar, L::TILE);
     tma_load_3d(smem + off, map, 0, row, head, bar);
@@ -323,7 +324,7 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
     }
     __syncwarp();
     load(L::Q_OFF, &tmQ, q0, h, q_full);
-    load(L::Q_OFF + L::TILE, &tmQ, q0 + 128, h, q_full);
+    load(L::Q_OFF + L::TILE, &tmQ, q0 + 128, h, q_full);   // (zeros past the sequence; unused at 128 rows)
     const int sure = known.z > known.y ? (known.z - known.y + 127) >> 7 : 0;
     for (; nv < min(sure, L::VST); ++nv) {
       if (nk < L::KST) load_k(nk++, known.y);
@@ -335,7 +336,7 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
   int lo = 0, hi = 0;
   if (warp < 8) {
     const int query = q0 + threadIdx.x;
-    if (query < p.S) {
+    if (query < q_end) {
       lo = p.lo ? max(p.lo[query], 0) : 0;
       hi = p.hi ? min(p.hi[query], p.S) : p.S;
     }
@@ -610,7 +611,7 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
       ok = __all_sync(~0u, ok && mbar_wait(&o_done[t], 0, 332) &&
                                mbar_wait(&v_ok[(steps - 1) % L::VST], ((steps - 1) / L::VST) & 1, 333));
     const int query0 = q0 + warp * 32;
-    if (ok && query0 < p.S) {
+    if (ok && query0 < q_end) {
       tc_fence_after();
       float la, lb, lc, ld;
       f32x2_unpack(l2a, la, lb);

@@ -814,7 +814,9 @@ int h3_attn_bf16(const void* q, long long ldq, long long hsq, const void* k, lon
   a.hi = span_hi;
   a.S = S;
   a.group = Hq / Hk;
-  a.tiles = (S + 255) / 256;
+  // Half the rows a CTA while all CTAs then run at once: a lone tile's step takes about 0.8 of a pair's
+  a.rows = !workspace && (long long)((S + 127) / 128) * Hq <= num_sms() ? 128 : 256;
+  a.tiles = (S + a.rows - 1) / a.rows;
   a.heads = Hq;
   // Tiles before heads lets the longest CTAs of all heads start first, but has every head's K and V in use at once:
   // only while those fit L2 beside the rest
@@ -828,7 +830,7 @@ int h3_attn_bf16(const void* q, long long ldq, long long hsq, const void* k, lon
     attn_bf16_prep_kernel<<<dim3((S + 127) / 128, Hk), 256, 0, S_(stream)>>>(pr);
     if ((rc = check_launch(who))) return rc;
     a.knorm = pr.knorm;
-    if (span_lo && a.tile_major) {
+    if (span_lo && a.tile_major && a.rows == 256) {
       attn_bf16_order_kernel<<<1, 1024, 0, S_(stream)>>>(pr, a.tiles);
       if ((rc = check_launch(who))) return rc;
       a.order = pr.order;
