@@ -162,10 +162,10 @@ int h3_gemm_nvfp4(const uint8_t* a_codes, const uint8_t* a_sf, const H3ScaleSlot
  * a = rows[m], for bf16 x [M, K], y and out [M, N] (row strides ldx, ldy, ldo; out may be y itself, and is otherwise
  * apart from the inputs), A [n, R, K] and B [n, N, R] contiguous (lower ranks padded with zeros), scale fp32 [n] or
  * NULL (1), rows int32 [M] in any order.  A row whose entry is outside [0, n) has no adapter and is copied bit for bit.
- * Sums in 32 bits; scale[a] A_a x_m is rounded to bf16 once.  K, N, R multiples of 8, R <= 128; pointers 16-byte
- * aligned.  workspace: h3_adapter_workspace_bytes(M, R) bytes, one per call in flight.  The reference merges one adapter
- * set into the weights instead (tfvideo/comfy_nodes.py:95-166). */
-size_t h3_adapter_workspace_bytes(int M, int R);
+ * Sums in 32 bits; scale[a] A_a x_m is rounded to bf16 once.  K, N, R multiples of 8, R <= 128, n <= 2^20; pointers
+ * 16-byte aligned.  workspace: h3_adapter_workspace_bytes(M, R, n) bytes, one per call in flight.  The reference merges
+ * one adapter set into the weights instead (tfvideo/comfy_nodes.py:95-166). */
+size_t h3_adapter_workspace_bytes(int M, int R, int n);
 int h3_adapter_add(const void* x, long long ldx, const void* y, long long ldy, const void* A, const void* B,
                    const float* scale, const int* rows, int M, int K, int N, int R, int n, void* out, long long ldo,
                    void* workspace, size_t workspace_bytes, void* stream);

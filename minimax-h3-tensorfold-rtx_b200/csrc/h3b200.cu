@@ -841,9 +841,30 @@ int h3_attn_bf16(const void* q, long long ldq, long long hsq, const void* k, lon
 }
 
 // ------------------------------------------------------------------------------------------------ adapters
-size_t h3_adapter_workspace_bytes(int M, int R) {
-  if (M <= 0 || R <= 0) return 0;
-  return (size_t)M * (size_t)((R + 15) / 16 * 16) * 2 + 16;   // T, and the counter of units
+namespace {
+// workspace of h3_adapter_add: counters, the plan (more than one adapter) and T
+struct AdapterWs {
+  long long blocks, tiles;   // of the plan; the most tiles there can be
+  size_t counters, tile, perm, t, total;
+};
+AdapterWs adapter_ws(int M, int R, int n) {
+  AdapterWs w;
+  const long long mtiles = ((long long)M + 127) / 128;
+  w.blocks = ((long long)M + kPlanRows - 1) / kPlanRows;
+  // every block of the plan cuts full tiles, and one that is not full for each run, at most 16, or each adapter and none
+  const long long most = n + 1 > 16 ? n + 1ll : 16, groups = most < kPlanRows ? most : kPlanRows;
+  w.tiles = n == 1 ? mtiles : mtiles + w.blocks * groups < M ? mtiles + w.blocks * groups : M;
+  w.counters = 0;
+  w.tile = 16;
+  w.perm = w.tile + (n == 1 ? 0 : (size_t)w.tiles * 16);
+  w.t = align_up(w.perm + (n == 1 ? 0 : (size_t)M * 4), 16);
+  w.total = w.t + (size_t)w.tiles * 128 * ((R + 15) / 16 * 16) * 2;
+  return w;
+}
+}  // namespace
+
+size_t h3_adapter_workspace_bytes(int M, int R, int n) {
+  return M <= 0 || R <= 0 || n <= 0 ? 0 : adapter_ws(M, R, n).total;
 }
 
 int h3_adapter_add(const void* x, long long ldx, const void* y, long long ldy, const void* A, const void* B,
@@ -851,59 +872,99 @@ int h3_adapter_add(const void* x, long long ldx, const void* y, long long ldy, c
                    void* workspace, size_t workspace_bytes, void* stream) {
   const char* who = "h3_adapter_add";
   if (!x || !y || !A || !B || !rows || !out || !workspace) return fail(H3_ERR_ARG, "%s: NULL pointer", who);
-  if (M <= 0 || K <= 0 || N <= 0 || n <= 0 || R <= 0 || K % 8 || N % 8 || R % 8 || R > 128)
-    return fail(H3_ERR_SHAPE, "%s: need K, N, R %% 8 == 0 and R <= 128 (M=%d K=%d N=%d R=%d n=%d)", who, M, K, N, R, n);
+  if (M <= 0 || K <= 0 || N <= 0 || n <= 0 || R <= 0 || K % 8 || N % 8 || R % 8 || R > 128 || n > kPlanMaxAdapters)
+    return fail(H3_ERR_SHAPE, "%s: need K, N, R %% 8 == 0, R <= 128 and n <= %d (M=%d K=%d N=%d R=%d n=%d)", who,
+                kPlanMaxAdapters, M, K, N, R, n);
   if (ldx % 8 || ldy % 8 || ldo % 8 || ldx < K || ldy < N || ldo < N)
     return fail(H3_ERR_SHAPE, "%s: row strides must be multiples of 8 elements, at least the row", who);
   if (!aligned(x, 16) || !aligned(y, 16) || !aligned(A, 16) || !aligned(B, 16) || !aligned(out, 16) ||
       !aligned(workspace, 16) || !aligned(rows, 4) || !aligned(scale, 4))
     return fail(H3_ERR_ARG, "%s: x / y / A / B / out / workspace 16-byte alignment required", who);
-  if (workspace_bytes < h3_adapter_workspace_bytes(M, R))
-    return fail(H3_ERR_ARG, "%s: workspace %zu bytes < %zu", who, workspace_bytes, h3_adapter_workspace_bytes(M, R));
+  const AdapterWs w = adapter_ws(M, R, n);
+  if (workspace_bytes < w.total)
+    return fail(H3_ERR_ARG, "%s: workspace %zu bytes < %zu", who, workspace_bytes, w.total);
   const int Rp = (R + 15) / 16 * 16;
   const long long mtiles = ((long long)M + 127) / 128, ntiles = ((long long)N + 127) / 128;
-  if (mtiles * ntiles > 0x7FFFFFFF) return fail(H3_ERR_SHAPE, "%s: M x N too large (M=%d N=%d)", who, M, N);
+  if (w.tiles * ntiles > 0x3FFFFFFF) return fail(H3_ERR_SHAPE, "%s: M x N too large (M=%d N=%d)", who, M, N);
+  const bool planned = n > 1;
   CUtensorMap tx, ta, ty, tt, tb, to;
   int rc;
   if ((rc = make_map_bf16(&tx, x, K, M, 1, ldx, 0, 128, who))) return rc;
   if ((rc = make_map_bf16(&ta, A, K, R, n, K, (long long)R * K, Rp, who))) return rc;
   if ((rc = make_map_bf16(&ty, y, N, M, 1, ldy, 0, 128, who))) return rc;
-  if ((rc = make_map_bf16(&tt, workspace, Rp, M, 1, Rp, 0, 128, who))) return rc;
+  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+  if ((rc = make_map_bf16(&tt, ws + w.t, Rp, w.tiles * 128, 1, Rp, 0, 128, who))) return rc;
   if ((rc = make_map_bf16(&tb, B, R, N, n, R, (long long)N * R, 128, who))) return rc;
   if ((rc = make_map_bf16(&to, out, N, M, 1, ldo, 0, 32, who))) return rc;
-  if ((rc = smem_optin(adapter_shrink_kernel, 220 * 1024, &g_optin_shrink, who))) return rc;
+  if ((rc = smem_optin(adapter_shrink_kernel, 232448, &g_optin_shrink, who))) return rc;
   if ((rc = smem_optin(adapter_expand_kernel, ExpandSmem::total(128), &g_optin_expand, who))) return rc;
-  AdapterArgs a{rows, scale, reinterpret_cast<__nv_bfloat16*>(workspace), M, K, N, n, Rp, out == y && ldo == ldy,
-                reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(workspace) + (size_t)M * Rp * 2), 1};
-  // units of up to eight column tiles, as long as every SM has four of them (the list of a unit's adapters takes about
-  // as long as one tile)
-  a.width = (int)(mtiles * ntiles / (4ll * num_sms()));
+  int* counters = reinterpret_cast<int*>(ws);   // tiles of the plan, units handed out
+  AdapterArgs a{};
+  a.rows = rows;
+  a.scale = scale;
+  a.x = reinterpret_cast<const __nv_bfloat16*>(x);
+  a.y = reinterpret_cast<const __nv_bfloat16*>(y);
+  a.out = reinterpret_cast<__nv_bfloat16*>(out);
+  a.ldx = ldx;
+  a.ldy = ldy;
+  a.ldo = ldo;
+  a.t = reinterpret_cast<__nv_bfloat16*>(ws + w.t);
+  a.M = M;
+  a.K = K;
+  a.N = N;
+  a.n = n;
+  a.Rp = Rp;
+  a.inplace = out == y && ldo == ldy;
+  a.next = counters + 1;
+  if (planned) {
+    int4* tile = reinterpret_cast<int4*>(ws + w.tile);
+    int* perm = reinterpret_cast<int*>(ws + w.perm);
+    a.tile = tile;
+    a.total = counters;
+    a.perm = perm;
+    if (w.blocks > 1) {   // (one block sets the counters itself)
+      cudaError_t e = cudaMemsetAsync(counters, 0, 8, S_(stream));
+      if (e != cudaSuccess) return fail(H3_ERR_CUDA, "%s: cudaMemsetAsync: %s", who, cudaGetErrorString(e));
+    }
+    adapter_plan_kernel<<<(unsigned)w.blocks, 1024, 0, S_(stream)>>>(
+        PlanArgs{rows, M, n, tile, counters, counters + 1, perm});
+    if ((rc = check_launch(who))) return rc;
+  }
+  // tiles there will be, about
+  const long long tiles = planned ? (mtiles + n < w.tiles ? mtiles + n : w.tiles) : mtiles;
+  // units of up to eight column tiles, as long as every SM has four of them
+  a.width = (int)(tiles * ntiles / (4ll * num_sms()));
   a.width = a.width < 1 ? 1 : a.width > 8 ? 8 : a.width;
-  const long long units = mtiles * ((ntiles + a.width - 1) / a.width);
   // the K range over a cluster of CTAs while the row tiles alone leave SMs idle, at least four 64-element stages each
   const int chunks = (K + 63) / 64;
   int splits = 1;
-  while (splits < 8 && mtiles * splits * 2 <= num_sms() && chunks >= splits * 8) splits *= 2;
+  const int fit = Rp > 64 ? num_sms() * 7 / 8 : 2 * num_sms();   // CTAs of clusters that are resident together, about
+  while (splits < 8 && tiles * splits * 2 <= fit && chunks >= splits * 8) splits *= 2;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)mtiles, splits);
+  cfg.gridDim = dim3((unsigned)w.tiles, splits);
   cfg.blockDim = dim3(192);
-  cfg.dynamicSmemBytes = ShrinkSmem::total(Rp, splits);
+  const long long per_sm = (tiles * splits + num_sms() - 1) / num_sms();
+  a.stages = ShrinkSmem::stages(Rp, splits, per_sm < 2 ? 1 : splits > 1 && Rp > 64 ? 1 : per_sm < 3 || splits > 1 ? 2 : 3);
+  cfg.dynamicSmemBytes = ShrinkSmem::total(Rp, splits, a.stages);
   cfg.stream = S_(stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 1;
-  attr[0].val.clusterDim.y = splits;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1;
+  attr[1].val.clusterDim.y = splits;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = planned ? attr : attr + 1;
+  cfg.numAttrs = planned ? 2 : 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, adapter_shrink_kernel, tx, ta, a);
   if (e != cudaSuccess) return fail(H3_ERR_CUDA, "%s: cluster launch: %s", who, cudaGetErrorString(e));
   if ((rc = check_launch(who))) return rc;
+  const long long units = w.tiles * ((ntiles + a.width - 1) / a.width);
   cfg.gridDim = dim3((unsigned)(units < num_sms() ? units : num_sms()));
-  cfg.blockDim = dim3(320);
+  cfg.blockDim = dim3(448);
   cfg.dynamicSmemBytes = ExpandSmem::total(Rp);
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, adapter_expand_kernel, ty, tt, tb, to, a);
   if (e != cudaSuccess) return fail(H3_ERR_CUDA, "%s: launch: %s", who, cudaGetErrorString(e));
   return check_launch(who);

@@ -224,8 +224,9 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tens
         raise ValueError(f"adapter_add: rows must be int32 [{M}], got {tuple(rows.shape)} {rows.dtype}")
     if scale is not None and (scale.shape != (n,) or scale.dtype != torch.float32):
         raise ValueError(f"adapter_add: scale must be fp32 [{n}], got {tuple(scale.shape)} {scale.dtype}")
-    if K & 7 or cols & 7 or R & 7 or R > 128:
-        raise ValueError(f"adapter_add: K, N and R must be multiples of 8 and R at most 128, got K={K} N={cols} R={R}")
+    if K & 7 or cols & 7 or R & 7 or R > 128 or n > 1 << 20:
+        raise ValueError("adapter_add: K, N and R must be multiples of 8, R at most 128 and n at most 2^20, got "
+                         f"K={K} N={cols} R={R} n={n}")
     for name, t in (("y", y), ("out", out)) if out is not y else (("y", y),):
         ld, cs = t.stride()
         if (cols > 1 and cs != 1) or ld & 7 or (M > 1 and ld < cols) or t.data_ptr() & 15:
@@ -241,9 +242,9 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tens
         scale = scale.contiguous()
         dev = N.one_device("adapter_add", y, x, A, B, rows, out, scale)
     if M and cols and n and K and R:
-        size = N.adapter_workspace_bytes(M, R)
+        size = N.adapter_workspace_bytes(M, R, n)
         ws = x.new_empty(size // 2)
-        N.launch(dev, "h3_adapter_add", 2, x.data_ptr(), ldx, y.data_ptr(), y.stride(0), A.data_ptr(), B.data_ptr(),
+        N.launch(dev, "h3_adapter_add", 2 if n == 1 else 3, x.data_ptr(), ldx, y.data_ptr(), y.stride(0), A.data_ptr(), B.data_ptr(),
                  None if scale is None else scale.data_ptr(), rows.data_ptr(), M, K, cols, R, n, out.data_ptr(),
                  out.stride(0), ws.data_ptr(), size)
     elif out is not y:

@@ -56,7 +56,7 @@ _SIGS = {
     "h3_modulation": [vp, i32, i32, vp, vp, i32, vp, vp],
     "h3_gemm_nvfp4": [vp, vp, vp, vp, vp, f32, vp, i32, i32, i32, C.POINTER(H3Epilogue), vp],
     "h3_qknorm_rope": [vp, vp, i64, i32, i32, i32, vp, vp, vp, f32, vp],
-    "h3_adapter_workspace_bytes": ([i32, i32], sz),
+    "h3_adapter_workspace_bytes": ([i32, i32, i32], sz),
     "h3_adapter_add": [vp, i64, vp, i64, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, i64, vp, sz, vp],
     "h3_rope_axes": [C.POINTER(H3Positions), i32, vp, vp],
     "h3_qknorm_rope_axes": [vp, i64, i64, vp, i64, i64, i32, i32, i32, vp, vp, C.POINTER(H3Positions), f32, vp, i64,
@@ -192,8 +192,8 @@ def attn_bf16_workspace_bytes(S: int, Hk: int) -> int:
 
 
 @lru_cache(maxsize=256)
-def adapter_workspace_bytes(M: int, R: int) -> int:
-    return int(lib().h3_adapter_workspace_bytes(M, R))
+def adapter_workspace_bytes(M: int, R: int, n: int) -> int:
+    return int(lib().h3_adapter_workspace_bytes(M, R, n))
 
 
 def slot_ptr(slots: torch.Tensor, i: int) -> int:

@@ -33,6 +33,8 @@ def make(M, K, N, R, n, seed=0, kind="runs"):
         rows = np.full(M, -1)
     elif kind == "runs":
         rows = np.sort(rs.randint(-1, n, M))
+    elif kind == "back":                            # runs in falling order, and some of an adapter twice
+        rows = np.concatenate([np.sort(rs.randint(-1, n, M - M // 3))[::-1], np.sort(rs.randint(-1, n, M // 3))])
     else:                                           # any order, entries outside [0, n) among them
         rows = rs.choice(np.array(list(range(n)) + [-1, -7, n, 2 ** 31 - 1, -2 ** 31]), M)
     return x, y, A, B, torch.from_numpy(rows.astype(np.int32)).cuda(), scale
@@ -62,6 +64,9 @@ def check(out, x, y, A, B, rows, scale=None):
     (128, 512, 512, 64, 4, "runs"), (129, 520, 264, 128, 3, "any"), (333, 512, 512, 16, 1, "one"), (300, 256, 384, 8, 130, "any"),
     (1000, 1024, 1000, 72, 5, "any"), (640, 2048, 256, 112, 2, "runs"), (500, 128, 200, 40, 3, "none"),
     (4096, 5120, 1280, 64, 4, "runs"), (20000, 512, 384, 32, 7, "any"), (257, 20480, 520, 96, 2, "any"),
+    (2048, 64, 72, 8, 2, "any"), (2049, 64, 72, 8, 2, "any"), (5000, 136, 200, 24, 300, "any"), (4100, 64, 64, 16, 5000, "any"),
+    (16, 5120, 1024, 64, 6, "any"), (130, 512, 512, 16, 1, "any"), (6000, 256, 136, 40, 3, "runs"), (700, 64, 128, 128, 2, "none"),
+    (3000, 200, 264, 16, 3, "back"), (300, 64, 64, 8, 20, "back"), (4500, 72, 136, 16, 9, "back"),
 ])
 def test_adapter_add(M, K, N, R, n, kind):
     from tfvideo import linear as L

@@ -153,12 +153,12 @@ def test_adapter_add_checks_its_arguments(lib):
         return lib.h3_adapter_add(x, ldx, y, ldy, FAKE, FAKE, None, rows, M, K, N, R, n, out, ldo, ws, size, None)
 
     for bad in (dict(x=None), dict(y=None), dict(rows=None), dict(out=None), dict(ws=None), dict(x=FAKE + 2),
-                dict(out=FAKE + 8), dict(rows=FAKE + 1), dict(size=10 * 32 - 1)):
+                dict(out=FAKE + 8), dict(rows=FAKE + 1), dict(size=lib.h3_adapter_workspace_bytes(10, 16, 2) - 1)):
         assert call(**bad) == -1, bad
-    for bad in (dict(M=0), dict(K=0), dict(K=60), dict(N=4), dict(R=0), dict(R=12), dict(R=136), dict(n=0), dict(ldx=56),
+    for bad in (dict(M=0), dict(K=0), dict(K=60), dict(N=4), dict(R=0), dict(R=12), dict(R=136), dict(n=0), dict(n=2 ** 20 + 1), dict(ldx=56),
                 dict(ldx=68), dict(ldy=56), dict(ldo=66)):
         assert call(**bad) == -2, bad
-    assert lib.h3_adapter_workspace_bytes(10, 8) >= 320 and lib.h3_adapter_workspace_bytes(0, 8) == 0
+    assert lib.h3_adapter_workspace_bytes(10, 8, 1) >= 320 and lib.h3_adapter_workspace_bytes(0, 8, 1) == 0
     assert lib.h3_act(FAKE, 16, FAKE, 8, 4, 8, 2, None, None) == -2 and lib.h3_act(FAKE, 16, FAKE, 8, 4, 8, 3, None, None) == -1
 
 
