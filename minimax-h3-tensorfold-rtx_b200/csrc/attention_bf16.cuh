@@ -157,12 +157,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // NaN when eithe
 }
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1u); }
 
-// 2^(s * scale - m) for a pair, m an integer: n = round(s * scale - m) from the low bits of the sum with 1.5 * 2^23,
-// then the degree-3 polynomial of exp2_poly_clamped at the remainder, its exponent raised by n.  For results that are
-// normal numbers.
-__device__ __forceinline__ uint64_t exp2_poly_int(uint64_t s, uint64_t scale2, uint64_t nm_magic2) {
-  const uint64_t t = fma2(s, scale2, nm_magic2);                            // 1.5 * 2^23 + n
-  const uint64_t g = fma2(s, scale2, fma2(t, f32x2_splat(-1.0f), nm_magic2));   // s * scale - m - n
+// 2^x for a pair whose results are normal numbers: exp2_poly_clamped's polynomial, without its clamp, and the exponent
+// raised by an integer addition.
+__device__ __forceinline__ uint64_t exp2_poly_normal(uint64_t x) {
+  constexpr float kMagic = 12582912.0f;                                     // 1.5 * 2^23: the sum's low bits are round(x)
+  const uint64_t t = add2(x, f32x2_splat(kMagic));
+  const uint64_t g = fma2(add2(t, f32x2_splat(-kMagic)), f32x2_splat(-1.0f), x);
   uint64_t p = fma2(f32x2_splat(0.0551716685295105f), g, f32x2_splat(0.2426111400127411f));
   p = fma2(p, g, f32x2_splat(0.6932609677314758f));
   p = fma2(p, g, f32x2_splat(0.9999280571937561f));
@@ -179,12 +179,11 @@ __device__ __forceinline__ uint64_t exp2_poly_int(uint64_t s, uint64_t scale2, u
 template <bool POLY>
 __device__ __forceinline__ void p_chunk_bf16(const uint32_t (&s)[32], uint64_t scale2, float nm, uint32_t (&pw)[16],
                                              uint64_t& l2a, uint64_t& l2b) {
-  const uint64_t nm2 = f32x2_splat(nm), nm_magic2 = f32x2_splat(nm + 12582912.0f);
+  const uint64_t nm2 = f32x2_splat(nm);
 #pragma unroll
   for (int w = 0; w < 16; ++w) {
-    const uint64_t x = f32x2_pack(__uint_as_float(s[2 * w]), __uint_as_float(s[2 * w + 1]));
-    const uint64_t y = POLY && ((kPolyPairsBf16 >> w) & 1u) ? exp2_poly_int(x, scale2, nm_magic2)
-                                                            : exp2_mufu_pair(fma2(x, scale2, nm2));
+    const uint64_t x = fma2(f32x2_pack(__uint_as_float(s[2 * w]), __uint_as_float(s[2 * w + 1])), scale2, nm2);
+    const uint64_t y = POLY && ((kPolyPairsBf16 >> w) & 1u) ? exp2_poly_normal(x) : exp2_mufu_pair(x);
     if (w & 1) l2b = add2(l2b, y);
     else l2a = add2(l2a, y);
     float a, b;
@@ -518,7 +517,7 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
     const float scale = kLog2e * 0.08838834764831845f;   // log2(e) / sqrt(128)
     const uint64_t scale2 = f32x2_splat(scale);
     const bool live = lo < hi;
-    float m_used = -INFINITY;   // an integer once a key was seen
+    float m_used = -INFINITY;   // the row's own largest score, not a rounded one: its P is then exactly 1 in bf16 too
     uint64_t l2a = 0, l2b = 0;
     bool ok = true, bounded = false;
     if (p.knorm && last > first) {
@@ -562,7 +561,7 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
       if (!bounded || __any_sync(~0u, m_used == -INFINITY)) {
         const float mx = fmaxf(fmaxf(max_chunk(s[0], -INFINITY), max_chunk(s[1], -INFINITY)),
                                fmaxf(max_chunk(s[2], -INFINITY), max_chunk(s[3], -INFINITY)));
-        const float mnew = ceilf(mx * scale);
+        const float mnew = mx * scale;
         const bool need = m_used == -INFINITY ? mnew > m_used : mnew > m_used + kTauBf16 && !bounded;
         float alpha = 1.0f;
         if (need) {

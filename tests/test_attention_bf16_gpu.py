@@ -225,6 +225,19 @@ def test_flat_and_peaked_scores(scale):
     check(A.bf16(q, k, v), q, k, v)
 
 
+def test_a_single_key_gives_its_value():
+    """A row that sees one key has that key's value, bit for bit (its P is 1, and so is its sum)."""
+
+    from tfvideo import attention as A
+
+    for S in (1, 300, 2500):
+        q, k, v = packed(S, 2, 2, 50 + S, 2.0)
+        i = torch.arange(S, dtype=torch.int32, device="cuda")
+        assert torch.equal(A.bf16(q, k, v, A.SpanMask(i, i + 1)), v)
+        at = (i * 7) % S
+        assert torch.equal(A.bf16(q, k, v, A.SpanMask(at, at + 1)), v[:, :, at.long()])
+
+
 def test_rising_scores_rescale_every_step():
     """Scores that grow along the keys raise each row's maximum in every step."""
 
