@@ -184,6 +184,14 @@ def bf16_tokens(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Te
     """Low-level form: q [S, Hq, 128], k and v [S, Hk, 128] bf16 views (token and head strides multiples of 8,
     16-byte aligned); out [S, Hq * 128] bf16, row stride a multiple of 8."""
 
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] or k.shape[1] == 0 \
+            or q.shape[1] % k.shape[1] or q.shape[2] != HEAD_DIM or k.shape[2] != HEAD_DIM \
+            or not q.stride(2) == k.stride(2) == v.stride(2) == 1 \
+            or tuple(out.shape) != (q.shape[0], q.shape[1] * HEAD_DIM) or out.stride(1) != 1 \
+            or not q.dtype == k.dtype == v.dtype == out.dtype == torch.bfloat16:
+        raise ValueError(f"bf16 attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, out "
+                         f"{tuple(out.shape)}: bf16 [S, H, {HEAD_DIM}] rows and [S, Hq * {HEAD_DIM}], query heads a "
+                         "multiple of the key heads")
     (S, Hq, _), Hk = q.shape, k.shape[1]
     _bf16_launch(S, Hq, Hk, q, q.stride(), k, k.stride(), v, v.stride(), out, out.stride(0), mask)
     return out

@@ -144,6 +144,12 @@ def test_bf16_attention_refuses_bad_arguments():
                 (q.expand(2, 4, 10, 128), q, q), (q, q, q)):                  # the last: CPU tensors
         with pytest.raises(ValueError):
             A.bf16(*bad)
+    r, out = torch.zeros((10, 4, 128), dtype=torch.bfloat16), torch.zeros((10, 512), dtype=torch.bfloat16)
+    for bad in ((r[0], r, r, out), (r, r[:9], r[:9], out), (r, r, r[:, :2], out), (r, r[:, :3], r[:, :3], out),
+                (r, r, r, out[:, :256]), (r, r, r, out.float()), (r.float(), r, r, out), (r[:, :, :64], r, r, out),
+                (r, r, r, out.t().contiguous().t()), (r, r, r, out, m), (r, r, r, out)):   # the last: CPU tensors
+        with pytest.raises(ValueError):
+            A.bf16_tokens(*bad)
 
 
 def test_adapter_add_checks_its_arguments(lib):
