@@ -269,6 +269,7 @@ __global__ void __launch_bounds__(192)
   constexpr uint32_t ncols = 128;
   if (a.tile) wait_primary();   // the plan
   else if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.next = 0;
+  launch_dependents();   // (the next kernel's blocks wait for this one to end before they read T)
   if (a.tile && blockIdx.x >= *a.total) return;   // (every CTA of the cluster)
   const TileInfo tile = tile_info(a, blockIdx.x);
   if (tile.adapter < 0) return;
@@ -301,9 +302,6 @@ __global__ void __launch_bounds__(192)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const bool skip = !a.tile && *skip_s;   // the same in every CTA of the cluster
-  // (the next kernel's blocks wait for this one to end before they read T; this block has its TMEM already, so none of
-  // theirs can keep it from it)
-  launch_dependents();
 
   if (skip) {
   } else if (warp == 4) {
