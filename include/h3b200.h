@@ -159,8 +159,8 @@ int h3_gemm_nvfp4(const uint8_t* a_codes, const uint8_t* a_sf, const H3ScaleSlot
 
 /* ---------------------------------------------------------------------------------------------- adapters */
 /* Low-rank adapters of several requests beside a shared projection: out_m = y_m + B_a (scale[a] A_a x_m) with
- * a = rows[m], for bf16 x [M, K], y and out [M, N] (row strides ldx, ldy, ldo; out may be y itself, and is otherwise
- * apart from the inputs), A [n, R, K] and B [n, N, R] contiguous (lower ranks padded with zeros), scale fp32 [n] or
+ * a = rows[m], for bf16 x [M, K], y and out [M, N] (row strides ldx, ldy, ldo; out may be y itself or lie apart
+ * from it, and either may be x), A [n, R, K] and B [n, N, R] contiguous (lower ranks padded with zeros), scale fp32 [n] or
  * NULL (1), rows int32 [M] in any order.  A row whose entry is outside [0, n) has no adapter and is copied bit for bit.
  * Sums in 32 bits; scale[a] A_a x_m is rounded to bf16 once.  K, N, R multiples of 8, R <= 128, n <= 2^20; pointers
  * 16-byte aligned.  workspace: h3_adapter_workspace_bytes(M, R, n) bytes, one per call in flight.  The reference merges
@@ -196,7 +196,8 @@ typedef struct H3Positions {
 int h3_rope_axes(const H3Positions* pos, int S, float* out, void* stream);
 /* h3_qknorm_rope straight from positions, with no table: per-head RMSNorm (weights qw, kw [128], 16-byte aligned) and
  * the split-half rotation of the first rot dims in one pass.  q holds Hq heads and k Hk (they may differ); element
- * (s, h, d) at s * ld + h * hs + d.  Outputs are the inputs themselves (in place) or memory apart from them.
+ * (s, h, d) at s * ld + h * hs + d.  Outputs are the inputs themselves (in place) or memory apart from them
+ * (H3_ERR_ARG otherwise).
  * rot % 8 == 0; strides multiples of 4 elements, pointers 8-byte aligned. */
 int h3_qknorm_rope_axes(const void* q, long long ldq, long long hsq, const void* k, long long ldk, long long hsk,
                         int S, int Hq, int Hk, const float* qw, const float* kw, const H3Positions* pos, float eps,
@@ -239,8 +240,8 @@ int h3_attn_fp8_peers(const void* q, const void* k, const void* v, long long ld,
  * or frame-causal tokens behind it and windows are all spans.  A token with an empty span gets zeros.  Keys and values
  * outside a token's span never reach its row, whatever they hold (NaN and infinities included).  Hq query heads share
  * Hk key heads in groups of Hq / Hk.  q, k and v are bf16 views with their own token and head strides (multiples of 8
- * elements, 16-byte aligned), element (t, h, d) at t * ld + h * hs + d; out (t, h, d) at out + t * ldo + h * 128 + d.
- * scores scaled by 1 / sqrt(128).  S <= 262,144.  workspace: h3_attn_bf16_workspace_bytes(S, Hk) bytes, 16-byte aligned
+ * elements, 16-byte aligned), element (t, h, d) at t * ld + h * hs + d; out (t, h, d) at out + t * ldo + h * 128 + d,
+ * apart from the inputs (H3_ERR_ARG otherwise).  Scores are scaled by 1 / sqrt(128).  S <= 262,144.  workspace: h3_attn_bf16_workspace_bytes(S, Hk) bytes, 16-byte aligned
  * (0, and NULL, for short sequences), one per call in flight: the key norms that let long rows of bounded scores skip
  * their running maximum; NULL is always accepted and only slower.  The reference's backends
  * (tfvideo/attention.py:29-54) attend to the whole sequence. */

@@ -37,6 +37,7 @@ struct AdapterArgs {
   int M, K, N, n;
   int Rp;               // rank rounded up to 16
   int inplace;          // expand: out is y
+  int early;            // expand: need not wait for shrink to write rows without an adapter (no rows of x)
   int stages;           // shrink: ring depth
   int* next;            // expand: units handed out beyond each CTA's first
   int width;            // expand: 128-column tiles a unit
@@ -416,6 +417,19 @@ struct ExpandSmem {
   }
 };
 
+// Shrink lets the expand kernel's blocks start before its own hold their TMEM (2 us of a small call).  They cannot take
+// it from them and wait for them at once: no SM has the shared memory for a block of each.
+constexpr bool never_share_an_sm() {
+  for (int rp = 16; rp <= 128; rp += 16)
+    for (int splits = 1; splits <= 2; ++splits)
+      for (int ctas = 1; ctas <= (splits > 1 ? 2 : 3); ++ctas) {
+        const int stages = ShrinkSmem::stages(rp, splits, ctas);
+        if (stages >= 1 && ShrinkSmem::total(rp, splits, stages) + ExpandSmem::total(rp) <= 233472) return false;
+      }
+  return true;
+}
+static_assert(never_share_an_sm(), "a block of each kernel on one SM");
+
 __global__ void __launch_bounds__(448)
     adapter_expand_kernel(const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmT,
                           const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmO,
@@ -487,7 +501,7 @@ __global__ void __launch_bounds__(448)
   if (warp == 8) {
     int ny = 0, nt = 0, nb = 0;   // y, T and B tiles asked for
     bool ok = true, waited = false;
-    if (a.tile) {
+    if (a.tile || !a.early) {
       wait_primary();             // (the plan is older than the kernel before this one)
       waited = true;
     }

@@ -3,6 +3,7 @@
 // builds TMA tensor maps (cuTensorMapEncodeTiled, fetched from the driver at first use) and launches on the
 // caller's stream.  Nothing here allocates device memory.
 #include <cmath>
+#include <cstdlib>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -575,6 +576,35 @@ int h3_qknorm_rope(void* q, void* k, long long ld, int S, int H, int rot, const 
 }
 
 namespace {
+// n x h rows of w bf16 elements, at t * ld + i * hs
+struct Rows {
+  const void* p;
+  long long ld, hs;
+  int n, h, w;
+};
+// Whether two such views may have elements in common; strides that both share tell views of one buffer apart.
+bool meet(const Rows& x, const Rows& y) {
+  long long lo[2], hi[2], in[2];   // elements a view reaches from its base, and without the steps of ld
+  int i = 0;
+  for (const Rows* v : {&x, &y}) {
+    const long long t = (v->n - 1) * v->ld, e = (v->h - 1) * v->hs;
+    lo[i] = (t < 0 ? t : 0) + (e < 0 ? e : 0);
+    hi[i] = (t > 0 ? t : 0) + (e > 0 ? e : 0) + v->w;
+    in[i++] = e < 0 ? -1 : e + v->w;
+  }
+  const long long d =
+      ((long long)reinterpret_cast<uintptr_t>(y.p) - (long long)reinterpret_cast<uintptr_t>(x.p)) / 2;
+  if (d + lo[1] >= hi[0] || lo[0] >= d + hi[1]) return false;
+  auto apart = [&](long long stride, long long wx, long long wy) {
+    if (stride <= 0 || wx < 0 || wy < 0) return false;
+    const long long r = (d % stride + stride) % stride;
+    return wx <= r && wy <= stride - r;
+  };
+  if (x.ld == y.ld && apart(x.ld, in[0], in[1])) return false;
+  return !(x.hs == y.hs && x.hs > 0 && x.ld % x.hs == 0 && y.ld % y.hs == 0 && apart(x.hs, x.w, y.w));
+}
+bool same(const Rows& x, const Rows& y) { return x.p == y.p && x.ld == y.ld && x.hs == y.hs; }
+
 // Checks an H3Positions and lays out each pair's axis and frequency for the kernels.
 int rope_pos(RopePos* r, const H3Positions* p, const char* who) {
   if (!p || !p->pos) return fail(H3_ERR_ARG, "%s: NULL positions", who);
@@ -635,6 +665,14 @@ int h3_qknorm_rope_axes(const void* q, long long ldq, long long hsq, const void*
   if (!aligned(q, 8) || !aligned(k, 8) || !aligned(out_q, 8) || !aligned(out_k, 8) || !aligned(qw, 16) ||
       !aligned(kw, 16))
     return fail(H3_ERR_ARG, "%s: q / k / outputs 8-byte and norm weights 16-byte alignment required", who);
+  if ((S > 1 && (std::llabs(ldoq) < 128 || std::llabs(ldok) < 128)) || (Hq > 1 && std::llabs(hsoq) < 128) ||
+      (Hk > 1 && std::llabs(hsok) < 128))
+    return fail(H3_ERR_SHAPE, "%s: rows of an output overlap", who);
+  const Rows rq{q, ldq, hsq, S, Hq, 128}, rk{k, ldk, hsk, S, Hk, 128}, roq{out_q, ldoq, hsoq, S, Hq, 128},
+      rok{out_k, ldok, hsok, S, Hk, 128};
+  if ((!same(roq, rq) && meet(roq, rq)) || (!same(rok, rk) && meet(rok, rk)) || meet(roq, rk) || meet(rok, rq) ||
+      meet(roq, rok))
+    return fail(H3_ERR_ARG, "%s: an output overlaps an input other than in place, or the other output", who);
   QkNormAxesArgs a{reinterpret_cast<const __nv_bfloat16*>(q), reinterpret_cast<const __nv_bfloat16*>(k),
                    reinterpret_cast<__nv_bfloat16*>(out_q), reinterpret_cast<__nv_bfloat16*>(out_k),
                    ldq, hsq, ldk, hsk, ldoq, hsoq, ldok, hsok, S, Hq, Hk, qw, kw, eps};
@@ -799,6 +837,10 @@ int h3_attn_bf16(const void* q, long long ldq, long long hsq, const void* k, lon
   if (workspace && (!aligned(workspace, 16) || workspace_bytes < h3_attn_bf16_workspace_bytes(S, Hk)))
     return fail(H3_ERR_ARG, "%s: workspace misaligned, or %zu bytes < %zu", who, workspace_bytes,
                 h3_attn_bf16_workspace_bytes(S, Hk));
+  const Rows ro{out, ldo, 128, S, Hq, 128};
+  if (meet(ro, {q, ldq, hsq, S, Hq, 128}) || meet(ro, {k, ldk, hsk, S, Hk, 128}) ||
+      meet(ro, {v, ldv, hsv, S, Hk, 128}))
+    return fail(H3_ERR_ARG, "%s: the output overlaps an input", who);
   CUtensorMap tq, tk, tv, to;
   int rc;
   if ((rc = make_map_bf16(&tq, q, 128, S, Hq, ldq, hsq, 128, who))) return rc;
@@ -880,6 +922,8 @@ int h3_adapter_add(const void* x, long long ldx, const void* y, long long ldy, c
   if (!aligned(x, 16) || !aligned(y, 16) || !aligned(A, 16) || !aligned(B, 16) || !aligned(out, 16) ||
       !aligned(workspace, 16) || !aligned(rows, 4) || !aligned(scale, 4))
     return fail(H3_ERR_ARG, "%s: x / y / A / B / out / workspace 16-byte alignment required", who);
+  const Rows rx{x, ldx, 0, M, 1, K}, ry{y, ldy, 0, M, 1, N}, ro{out, ldo, 0, M, 1, N};
+  if (!same(ro, ry) && meet(ro, ry)) return fail(H3_ERR_ARG, "%s: out overlaps y other than in place", who);
   const AdapterWs w = adapter_ws(M, R, n);
   if (workspace_bytes < w.total)
     return fail(H3_ERR_ARG, "%s: workspace %zu bytes < %zu", who, workspace_bytes, w.total);
@@ -914,7 +958,8 @@ int h3_adapter_add(const void* x, long long ldx, const void* y, long long ldy, c
   a.N = N;
   a.n = n;
   a.Rp = Rp;
-  a.inplace = out == y && ldo == ldy;
+  a.inplace = same(ro, ry);
+  a.early = a.inplace || !meet(ro, rx);
   a.next = counters + 1;
   if (planned) {
     int4* tile = reinterpret_cast<int4*>(ws + w.tile);

@@ -207,8 +207,8 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tens
                 scale: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """y[m] + B[a] (scale[a] A[a] x[m]) with a = rows[m], for bf16 x [M, K], y [M, N], A [n, R, K], B [n, N, R] (lower
     ranks padded with zeros), scale fp32 [n] (None: 1) and rows int32 [M], in any order; a row whose entry is outside
-    [0, n) has no adapter and keeps y's bits.  In place on y, unless ``out`` names other memory (apart from the
-    inputs).  K, N and R multiples of 8, R <= 128."""
+    [0, n) has no adapter and keeps y's bits.  In place on y, unless ``out`` names other memory (apart from
+    y); either may be x itself.  K, N and R multiples of 8, R <= 128."""
 
     out = y if out is None else out
     bf16 = torch.bfloat16
@@ -244,9 +244,9 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tens
     if M and cols and n and K and R:
         size = N.adapter_workspace_bytes(M, R, n)
         ws = x.new_empty(size // 2)
-        N.launch(dev, "h3_adapter_add", 2 if n == 1 else 3, x.data_ptr(), ldx, y.data_ptr(), y.stride(0), A.data_ptr(), B.data_ptr(),
-                 None if scale is None else scale.data_ptr(), rows.data_ptr(), M, K, cols, R, n, out.data_ptr(),
-                 out.stride(0), ws.data_ptr(), size)
+        N.launch(dev, "h3_adapter_add", 2 if n == 1 else 3, x.data_ptr(), ldx, y.data_ptr(), y.stride(0), A.data_ptr(),
+                 B.data_ptr(), None if scale is None else scale.data_ptr(), rows.data_ptr(), M, K, cols, R, n,
+                 out.data_ptr(), out.stride(0), ws.data_ptr(), size)
     elif out is not y:
         out.copy_(y)
     return out

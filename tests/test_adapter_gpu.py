@@ -144,6 +144,28 @@ def test_strides_views_and_offsets_past_32_bits():
     device_ok()
 
 
+@pytest.mark.parametrize("n", [1, 3])
+@pytest.mark.parametrize("kind", ["runs", "none", "any"])
+def test_out_and_y_may_be_x(n, kind):
+    """A square projection's input overwritten, by a call of its own memory or as y: every row's A x comes first."""
+
+    from tfvideo import linear as L
+
+    x, y, A, B, rows, scale = make(20_000, 1024, 1024, 16, n, seed=n, kind=kind)
+    ref = L.adapter_add(y, x, A, B, rows, scale, out=torch.empty_like(y))
+    over = x.clone()
+    assert L.adapter_add(y, over, A, B, rows, scale, out=over) is over and torch.equal(over, ref)
+    ref = L.adapter_add(x, x, A, B, rows, scale, out=torch.empty_like(y))
+    check(ref, x, x, A, B, rows, scale)
+    assert torch.equal(L.adapter_add(x, x, A, B, rows, scale), ref)
+    both = torch.empty((400, 2048), dtype=torch.bfloat16, device="cuda")     # y and out side by side in one buffer
+    both[:, :1024] = y[:400]
+    L.adapter_add(both[:, :1024], y[:400], A, B, rows[:400], scale, out=both[:, 1024:])
+    assert torch.equal(both[:, :1024], y[:400])
+    check(both[:, 1024:], y[:400], y[:400], A, B, rows[:400], scale)
+    device_ok()
+
+
 def test_sets_of_mixed_ranks_and_interleaved_outputs():
     from tfvideo import linear as L
 

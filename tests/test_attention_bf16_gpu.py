@@ -158,6 +158,12 @@ def test_layouts():
     out = torch.full((S, H * 128 + 64), 7.0, dtype=torch.bfloat16, device="cuda")
     A.bf16_tokens(q[0].transpose(0, 1), k[0].transpose(0, 1), v[0].transpose(0, 1), out[:, :H * 128])
     assert torch.equal(out[:, :H * 128].view(S, H, 128).transpose(0, 1)[None], ref) and (out[:, H * 128:] == 7).all()
+    rows = torch.cat([t[0].transpose(0, 1).reshape(S, H * 128) for t in (q, k, v, v)], 1)    # out beside q, k, v
+    h = rows.view(S, 4 * H, 128)
+    A.bf16_tokens(h[:, :H], h[:, H:2 * H], h[:, 2 * H:3 * H], rows[:, 3 * H * 128:])
+    assert torch.equal(h[:, 3 * H:].transpose(0, 1)[None], ref) and torch.equal(h[:, :H].transpose(0, 1)[None], q)
+    with pytest.raises(RuntimeError, match="overlap"):
+        A.bf16_tokens(h[:, :H], h[:, H:2 * H], h[:, 2 * H:3 * H], rows[:, :H * 128])
     assert A.bf16(q[:, :, :0], k[:, :, :0], v[:, :, :0]).shape == (1, H, 0, 128)
     device_ok()
 

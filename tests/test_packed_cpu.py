@@ -64,6 +64,38 @@ def test_rope_entry_points_check_their_arguments(lib):
     assert qk(pos=ctypes.byref(_pos(dims=(44, 42, 40)))) == -2 and "multiple of 8" in N.last_error()   # rot 126
 
 
+def test_outputs_over_other_memory_are_refused(lib):
+    from tfvideo import native as N
+
+    p, e = ctypes.byref(_pos()), 2   # bytes an element
+    far = FAKE + (1 << 24)
+
+    def qk(q=(FAKE, 768, 128), k=(FAKE + 256 * e, 768, 128), oq=(far, 256, 128), ok=(far + (1 << 20), 256, 128), H=2):
+        return lib.h3_qknorm_rope_axes(*q, *k, 10, H, H, FAKE, FAKE, p, 1e-5, *oq, *ok, None)
+
+    q, k = (FAKE, 768, 128), (FAKE + 256 * e, 768, 128)
+    for oq, ok in ((k, q), (k, k), (q, q), ((FAKE + 8, 768, 128), k), (q, (far, 0, 128)), (q, (far, 256, 0)),
+                   ((FAKE, 256, 128), k), (q, (FAKE + 128 * e, 768, 128)), ((FAKE - 256, 768, 128), k),
+                   ((far, 256, 128), (far + 128 * e, 256, 128))):
+        assert qk(oq=oq, ok=ok) in (-1, -2) and "overlap" in N.last_error(), (oq, ok)
+    q3, k3 = (FAKE, 768, 384), (FAKE + 128 * e, 768, 384)         # q, k and v of a head side by side
+    assert qk(q3, k3, q3, (FAKE + 192 * e, 768, 384)) == -1 and "overlap" in N.last_error()
+
+    def attn(out, ldo):
+        return lib.h3_attn_bf16(FAKE, 1024, 128, FAKE + 256 * e, 1024, 128, FAKE + 512 * e, 1024, 128, 10, 2, 2, None,
+                                None, out, ldo, None, 0, None)
+
+    for at, ldo in ((0, 1024), (256, 1024), (512, 1024), (640, 1024), (0, 256), (896, 1024), (9000, 256)):
+        assert attn(FAKE + at * e, ldo) == -1 and "overlap" in N.last_error(), (at, ldo)
+
+    def add(out, ldo, y=FAKE, ldy=512):
+        return lib.h3_adapter_add(far, 64, y, ldy, far, far, None, far, 10, 64, 256, 16, 2, out, ldo, far,
+                                  lib.h3_adapter_workspace_bytes(10, 16, 2), None)
+
+    for at, ldo in ((0, 256), (8, 512), (248, 512), (4096, 512), (4608, 264)):
+        assert add(FAKE + at * e, ldo) == -1 and "overlap" in N.last_error(), (at, ldo)
+
+
 def test_rope_functions_refuse_bad_arguments():
     from tfvideo import kernels as K
 

@@ -143,6 +143,31 @@ def test_qknorm_rope_axes_equals_the_table_path():
         assert (d <= 2.0 ** -7 * y.float().abs() + 1e-6).all()
 
 
+def test_parts_of_one_buffer():
+    """q, k and v of a head side by side: in place, and into the memory of the third part; [q | k | out] rows."""
+
+    from tfvideo import kernels as K
+
+    S, H, dims = 45, 5, (32, 32, 32)
+    x = to_dev(bf16_array((S, H, 3, 128), seed=6))
+    pos = torch.from_numpy(grid_positions(S, 3, 0, "grid")).cuda()
+    w = 1 + 0.1 * torch.randn(128, device="cuda")
+    q, k, v = (x[:, :, i].clone() for i in range(3))
+    oq, ok = K.qknorm_rope_axes(q, k, w, w, pos, dims, out_q=torch.empty_like(q), out_k=torch.empty_like(k))
+    y = x.clone()
+    K.qknorm_rope_axes(y[:, :, 0], y[:, :, 1], w, w, pos, dims)
+    assert torch.equal(y, torch.stack([oq, ok, v], 2))
+    y = x.clone()
+    K.qknorm_rope_axes(y[:, :, 0], y[:, :, 1], w, w, pos, dims, out_q=y[:, :, 2])
+    assert torch.equal(y, torch.stack([q, ok, oq], 2))
+    y = torch.cat([q, k, v], 1)
+    K.qknorm_rope_axes(y[:, :H], y[:, H:2 * H], w, w, pos, dims, out_q=y[:, 2 * H:])
+    assert torch.equal(y, torch.cat([q, ok, oq], 1))
+    with pytest.raises(RuntimeError, match="overlap"):
+        K.qknorm_rope_axes(y[:, :H], y[:, H:2 * H], w, w, pos, dims, out_q=y[:, 1:H + 1])
+    assert torch.equal(y, torch.cat([q, ok, oq], 1))
+
+
 def test_head_major_strides_zero_rows_and_non_finite_rows():
     """[H, S, 128] memory; a zero row stays zero (eps under the root); inf and NaN stay in their own head rows."""
 
