@@ -58,10 +58,6 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {   // addr: clus
                : "r"(addr));
   return v;
 }
-// Programmatic dependent launch: the next kernel of the stream may start its blocks once every block of this one got
-// here, and waits in wait_primary for this one's end (memory included) before it touches what this one wrote.
-__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ------------------------------------------------------------------------------------------------ plan
 // One block takes 2,048 rows, cuts each run of one adapter every 128 rows, and appends the tiles to the list.  Rows in

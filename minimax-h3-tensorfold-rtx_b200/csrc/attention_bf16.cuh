@@ -119,27 +119,39 @@ struct AttnBf16Args {
   const int* lo;             // spans, or NULL: every key
   const int* hi;
   const float* knorm;        // [key heads][S / 128 tiles]: largest |k|^2 of each 128 keys, or NULL
-  const int4* order;         // [S / 256 tiles]: query tiles by falling number of key steps, or NULL; x: tile, y and z:
-                             // first and end key of its rows
+  const int* order;          // [S / 256 tiles]: query tiles by falling number of key steps, or NULL
   int S, group;              // group: query heads that share a key head
-  int rows;                  // query rows a CTA: 256, or 128 (tile B unused) when that many CTAs still fit at once
-  int tiles, heads;          // CTAs: query tiles of that many rows x query heads
-  int tile_major;            // CTAs in order of tiles (every head of one, then the next), else of heads
+  int* next;                 // units handed out beyond each CTA's first, or NULL: a CTA for every unit
+  int rows;                  // query rows a unit: 256, or 128 (tile B unused) when that many CTAs still fit at once
+  int tiles, heads;          // units: query tiles of that many rows x query heads
+  int tile_major;            // units in order of tiles (every head of one, then the next), else of heads
+};
+
+// What one CTA works on at a time: two query tiles of one head.  Step j covers keys base + 128 j ..; tile t takes part
+// in steps [j0[t], j1[t]).
+struct AttnBf16Unit {
+  int q0;                        // first query row; -1: no more units
+  int h, base, steps;
+  int j0[2], j1[2];
+  int lo_max[2], hi_min[2];      // over the tile's rows that have keys
+  float kk;                      // largest |k|^2 of the unit's keys
 };
 
 struct AttnBf16Smem {
   static constexpr int SUB = 128 * 128;            // 128 rows x 64 dims of bf16 (128-byte rows, 128-byte swizzle)
   static constexpr int TILE = 2 * SUB;             // 128 rows x 128 dims
-  static constexpr int KST = 2, VST = 3;           // ring depths
+  static constexpr int KST = 2, VST = 2;           // ring depths (a third V tile measured the same)
+  static constexpr int STAGE = 32 * 128;           // output on its way: 32 rows x 64 dims a softmax warp
   static constexpr int Q_OFF = 0;                  // tiles A, B
   static constexpr int K_OFF = 2 * TILE;
   static constexpr int V_OFF = K_OFF + KST * TILE;
-  static constexpr int BAR_OFF = V_OFF + VST * TILE;
+  static constexpr int STAGE_OFF = V_OFF + VST * TILE;
+  static constexpr int BAR_OFF = STAGE_OFF + 8 * STAGE;
   static constexpr int MAX_S = 262144;
   static constexpr int BAD_WORDS = MAX_S / 128 / 32 + 1;   // a bit per step whose V tile held masked non-finite values
-  static constexpr int BAD_OFF = BAR_OFF + 256;
-  static constexpr int RED_OFF = BAD_OFF + (BAD_WORDS + 3) / 4 * 16;   // span reductions: 8 warps x 4 ints
-  static constexpr int TOTAL = RED_OFF + 128 + 16 + 1024;
+  static constexpr int BAD_OFF = BAR_OFF + 256;            // of two units
+  static constexpr int UNIT_OFF = BAD_OFF + (2 * BAD_WORDS + 3) / 4 * 16;
+  static constexpr int TOTAL = UNIT_OFF + 2 * (int)sizeof(AttnBf16Unit) + 16 + 1024;
 };
 static_assert(AttnBf16Smem::TOTAL <= 232448, "shared memory of one SM");
 
@@ -205,12 +217,15 @@ struct AttnBf16Prep {
   const int *lo, *hi;
   float* knorm;
   int2* range;         // [S / 128 tiles]: first and end key of the tile's rows
-  int4* order;
+  int* order;
+  int* next;           // to zero
 };
 __global__ void __launch_bounds__(256) attn_bf16_prep_kernel(const AttnBf16Prep a) {
   __shared__ float red[16];
   __shared__ int2 rr[4];
   const int part = threadIdx.x & 15, row0 = threadIdx.x >> 4;
+  launch_dependents();
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.next = 0;
   uint4 u[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -249,16 +264,17 @@ __global__ void __launch_bounds__(256) attn_bf16_prep_kernel(const AttnBf16Prep 
                                       max(max(rr[0].y, rr[1].y), max(rr[2].y, rr[3].y)));
   }
 }
-// The 256-row query tiles (at most 1,024) by falling number of key steps: the longest CTAs start first, so that the
+// The 256-row query tiles (at most 1,024) by falling number of key steps: the longest units start first, so that the
 // last ones to start are short.  One block; each thread ranks its tile against all.
 __global__ void __launch_bounds__(1024) attn_bf16_order_kernel(const AttnBf16Prep a, int tiles) {
   __shared__ int w[1024];
   const int t = threadIdx.x, n128 = (a.S + 127) >> 7;
-  int mine = 0, lo = 0, hi = 0;
+  launch_dependents();
+  wait_primary();
+  int mine = 0;
   if (t < tiles) {
     const int2 x = a.range[2 * t], y = 2 * t + 1 < n128 ? a.range[2 * t + 1] : make_int2(INT_MAX, 0);
-    lo = min(x.x, y.x);
-    hi = max(x.y, y.y);
+    const int lo = min(x.x, y.x), hi = max(x.y, y.y);
     mine = hi > lo ? (hi - lo + 127) >> 7 : 0;
   }
   w[t] = mine;
@@ -266,7 +282,7 @@ __global__ void __launch_bounds__(1024) attn_bf16_order_kernel(const AttnBf16Pre
   if (t >= tiles) return;
   int rank = 0;
   for (int i = 0; i < tiles; ++i) rank += w[i] > mine || (w[i] == mine && i < t);
-  a.order[rank] = make_int4(t, lo, hi, 0);
+  a.order[rank] = t;
 }
 
 __global__ void __launch_bounds__(kAttnBf16Threads, 1)
@@ -278,42 +294,105 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
   uint64_t* q_full = bars;
-  uint64_t* k_full = bars + 1;             // [KST]
+  uint64_t* q_empty = bars + 1;            // both tiles' S issued for good, and every softmax warp past its look at Q
+  uint64_t* k_full = q_empty + 1;          // [KST]
   uint64_t* k_empty = k_full + L::KST;
   uint64_t* v_full = k_empty + L::KST;     // [VST]
   uint64_t* v_ok = v_full + L::VST;        // [VST]: landed, and its masked non-finite values are zero
   uint64_t* v_empty = v_ok + L::VST;
   uint64_t* s_full = v_empty + L::VST;     // [tile]
   uint64_t* p_full = s_full + 2;           // [tile][half]: P of keys 0-63 / 64-127 written, by four warps
-  uint64_t* o_done = p_full + 4;           // [tile]
-  uint64_t* turn = o_done + 2;             // [tile]: the other tile's MMAs of this round are issued
-  uint64_t* drained = turn + 2;
-  uint32_t* bad = reinterpret_cast<uint32_t*>(smem + L::BAD_OFF);
-  int* red = reinterpret_cast<int*>(smem + L::RED_OFF);      // [warp][lo min, lo max, hi min, hi max]
-  int* any_bad = red + 32;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(red + 33);
+  uint64_t* o_done = p_full + 4;           // [tile]: the unit's last PV
+  uint64_t* o_free = o_done + 2;           // [tile]: O is in registers
+  uint64_t* turn = o_free + 2;             // [tile]: the other tile's MMAs of this round are issued
+  uint64_t* guard_done = turn + 2;         // [unit]: the V guard has seen all of it
+  uint64_t* unit_full = guard_done + 2;    // [unit]
+  uint64_t* unit_empty = unit_full + 2;
+  uint64_t* drained = unit_empty + 2;
+  uint32_t* bad = reinterpret_cast<uint32_t*>(smem + L::BAD_OFF);            // [unit][BAD_WORDS]
+  AttnBf16Unit* units = reinterpret_cast<AttnBf16Unit*>(smem + L::UNIT_OFF);   // [2]
+  int* any_bad = reinterpret_cast<int*>(units + 2);                          // [unit]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(any_bad + 2);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // the order of CTAs: long ones first where they are known, else the last tiles, which see most under causal spans
-  const int h = p.tile_major ? blockIdx.x % p.heads : blockIdx.x / p.tiles, hk = h / p.group;
-  const int rank = p.tile_major ? blockIdx.x / p.heads : blockIdx.x % p.tiles;
-  const int4 known = p.order ? p.order[rank] : make_int4(p.tiles - 1 - rank, 0, p.lo ? 0 : p.S, 0);
-  const int q0 = known.x * p.rows, q_end = min(q0 + p.rows, p.S);
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   auto load = [&](int off, const CUtensorMap* map, int row, int head, uint64_t* bar) {
     mbar_arrive_expect_tx(bar, L::TILE);
     tma_load_3d(smem + off, map, 0, row, head, bar);
     tma_load_3d(smem + off + L::SUB, map, 64, row, head, bar);
   };
-  auto load_k = [&](int j, int row) {
-    load(L::K_OFF + j % L::KST * L::TILE, &tmK, row + 128 * j, hk, &k_full[j % L::KST]);
+  // (TMA warp) K and V tiles asked for, over all units
+  int nk = 0, nv = 0;
+  auto load_k = [&](int row, int h) {
+    load(L::K_OFF + nk % L::KST * L::TILE, &tmK, row, h / p.group, &k_full[nk % L::KST]);
+    ++nk;
   };
-  auto load_v = [&](int j, int row) {
-    load(L::V_OFF + j % L::VST * L::TILE, &tmV, row + 128 * j, hk, &v_full[j % L::VST]);
+  auto load_v = [&](int row, int h) {
+    load(L::V_OFF + nv % L::VST * L::TILE, &tmV, row, h / p.group, &v_full[nv % L::VST]);
+    ++nv;
   };
-  int nk = 0, nv = 0;   // (TMA warp) K and V tiles asked for
-  if (warp == 8) {      // Q, and K and V where their range is known, are on their way before the rest is set up
+  auto load_q = [&](const AttnBf16Unit& u) {
+    load(L::Q_OFF, &tmQ, u.q0, u.h, q_full);
+    load(L::Q_OFF + L::TILE, &tmQ, u.q0 + 128, u.h, q_full);   // (zeros past the sequence; unused at 128 rows)
+  };
+  // Unit n of the list: long ones first where they are known, else the last tiles, which see most under causal spans.
+  auto place = [&](AttnBf16Unit& u, int n) {
+    u.h = p.tile_major ? n % p.heads : n / p.tiles;
+    const int rank = p.tile_major ? n / p.heads : n % p.tiles;
+    u.q0 = uniform(p.order ? p.order[rank] : p.tiles - 1 - rank) * p.rows;
+  };
+  auto describe = [&](AttnBf16Unit& u) {
+    const int q_end = min(u.q0 + p.rows, p.S);
+    int lo[8], hi[8];   // of rows lane, 32 + lane ..
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int query = u.q0 + 32 * i + lane;
+      lo[i] = hi[i] = 0;
+      if (query < q_end) {
+        lo[i] = p.lo ? p.lo[query] : 0;
+        hi[i] = p.hi ? p.hi[query] : p.S;
+      }
+    }
+    u.base = INT_MAX;
+    int lo_min[2], hi_max[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      int v[4] = {INT_MAX, -1, INT_MAX, -1};
+#pragma unroll
+      for (int i = 4 * t; i < 4 * t + 4; ++i) {
+        const int a = max(lo[i], 0), b = min(hi[i], p.S);
+        if (a < b) {
+          v[0] = min(v[0], a);
+          v[1] = max(v[1], a);
+          v[2] = min(v[2], b);
+          v[3] = max(v[3], b);
+        }
+      }
+      lo_min[t] = __reduce_min_sync(~0u, v[0]);
+      u.lo_max[t] = __reduce_max_sync(~0u, v[1]);
+      u.hi_min[t] = __reduce_min_sync(~0u, v[2]);
+      hi_max[t] = __reduce_max_sync(~0u, v[3]);
+      u.base = min(u.base, lo_min[t]);
+    }
+    const int kend = max(hi_max[0], hi_max[1]);
+    u.steps = kend > 0 ? (kend - u.base + 127) >> 7 : 0;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      u.j0[t] = hi_max[t] > 0 ? (lo_min[t] - u.base) >> 7 : 0;
+      u.j1[t] = hi_max[t] > 0 ? (hi_max[t] - u.base + 127) >> 7 : 0;
+    }
+    u.kk = 0.f;
+    if (p.knorm && u.steps > 0) {
+      const float* kn = p.knorm + (size_t)(u.h / p.group) * ((p.S + 127) >> 7);
+      for (int i = (u.base >> 7) + lane; i <= (kend - 1) >> 7; i += 32) u.kk = max_nan(u.kk, kn[i]);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) u.kk = max_nan(u.kk, __shfl_xor_sync(~0u, u.kk, o));
+    }
+  };
+  AttnBf16Unit first_unit;   // (TMA warp)
+  if (warp == 8) {      // the first unit's loads are on their way before the rest is set up
     if (lane == 0) {
       mbar_init(q_full, 2);
+      mbar_init(q_empty, 10);
       for (int s = 0; s < L::KST; ++s) {
         mbar_init(&k_full[s], 1);
         mbar_init(&k_empty[s], 2);   // a commit of each MMA warp
@@ -323,45 +402,35 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
         mbar_init(&v_ok[s], 1);
         mbar_init(&v_empty[s], 2);
       }
+      mbar_init(&unit_full[0], 1);
+      mbar_init(&unit_full[1], 1);
       fence_barrier_init();
     }
     __syncwarp();
-    load(L::Q_OFF, &tmQ, q0, h, q_full);
-    load(L::Q_OFF + L::TILE, &tmQ, q0 + 128, h, q_full);   // (zeros past the sequence; unused at 128 rows)
-    const int sure = known.z > known.y ? (known.z - known.y + 127) >> 7 : 0;
-    for (; nv < min(sure, L::VST); ++nv) {
-      if (nk < L::KST) load_k(nk++, known.y);
-      load_v(nv, known.y);
+    wait_primary();   // the preparation's results
+    place(first_unit, blockIdx.x);
+    load_q(first_unit);
+    describe(first_unit);
+    for (int j = 0; j < min(first_unit.steps, 2); ++j) {
+      load_k(first_unit.base + 128 * j, first_unit.h);
+      load_v(first_unit.base + 128 * j, first_unit.h);
     }
-  }
-
-  // ---- this thread's span (softmax warps: a thread per query row) and the spans' ranges over each query tile
-  int lo = 0, hi = 0;
-  if (warp < 8) {
-    const int query = q0 + threadIdx.x;
-    if (query < q_end) {
-      lo = p.lo ? max(p.lo[query], 0) : 0;
-      hi = p.hi ? min(p.hi[query], p.S) : p.S;
-    }
-    const bool live = lo < hi;
-    const int a = __reduce_min_sync(~0u, live ? lo : INT_MAX), b = __reduce_max_sync(~0u, live ? lo : -1);
-    const int c = __reduce_min_sync(~0u, live ? hi : INT_MAX), d = __reduce_max_sync(~0u, live ? hi : -1);
     if (lane == 0) {
-      red[warp * 4] = a;
-      red[warp * 4 + 1] = b;
-      red[warp * 4 + 2] = c;
-      red[warp * 4 + 3] = d;
+      units[0] = first_unit;
+      mbar_arrive(&unit_full[0]);
     }
   }
-  for (int i = threadIdx.x; i < L::BAD_WORDS; i += kAttnBf16Threads) bad[i] = 0;
+  static_assert(L::KST == 2 && L::VST == 2, "first loads");
   if (threadIdx.x == 0) {
-    *any_bad = 0;
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
       mbar_init(&p_full[2 * t], 4);
       mbar_init(&p_full[2 * t + 1], 4);
       mbar_init(&o_done[t], 1);
+      mbar_init(&o_free[t], 4);
       mbar_init(&turn[t], 1);
+      mbar_init(&guard_done[t], 1);
+      mbar_init(&unit_empty[t], 11);   // MMA, guard and softmax warps
     }
     mbar_init(drained, 2);
     fence_barrier_init();
@@ -373,299 +442,393 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform(*tmem_slot);
 
-  int lo_min[2], lo_max[2], hi_min[2], hi_max[2];
+  if (warp >= 8) {
+    // The softmax warps hold a row's scores: 8 x 32 x 208 registers + 4 x 32 x 88 are the 384 x 168 of the launch.
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 8) {
+      // ---------------------------------------------------------------- TMA
+      AttnBf16Unit u = first_unit;
+      const int all = p.tiles * p.heads;
+      bool ok = true;
+      int nq = 1;   // Q tiles asked for
+      for (int it = 0; ok; ++it) {
+        if (it > 0) {
+          if (!(ok = __all_sync(~0u, mbar_wait(&unit_empty[it & 1], ((it >> 1) & 1) ^ 1, 300)))) break;
+          if (lane == 0) {
+            units[it & 1] = u;
+            mbar_arrive(&unit_full[it & 1]);
+          }
+          __syncwarp();
+          if (u.q0 < 0) break;
+        }
+        const int k0 = nk - (it ? 0 : min(u.steps, 2));   // tiles of earlier units
+        int n = all;
+        for (int j = 0; ok && j < max(u.steps, 1); ++j) {
+          if (j < u.steps && k0 + j >= nk) {
+            if (!(ok = __all_sync(~0u, mbar_wait(&k_empty[nk % L::KST], ((nk / L::KST) & 1) ^ 1, 301)))) break;
+            load_k(u.base + 128 * j, u.h);
+          }
+          if (it > 0 && j == 0) {
+            if (!(ok = __all_sync(~0u, mbar_wait(q_empty, (nq - 1) & 1, 304)))) break;
+            load_q(u);
+            ++nq;
+          }
+          // (asked for here, needed behind the loop; earlier would hand units to busy CTAs)
+          if (p.next && j == max(u.steps - 3, 0) && lane == 0) n = gridDim.x + atomicAdd(p.next, 1);
+          if (j < u.steps && k0 + j >= nv) {
+            if (!(ok = __all_sync(~0u, mbar_wait(&v_empty[nv % L::VST], ((nv / L::VST) & 1) ^ 1, 302)))) break;
+            load_v(u.base + 128 * j, u.h);
+          }
+        }
+        n = uniform(lane == 0 ? n : 0);
+        u.q0 = -1;
+        if (n < all) {
+          place(u, n);
+          describe(u);
+        }
+      }
+      // nothing may still be landing in this CTA's memory when it ends, after a wait that gave up included
+      mbar_drain(q_full, (nq - 1) & 1, 303);
+      for (int j = max(nk - L::KST, 0); j < nk; ++j) mbar_drain(&k_full[j % L::KST], (j / L::KST) & 1, 303);
+      for (int j = max(nv - L::VST, 0); j < nv; ++j) mbar_drain(&v_full[j % L::VST], (j / L::VST) & 1, 303);
+    } else if (warp < 11) {
+      // ---------------------------------------------------------------- MMA of one tile
+      constexpr uint32_t idesc_s = idesc_bf16(128, 128, false), idesc_o = idesc_bf16(128, 128, true);
+      const int t = warp - 9;
+      const uint32_t s_tm = tmem + t * 128, o_tm = tmem + 256 + t * 128;
+      // descriptors of the first tiles; others differ by 16-byte units in the low bits.  V rows are keys (the K
+      // dimension), 64 dims contiguous: MN-major, 8-key groups 1,024 bytes apart, the two 64-dim halves SUB apart
+      const uint64_t qd = sdesc_kmajor_sw128(smem_u32(smem + L::Q_OFF + t * L::TILE));
+      const uint64_t kd0 = sdesc_kmajor_sw128(smem_u32(smem + L::K_OFF));
+      const uint64_t vd0 = make_sdesc(smem_u32(smem + L::V_OFF), L::SUB, 1024, kLayoutSW128);
+      auto issue_s = [&](int slot) {   // S = Q K^T: 8 MMAs over 16 dims each
+        const uint64_t kd = kd0 + slot * (L::TILE >> 4);
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    lo_min[t] = hi_min[t] = INT_MAX;
-    lo_max[t] = hi_max[t] = -1;
-    for (int w = 4 * t; w < 4 * t + 4; ++w) {
-      lo_min[t] = min(lo_min[t], red[4 * w]);
-      lo_max[t] = max(lo_max[t], red[4 * w + 1]);
-      hi_min[t] = min(hi_min[t], red[4 * w + 2]);
-      hi_max[t] = max(hi_max[t], red[4 * w + 3]);
-    }
-  }
-  // key steps: step j covers keys base + 128 j ..; tile t takes part in steps [j0[t], j1[t])
-  const int base = min(lo_min[0], lo_min[1]);
-  const int kend = max(hi_max[0], hi_max[1]);
-  const int steps = kend > 0 ? (kend - base + 127) >> 7 : 0;
-  int j0[2], j1[2];
+        for (int kk = 0; kk < 8; ++kk) {
+          const uint32_t off = ((kk >> 2) * L::SUB + (kk & 3) * 32) >> 4;
+          mma_bf16_ss(s_tm, qd + off, kd + off, idesc_s, kk != 0);
+        }
+      };
+      auto issue_pv = [&](int slot, int half, bool add) {   // O (+)= P V over 64 keys: 4 MMAs over 16 keys each
+        const uint64_t vd = vd0 + slot * (L::TILE >> 4);
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    j0[t] = hi_max[t] > 0 ? (lo_min[t] - base) >> 7 : 0;
-    j1[t] = hi_max[t] > 0 ? (hi_max[t] - base + 127) >> 7 : 0;
-  }
-  // whether step j hides a key from some live row of tile t
-  auto hides = [&](int t, int j) {
-    const int kb = base + 128 * j;
-    return lo_max[t] > kb || hi_min[t] < kb + 128;
-  };
-
-  if (warp == 8) {
-    // ------------------------------------------------------------------ TMA
-    for (int j = 0; j < steps; ++j) {
-      if (j >= nk) {
-        if (!__all_sync(~0u, mbar_wait(&k_empty[j % L::KST], ((j / L::KST) & 1) ^ 1, 301))) break;
-        load_k(nk++, base);
+        for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+          mma_bf16_ts(o_tm, s_tm + kk * 8, vd + kk * (2048 >> 4), idesc_o, add || kk != 0);
+      };
+      bool ok = true;
+      int g0 = 0, r0 = 0, np = 0, no = 0;   // steps and rounds, this tile's P and O of earlier units
+      for (int it = 0; ok; ++it) {
+        if (!(ok = __all_sync(~0u, mbar_wait(&unit_full[it & 1], (it >> 1) & 1, 309)))) break;
+        const AttnBf16Unit& u = units[it & 1];
+        const int q0 = uniform(u.q0), steps = uniform(u.steps);
+        const int first = uniform(t ? u.j0[1] : u.j0[0]), last = uniform(t ? u.j1[1] : u.j1[0]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&unit_empty[it & 1]);
+        if (q0 < 0) break;
+        const int q_last = last > first ? last - 1 : 0;   // the last step that reads Q
+        ok = __all_sync(~0u, mbar_wait(q_full, it & 1, 310));
+        if (steps == 0) {
+          tc_commit(q_empty);
+          continue;
+        }
+        for (int j = -1; ok && j < steps; ++j) {
+          const int n = j + 1, g = g0 + j;
+          // (also for steps this tile has no part in: a ring slot is free once both warps have let go of it)
+          if (j >= 0 && !(ok = __all_sync(~0u, mbar_wait(&v_ok[g % L::VST], (g / L::VST) & 1, 311)))) break;
+          if (n < steps && !(ok = __all_sync(~0u, mbar_wait(&k_full[(g + 1) % L::KST], ((g + 1) / L::KST) & 1, 312)))) break;
+          const bool pv = j >= first && j < last, qk = n >= first && n < last;
+          // The warps take turns, A first.  Left to themselves the two tiles' MMAs interleave and finish together, and
+          // both softmaxes then wait for both: 4,160 cycles a step, against 2,920 in turns.  (Passing the turn on before
+          // the last MMAs of S are issued, or waiting for P before the turn, settles into unequal halves: 3,220 cycles.)
+          if (t + r0 + n > 0 && !(ok = __all_sync(~0u, mbar_wait(&turn[t], (r0 + n - 1 + t) & 1, 316 + t)))) break;
+          if (pv) {
+            // O of the unit before is in registers
+            if (j == first && no > 0 && !(ok = __all_sync(~0u, mbar_wait(&o_free[t], (no - 1) & 1, 318)))) break;
+            if (!(ok = __all_sync(~0u, mbar_wait(&p_full[2 * t], (np + j - first) & 1, 313 + t)))) break;
+            tc_fence_after();
+            issue_pv(g % L::VST, 0, j != first);
+            if (!(ok = __all_sync(~0u, mbar_wait(&p_full[2 * t + 1], (np + j - first) & 1, 313 + t)))) break;
+            tc_fence_after();
+            issue_pv(g % L::VST, 1, true);
+            if (n == last) tc_commit(&o_done[t]);
+          }
+          tc_fence_after();
+          if (qk) {   // after PV(j) in issue order: P is read before S overwrites it
+            issue_s((g + 1) % L::KST);
+            tc_commit(&s_full[t]);
+          }
+          if (lane == 0) mbar_arrive(&turn[t ^ 1]);
+          __syncwarp();
+          if (j >= 0) tc_commit(&v_empty[g % L::VST]);
+          if (n < steps) tc_commit(&k_empty[(g + 1) % L::KST]);
+          if (n == q_last) tc_commit(q_empty);
+        }
+        g0 += steps;
+        r0 += steps + 1;
+        np += last - first;
+        no += last > first;
       }
-      if (j >= nv) {
-        if (!__all_sync(~0u, mbar_wait(&v_empty[j % L::VST], ((j / L::VST) & 1) ^ 1, 302))) break;
-        load_v(nv++, base);
-      }
-    }
-    // nothing may still be landing in this CTA's memory when it ends, after a wait that gave up included
-    mbar_drain(q_full, 0, 303);
-    for (int j = max(nk - L::KST, 0); j < nk; ++j) mbar_drain(&k_full[j % L::KST], (j / L::KST) & 1, 303);
-    for (int j = max(nv - L::VST, 0); j < nv; ++j) mbar_drain(&v_full[j % L::VST], (j / L::VST) & 1, 303);
-  } else if (warp == 9 || warp == 10) {
-    // ------------------------------------------------------------------ MMA of one tile
-    constexpr uint32_t idesc_s = idesc_bf16(128, 128, false), idesc_o = idesc_bf16(128, 128, true);
-    const int t = warp - 9;
-    const int first = t ? j0[1] : j0[0], last = t ? j1[1] : j1[0];
-    const uint32_t qa = smem_u32(smem + L::Q_OFF + t * L::TILE), s_tm = tmem + t * 128, o_tm = tmem + 256 + t * 128;
-    auto issue_s = [&](int j) {   // S = Q K_j^T: 8 MMAs over 16 dims each
-      const uint32_t ka = smem_u32(smem + L::K_OFF + (j % L::KST) * L::TILE);
-#pragma unroll
-      for (int kk = 0; kk < 8; ++kk) {
-        const uint32_t off = (kk >> 2) * L::SUB + (kk & 3) * 32;
-        mma_bf16_ss(s_tm, sdesc_kmajor_sw128(qa + off), sdesc_kmajor_sw128(ka + off), idesc_s, kk != 0);
-      }
-    };
-    auto issue_pv = [&](int j, int half) {   // O (+)= P V_j over 64 keys: 4 MMAs over 16 keys each
-      // V rows are keys (the K dimension), 64 dims contiguous: MN-major, 8-key groups 1,024 bytes apart, the two
-      // 64-dim halves SUB apart
-      const uint32_t va = smem_u32(smem + L::V_OFF + (j % L::VST) * L::TILE);
-#pragma unroll
-      for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
-        mma_bf16_ts(o_tm, s_tm + kk * 8, make_sdesc(va + kk * 2048, L::SUB, 1024, kLayoutSW128), idesc_o,
-                    j != first || kk != 0);
-    };
-    bool ok = steps > 0 && __all_sync(~0u, mbar_wait(q_full, 0, 310));
-    for (int j = -1; ok && j < steps; ++j) {
-      const int n = j + 1;
-      // (also for steps this tile has no part in: a ring slot is free once both warps have let go of it)
-      if (j >= 0 && !(ok = __all_sync(~0u, mbar_wait(&v_ok[j % L::VST], (j / L::VST) & 1, 311)))) break;
-      if (n < steps && !(ok = __all_sync(~0u, mbar_wait(&k_full[n % L::KST], (n / L::KST) & 1, 312)))) break;
-      const bool pv = j >= first && j < last, qk = n >= first && n < last;
-      // The warps take turns, A first.  Left to themselves the two tiles' MMAs interleave and finish together, and both
-      // softmaxes then wait for both: 4,160 cycles a step, against 2,920 in turns.  (Passing the turn on before the
-      // last MMAs of S are issued, or waiting for P before the turn, settles into unequal halves: 3,220 cycles.)
-      if (t + n > 0 && !(ok = __all_sync(~0u, mbar_wait(&turn[t], (n - 1 + t) & 1, 316 + t)))) break;
-      if (pv && !(ok = __all_sync(~0u, mbar_wait(&p_full[2 * t], (j - first) & 1, 313 + t)))) break;
-      tc_fence_after();
-      if (pv) {
-        issue_pv(j, 0);
-        if (!(ok = __all_sync(~0u, mbar_wait(&p_full[2 * t + 1], (j - first) & 1, 313 + t)))) break;
-        tc_fence_after();
-        issue_pv(j, 1);
-        if (n == last) tc_commit(&o_done[t]);
-      }
-      if (qk) {   // after PV(j) in issue order: P is read before S overwrites it
-        issue_s(n);
-        tc_commit(&s_full[t]);
-      }
-      if (lane == 0) mbar_arrive(&turn[t ^ 1]);
-      __syncwarp();
-      if (j >= 0) tc_commit(&v_empty[j % L::VST]);
-      if (n < steps) tc_commit(&k_empty[n % L::KST]);
-    }
-    if (steps > 0) {   // every MMA has left the tensor core before TMEM and shared memory are given back
+      // every MMA has left the tensor core before TMEM and shared memory are given back
       tc_commit(drained);
       mbar_drain(drained, 0, 315);
-    }
-  } else if (warp == 11) {
-    // ------------------------------------------------------------------ V guard
-    for (int j = 0; j < steps; ++j) {
-      const int vs = j % L::VST;
-      if (!__all_sync(~0u, mbar_wait(&v_full[vs], (j / L::VST) & 1, 320))) break;
-      if ((j >= j0[0] && j < j1[0] && hides(0, j)) || (j >= j0[1] && j < j1[1] && hides(1, j))) {
-        uint4* vt = reinterpret_cast<uint4*>(smem + L::V_OFF + vs * L::TILE);
-        uint32_t seen = 0;   // adding one to an exponent of all ones carries into the sign's place
-#pragma unroll 16
-        for (int i = lane; i < L::TILE / 16; i += 32) {
-          const uint4 u = vt[i];
-          seen |= ((u.x & 0x7F807F80u) + 0x00800080u) | ((u.y & 0x7F807F80u) + 0x00800080u) |
-                  ((u.z & 0x7F807F80u) + 0x00800080u) | ((u.w & 0x7F807F80u) + 0x00800080u);
-        }
-        const bool hit = __any_sync(~0u, (seen & 0x80008000u) != 0);
-        if (hit) {
-          for (int i = lane; i < L::TILE / 16; i += 32) {
-            uint4 u = vt[i];
-            uint32_t* w = &u.x;
+    } else {
+      // ---------------------------------------------------------------- V guard
+      bool ok = true;
+      int g = 0;
+      for (int it = 0; ok; ++it) {
+        if (!(ok = __all_sync(~0u, mbar_wait(&unit_full[it & 1], (it >> 1) & 1, 321)))) break;
+        const AttnBf16Unit u = units[it & 1];
+        if (u.q0 < 0) break;
+        // (a unit is published once the softmax warps are past the notes of the one two before it)
+        uint32_t* notes = bad + (it & 1) * L::BAD_WORDS;
+        for (int i = lane; i < (u.steps + 31) >> 5; i += 32) notes[i] = 0;
+        if (lane == 0) any_bad[it & 1] = 0;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&unit_empty[it & 1]);
+        for (int j = 0; j < u.steps; ++j, ++g) {
+          const int vs = g % L::VST;
+          if (!(ok = __all_sync(~0u, mbar_wait(&v_full[vs], (g / L::VST) & 1, 320)))) break;
+          const int kb = u.base + 128 * j;
+          bool hides = false;   // some key of the step from some live row of a tile
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if ((w[e] & 0x7F80u) == 0x7F80u) w[e] &= 0xFFFF0000u;
-              if ((w[e] & 0x7F800000u) == 0x7F800000u) w[e] &= 0x0000FFFFu;
+          for (int t = 0; t < 2; ++t)
+            hides |= j >= u.j0[t] && j < u.j1[t] && (u.lo_max[t] > kb || u.hi_min[t] < kb + 128);
+          if (hides) {
+            uint4* vt = reinterpret_cast<uint4*>(smem + L::V_OFF + vs * L::TILE);
+            uint32_t seen = 0;   // adding one to an exponent of all ones carries into the sign's place
+#pragma unroll 8
+            for (int i = lane; i < L::TILE / 16; i += 32) {
+              const uint4 w = vt[i];
+              seen |= ((w.x & 0x7F807F80u) + 0x00800080u) | ((w.y & 0x7F807F80u) + 0x00800080u) |
+                      ((w.z & 0x7F807F80u) + 0x00800080u) | ((w.w & 0x7F807F80u) + 0x00800080u);
             }
-            vt[i] = u;
+            if (__any_sync(~0u, (seen & 0x80008000u) != 0)) {
+              for (int i = lane; i < L::TILE / 16; i += 32) {
+                uint4 x = vt[i];
+                uint32_t* w = &x.x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  if ((w[e] & 0x7F80u) == 0x7F80u) w[e] &= 0xFFFF0000u;
+                  if ((w[e] & 0x7F800000u) == 0x7F800000u) w[e] &= 0x0000FFFFu;
+                }
+                vt[i] = x;
+              }
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMA reads these writes
+              if (lane == 0) {
+                notes[j >> 5] |= 1u << (j & 31);
+                any_bad[it & 1] = 1;
+              }
+            }
           }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMA reads these writes
-          if (lane == 0) {
-            bad[j >> 5] |= 1u << (j & 31);
-            *any_bad = 1;
-          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_ok[vs]);
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&guard_done[it & 1]);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&v_ok[vs]);
     }
   } else {
     // ------------------------------------------------------------------ softmax: one thread per query row
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int t = warp >> 2;
-    const int first = t ? j0[1] : j0[0], last = t ? j1[1] : j1[0];
-    const int lo_top = t ? lo_max[1] : lo_max[0], hi_low = t ? hi_min[1] : hi_min[0];
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_col = tmem + lane_off + t * 128, o_col = tmem + lane_off + 256 + t * 128;
     const float scale = kLog2e * 0.08838834764831845f;   // log2(e) / sqrt(128)
     const uint64_t scale2 = f32x2_splat(scale);
-    const bool live = lo < hi;
-    float m_used = -INFINITY;   // the row's own largest score, not a rounded one: its P is then exactly 1 in bf16 too
-    uint64_t l2a = 0, l2b = 0;
-    bool ok = true, bounded = false;
-    if (p.knorm && last > first) {
-      const int ntiles = (p.S + 127) >> 7;
-      const float* kn = p.knorm + (size_t)hk * ntiles;
-      float kk = 0.f;
-      for (int i = (base >> 7) + lane; i <= (kend - 1) >> 7; i += 32) kk = max_nan(kk, kn[i]);
-#pragma unroll
-      for (int o = 16; o; o >>= 1) kk = max_nan(kk, __shfl_xor_sync(~0u, kk, o));
-      ok = __all_sync(~0u, mbar_wait(q_full, 0, 334));
-      float qq = 0.f;
-      const uint8_t* qr = smem + L::Q_OFF + t * L::TILE + (threadIdx.x & 127) * 128;
-#pragma unroll
-      for (int c = 0; c < 16; ++c) {   // (any order of the row's pieces will do)
-        const uint4 u = *reinterpret_cast<const uint4*>(qr + (c >> 3) * L::SUB + (((c ^ lane) & 7) << 4));
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) qq += bf16_lo(w[e]) * bf16_lo(w[e]) + bf16_hi(w[e]) * bf16_hi(w[e]);
+    uint8_t* stage = smem + L::STAGE_OFF + warp * L::STAGE;
+    bool ok = true;
+    int ns = 0, no = 0;   // this tile's steps and its units with keys so far
+    for (int it = 0; ok; ++it) {
+      if (!(ok = __all_sync(~0u, mbar_wait(&unit_full[it & 1], (it >> 1) & 1, 336)))) break;
+      const AttnBf16Unit& u = units[it & 1];
+      const int q0 = u.q0, h = u.h, base = u.base;
+      if (q0 < 0) break;
+      const int first = t ? u.j0[1] : u.j0[0], last = t ? u.j1[1] : u.j1[0];
+      const int lo_top = t ? u.lo_max[1] : u.lo_max[0], hi_low = t ? u.hi_min[1] : u.hi_min[0];
+      const bool any = last > first;
+      const int query = q0 + threadIdx.x, q_end = min(q0 + p.rows, p.S);
+      int lo = 0, hi = 0;   // this row's span
+      if (query < q_end) {
+        lo = p.lo ? max(p.lo[query], 0) : 0;
+        hi = p.hi ? min(p.hi[query], p.S) : p.S;
       }
-      bounded = __all_sync(~0u, !live || 2.0f * scale * sqrtf(qq) * sqrtf(kk) < kBoundBf16);
-    }
-    for (int j = first; ok && j < last; ++j) {
-      const int i = j - first, kb = base + 128 * j;
-      ok = __all_sync(~0u, mbar_wait(&s_full[t], i & 1, 330 + t));
-      if (!ok) break;
-      tc_fence_after();
-      uint32_t s[4][32];
+      const bool live = lo < hi;
+      float m_used = -INFINITY;   // the row's own largest score, not a rounded one: its P is then exactly 1 in bf16 too
+      uint64_t l2a = 0, l2b = 0;
+      bool bounded = false;
+      if (!(ok = __all_sync(~0u, mbar_wait(q_full, it & 1, 334)))) break;
+      if (p.knorm && any) {
+        float qq = 0.f;
+        const uint8_t* qr = smem + L::Q_OFF + t * L::TILE + (threadIdx.x & 127) * 128;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(s_col + 32 * c, s[c]);
-      tmem_ld_wait();
-      const bool masked = lo_top > kb || hi_low < kb + 128;
-      if (masked && live) {   // (a row without keys takes the scores as they are and is zeroed at the end)
+        for (int c = 0; c < 16; ++c) {   // (any order of the row's pieces will do)
+          const uint4 v = *reinterpret_cast<const uint4*>(qr + (c >> 3) * L::SUB + (((c ^ lane) & 7) << 4));
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const uint32_t vis = bits_below(hi - kb - 32 * c) & ~bits_below(lo - kb - 32 * c);
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!((vis >> e) & 1u)) s[c][e] = __float_as_uint(-INFINITY);
+          for (int e = 0; e < 4; ++e) qq += bf16_lo(w[e]) * bf16_lo(w[e]) + bf16_hi(w[e]) * bf16_hi(w[e]);
         }
+        bounded = __all_sync(~0u, !live || 2.0f * scale * sqrtf(qq) * sqrtf(u.kk) < kBoundBf16);
       }
-      if (!bounded || __any_sync(~0u, m_used == -INFINITY)) {
-        const float mx = fmaxf(fmaxf(max_chunk(s[0], -INFINITY), max_chunk(s[1], -INFINITY)),
-                               fmaxf(max_chunk(s[2], -INFINITY), max_chunk(s[3], -INFINITY)));
-        const float mnew = mx * scale;
-        const bool need = m_used == -INFINITY ? mnew > m_used : mnew > m_used + kTauBf16 && !bounded;
-        float alpha = 1.0f;
-        if (need) {
-          alpha = m_used == -INFINITY ? 0.0f : ex2(m_used - mnew);
-          m_used = mnew;
-          const uint64_t a2 = f32x2_splat(alpha);
-          l2a = mul2(l2a, a2);
-          l2b = mul2(l2b, a2);
-        }
-        // O holds the PV of every earlier step here: those MMAs were issued before S of this step by the same thread,
-        // and s_full counts everything issued before its commit
-        if (i > 0 && __any_sync(~0u, need)) {
-#pragma unroll 1
-          for (int c = 0; c < 8; ++c) {
-            uint32_t o[16];
-            tmem_ld16(o_col + 16 * c, o);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_empty);
+      for (int j = first; j < last; ++j, ++ns) {
+        const int kb = base + 128 * j;
+        if (!(ok = __all_sync(~0u, mbar_wait(&s_full[t], ns & 1, 330 + t)))) break;
+        tc_fence_after();
+        auto written = [&](int half) {   // P of 64 keys
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[2 * t + half]);
+        };
+        const bool masked = lo_top > kb || hi_low < kb + 128;
+        if (bounded && !masked && !__any_sync(~0u, m_used == -INFINITY)) {
+          // nearly every step of a long row: 32 scores at a time, the next on their way (P's words lie over scores that
+          // have been read)
+          uint32_t s[2][32];
+          tmem_ld32(s_col, s[0]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
             tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st16(o_col + 16 * c, o);
+            if (c < 3) tmem_ld32(s_col + 32 * (c + 1), s[(c + 1) & 1]);
+            uint32_t pw[16];
+            p_chunk_bf16<true>(s[c & 1], scale2, -m_used, pw, l2a, l2b);
+            tmem_st16(s_col + 16 * c, pw);
+            if (c & 1) written(c >> 1);
           }
+          continue;
+        }
+        // 64 scores at a time, twice: for the maximum, and for P
+        uint32_t s[2][32];
+        auto scores = [&](int half) {
+          tmem_ld32(s_col + 64 * half, s[0]);
+          tmem_ld32(s_col + 64 * half + 32, s[1]);
+          tmem_ld_wait();
+          if (masked && live) {   // (a row without keys takes the scores as they are and is zeroed at the end)
+            const int k = kb + 64 * half;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const uint32_t vis = bits_below(hi - k - 32 * c) & ~bits_below(lo - k - 32 * c);
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!((vis >> e) & 1u)) s[c][e] = __float_as_uint(-INFINITY);
+            }
+          }
+        };
+        if (!bounded || __any_sync(~0u, m_used == -INFINITY)) {
+          float mx = -INFINITY;
+#pragma unroll 1
+          for (int half = 0; half < 2; ++half) {
+            scores(half);
+            mx = fmaxf(mx, fmaxf(max_chunk(s[0], -INFINITY), max_chunk(s[1], -INFINITY)));
+          }
+          const float mnew = mx * scale;
+          const bool need = m_used == -INFINITY ? mnew > m_used : mnew > m_used + kTauBf16 && !bounded;
+          float alpha = 1.0f;
+          if (need) {
+            alpha = m_used == -INFINITY ? 0.0f : ex2(m_used - mnew);
+            m_used = mnew;
+            const uint64_t a2 = f32x2_splat(alpha);
+            l2a = mul2(l2a, a2);
+            l2b = mul2(l2b, a2);
+          }
+          // O holds the PV of every earlier step here: those MMAs were issued before S of this step by the same thread,
+          // and s_full counts everything issued before its commit
+          if (j > first && __any_sync(~0u, need)) {
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+              uint32_t o[16];
+              tmem_ld16(o_col + 16 * c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_st16(o_col + 16 * c, o);
+            }
+          }
+        }
+        const float nm = m_used == -INFINITY ? 0.0f : -m_used;   // no key yet: P = exp2(-inf) = 0
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          scores(half);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t pw[16];
+            p_chunk_bf16<false>(s[c], scale2, nm, pw, l2a, l2b);
+            tmem_st16(s_col + 32 * half + 16 * c, pw);
+          }
+          written(half);
         }
       }
-      const float nm = m_used == -INFINITY ? 0.0f : -m_used;   // no key yet: P = exp2(-inf) = 0
-      auto emit = [&](auto poly) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pw[16];
-          p_chunk_bf16<decltype(poly)::value>(s[c], scale2, nm, pw, l2a, l2b);
-          tmem_st16(s_col + 16 * c, pw);
-          if (c & 1) {
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[2 * t + (c >> 1)]);
-          }
-        }
-      };
-      if (bounded && !masked) emit(std::true_type{});
-      else emit(std::false_type{});
-    }
-    // ---- epilogue: O / l -> bf16, this thread's row
-    const bool any = last > first;
-    // (the last v_ok: every note of the V guard is visible)
-    if (any)
-      ok = __all_sync(~0u, ok && mbar_wait(&o_done[t], 0, 332) &&
-                               mbar_wait(&v_ok[(steps - 1) % L::VST], ((steps - 1) / L::VST) & 1, 333));
-    const int query0 = q0 + warp * 32;
-    if (ok && query0 < q_end) {
-      tc_fence_after();
+      // ---- epilogue: O / l -> bf16, this thread's row
+      if (ok && any) ok = __all_sync(~0u, mbar_wait(&o_done[t], no & 1, 332));
+      if (ok) ok = __all_sync(~0u, mbar_wait(&guard_done[it & 1], (it >> 1) & 1, 333));
+      if (!ok) break;
+      if (any) tc_fence_after();
       float la, lb, lc, ld;
       f32x2_unpack(l2a, la, lb);
       f32x2_unpack(l2b, lc, ld);
       const float inv_l = 1.0f / ((la + lb) + (lc + ld));
-      const bool repair = any && *(volatile int*)any_bad != 0;
-      // through the tile's Q rows (its MMAs are complete), swizzled, and out by TMA: 32 rows a warp, whole lines
-      // instead of one row a thread (3.7 us of a CTA)
-      if (!any) ok = __all_sync(~0u, mbar_wait(q_full, 0, 335));   // Q has landed: nothing overwrites these rows
-      uint8_t* rows = smem + L::Q_OFF + t * L::TILE + (warp & 3) * 32 * 128;
-      uint32_t o[4][32];
-      if (any) {
+      const bool repair = any && live && *(volatile int*)&any_bad[it & 1] != 0;
+      const uint32_t* notes = bad + (it & 1) * L::BAD_WORDS;
+      const int query0 = q0 + warp * 32;
+      // 64 dims at a time through shared memory, swizzled, and out by TMA: whole lines instead of one row a thread
+      // (3.7 us of a unit)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(o_col + 32 * c, o[c]);
-        tmem_ld_wait();
-      }
+      for (int half = 0; half < 2; ++half) {
+        uint32_t o[2][32];
+        if (any) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float f[32];
+          for (int c = 0; c < 2; ++c) tmem_ld32(o_col + 64 * half + 32 * c, o[c]);
+          tmem_ld_wait();
+          if (half == 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_free[t]);
+          }
+        }
+        if (query0 >= q_end) continue;
+        uint32_t w[32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) f[e] = live ? __uint_as_float(o[c][e]) * inv_l : 0.0f;
-        if (repair && live) {   // non-finite V elements this row does see
-          for (int j = first; j < last; ++j) {
-            if (!((bad[j >> 5] >> (j & 31)) & 1u)) continue;
-            const int kb = base + 128 * j;
-            for (int key = max(kb, lo); key < min(kb + 128, hi); ++key) {
-              const __nv_bfloat16* vr = p.v + (long long)key * p.ldv + (long long)hk * p.hsv + 32 * c;
+        for (int c = 0; c < 2; ++c) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                const float x = __bfloat162float(vr[e]);
-                if (!isfinite(x)) f[e] += x;
+          for (int e = 0; e < 32; ++e) o[c][e] = live ? __float_as_uint(__uint_as_float(o[c][e]) * inv_l) : 0u;
+          if (repair) {   // non-finite V elements this row does see
+            for (int j = first; j < last; ++j) {
+              if (!((notes[j >> 5] >> (j & 31)) & 1u)) continue;
+              const int kb = base + 128 * j;
+              for (int key = max(kb, lo); key < min(kb + 128, hi); ++key) {
+                const __nv_bfloat16* vr =
+                    p.v + (long long)key * p.ldv + (long long)(h / p.group) * p.hsv + 64 * half + 32 * c;
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                  const float x = __bfloat162float(vr[e]);
+                  if (!isfinite(x)) o[c][e] = __float_as_uint(__uint_as_float(o[c][e]) + x);
+                }
               }
             }
           }
-        }
-        uint8_t* row = rows + (c >> 1) * L::SUB + lane * 128;
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4)
-          *reinterpret_cast<uint4*>(row + ((((c & 1) * 4 + q4) ^ (lane & 7)) << 4)) =
-              make_uint4(pack_bf16(f[8 * q4], f[8 * q4 + 1]), pack_bf16(f[8 * q4 + 2], f[8 * q4 + 3]),
-                         pack_bf16(f[8 * q4 + 4], f[8 * q4 + 5]), pack_bf16(f[8 * q4 + 6], f[8 * q4 + 7]));
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the store reads these writes
-      __syncwarp();
-      if (ok) {
-        tma_store_3d(&tmO, rows, 0, query0, h);
-        tma_store_3d(&tmO, rows + L::SUB, 64, query0, h);
+          for (int e = 0; e < 16; ++e)
+            w[16 * c + e] = pack_bf16(__uint_as_float(o[c][2 * e]), __uint_as_float(o[c][2 * e + 1]));
+        }
+        tma_store_wait_read<0>();   // the rows that were here have been read
+        __syncwarp();
+#pragma unroll
+        for (int q8 = 0; q8 < 8; ++q8)
+          *reinterpret_cast<uint4*>(stage + lane * 128 + ((q8 ^ (lane & 7)) << 4)) =
+              make_uint4(w[4 * q8], w[4 * q8 + 1], w[4 * q8 + 2], w[4 * q8 + 3]);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the store reads these writes
+        __syncwarp();
+        tma_store_3d(&tmO, stage, 64 * half, query0, h);
         tma_store_commit();
-        tma_store_wait_read<0>();
       }
+      no += any;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&unit_empty[it & 1]);
     }
+    tma_store_wait_read<0>();
   }
   tc_fence_before();
   __syncthreads();

@@ -38,6 +38,9 @@ __device__ __forceinline__ void fence_barrier_init() {
 // elect.sync inside the instruction sequence picks the one lane that issues.  The operands then stay in warp-uniform
 // registers: issuing the same instructions from a lane-0 branch instead costs tens of cycles each (a tcgen05.mma
 // from a lane-0 branch takes ~60 cycles to issue, from the whole warp ~7), which starves the tensor pipe.
+// A value that all lanes hold, such as a warp's index or one read from shared memory, as the compiler can know it: an
+// operand that it takes for a lane's own costs a move to a uniform register at every issue.
+__device__ __forceinline__ int uniform(int x) { return __reduce_max_sync(~0u, x); }
 #define H3_ELECT "elect.sync rx|e, 0xffffffff;\n\t"
 // warp-wide: one arrival that also expects `bytes` of transaction data
 __device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t* bar, uint32_t bytes) {
@@ -202,6 +205,11 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
                : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Programmatic dependent launch: the next kernel of the stream may start its blocks once every block of this one got
+// here, and waits in wait_primary for this one's end (memory included) before it touches what this one wrote.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ------------------------------------------------------------------------------------------------ CTA pairs (cta_group::2)
 // A cluster of two CTAs on two SMs sharing one MMA: rank 0 (the leader) issues every tcgen05.mma / tcgen05.cp of the

@@ -238,6 +238,22 @@ AttnWs attn_ws(int S, int H) {
   return w;
 }
 
+// Launches a kernel that waits itself, by griddepcontrol.wait, for the stream's kernel before it.
+template <typename... P, typename... A>
+cudaError_t launch_after(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream, A&&... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
 }  // namespace
 
 extern "C" {
@@ -797,9 +813,9 @@ int h3_attn_fp8_sparse(const void* q, const void* k, const void* v, long long ld
 }
 
 namespace {
-// workspace of h3_attn_bf16: key norms, span ranges, tile order
+// workspace of h3_attn_bf16: key norms, span ranges, tile order, units handed out
 struct AttnBf16Ws {
-  size_t knorm, range, order, total;
+  size_t knorm, range, order, next, total;
 };
 AttnBf16Ws attn_bf16_ws(int S, int Hk) {
   const size_t n = (S + 127) / 128;
@@ -807,7 +823,8 @@ AttnBf16Ws attn_bf16_ws(int S, int Hk) {
   w.knorm = 0;
   w.range = align_up((size_t)Hk * n * 4, 16);
   w.order = w.range + align_up(n * 8, 16);
-  w.total = w.order + (n + 1) / 2 * 16;
+  w.next = w.order + align_up((n + 1) / 2 * 4, 16);
+  w.total = w.next + 16;
   return w;
 }
 }  // namespace
@@ -868,17 +885,25 @@ int h3_attn_bf16(const void* q, long long ldq, long long hsq, const void* k, lon
     uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
     AttnBf16Prep pr{reinterpret_cast<const __nv_bfloat16*>(k), ldk, hsk, S, span_lo, span_hi,
                     reinterpret_cast<float*>(ws + w.knorm), reinterpret_cast<int2*>(ws + w.range),
-                    reinterpret_cast<int4*>(ws + w.order)};
+                    reinterpret_cast<int*>(ws + w.order), reinterpret_cast<int*>(ws + w.next)};
     attn_bf16_prep_kernel<<<dim3((S + 127) / 128, Hk), 256, 0, S_(stream)>>>(pr);
     if ((rc = check_launch(who))) return rc;
     a.knorm = pr.knorm;
+    a.next = pr.next;
     if (span_lo && a.tile_major && a.rows == 256) {
-      attn_bf16_order_kernel<<<1, 1024, 0, S_(stream)>>>(pr, a.tiles);
-      if ((rc = check_launch(who))) return rc;
+      cudaError_t e = launch_after(attn_bf16_order_kernel, 1, 1024, 0, S_(stream), pr, a.tiles);
+      if (e != cudaSuccess) return fail(H3_ERR_CUDA, "%s: launch: %s", who, cudaGetErrorString(e));
       a.order = pr.order;
     }
   }
-  attn_bf16_kernel<<<(unsigned)((long long)a.tiles * Hq), kAttnBf16Threads, L::TOTAL, S_(stream)>>>(tq, tk, tv, to, a);
+  const long long units = (long long)a.tiles * Hq;
+  if (!workspace) {
+    attn_bf16_kernel<<<(unsigned)units, kAttnBf16Threads, L::TOTAL, S_(stream)>>>(tq, tk, tv, to, a);
+  } else {
+    cudaError_t e = launch_after(attn_bf16_kernel, (unsigned)(units < num_sms() ? units : num_sms()), kAttnBf16Threads,
+                                 L::TOTAL, S_(stream), tq, tk, tv, to, a);
+    if (e != cudaSuccess) return fail(H3_ERR_CUDA, "%s: launch: %s", who, cudaGetErrorString(e));
+  }
   return check_launch(who);
 }
 
