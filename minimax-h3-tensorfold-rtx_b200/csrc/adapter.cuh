@@ -199,7 +199,7 @@ struct TileInfo {
 __device__ __forceinline__ TileInfo tile_info(const AdapterArgs& a, int t) {
   if (!a.tile) return {0, t * 128, min(128, a.M - t * 128), t * 128};
   const int4 v = a.tile[t];
-  return {v.x, v.y, v.z, v.w};
+  return {uniform(v.x), uniform(v.y), uniform(v.z), uniform(v.w)};
 }
 // Rows a lane copies of a tile whose rows do not follow one another: G of them from r0 on, every fourth (a lane's eighth
 // of 128 bytes); -1 past the last.
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(192)
   uint64_t* acc_full = empty + L::MAX_STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   int* skip_s = reinterpret_cast<int*>(tmem_slot + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   constexpr uint32_t ncols = 128;
   if (a.tile) wait_primary();   // the plan
   else if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.next = 0;
@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(192)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform(*tmem_slot);
   const bool skip = !a.tile && *skip_s;   // the same in every CTA of the cluster
 
   if (skip) {
@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(448)
   int* first_s = kind_s + 2;                              // [2]: first row when the rows follow one another, else -1
   int* count_s = first_s + 2;                             // [2]: rows
   uint32_t* has_s = reinterpret_cast<uint32_t*>(count_s + 2);   // [2][4]: the rows that have the adapter
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int ntile = (a.N + 127) >> 7;
   const int strips = (ntile + a.width - 1) / a.width;
 
@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(448)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform(*tmem_slot);
   auto cols = [&](int unit, int& x0, int& x1) {   // a unit's tiles [x0, x1) of columns
     x0 = unit % strips * a.width;
     x1 = min(x0 + a.width, ntile);
@@ -573,7 +573,7 @@ __global__ void __launch_bounds__(448)
           tma_load_3d(bs + (st * kc + c) * L::SUB, &tmB, 64 * c, x * 128, tile.adapter, &b_full[st]);
         ++nb;
       }
-      unit = __shfl_sync(~0u, unit, 0);
+      unit = uniform(lane == 0 ? unit : 0);
     }
     if (!waited) wait_primary();   // (a call ends after all its kernels)
     for (int j = max(ny - nys, 0); j < ny; ++j) mbar_drain(&y_full[j % nys], (j / nys) & 1, 454);
@@ -587,7 +587,7 @@ __global__ void __launch_bounds__(448)
     for (int it = 0; ok; ++it) {
       const int b = it & 1;
       if (!(ok = __all_sync(~0u, mbar_wait(&unit_full[b], (it >> 1) & 1, 460)))) break;
-      const int unit = unit_s[b], kind = kind_s[b];
+      const int unit = uniform(unit_s[b]), kind = uniform(kind_s[b]);
       __syncwarp();
       if (lane == 0) mbar_arrive(&unit_empty[b]);
       if (unit < 0) break;
