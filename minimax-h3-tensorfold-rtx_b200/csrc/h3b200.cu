@@ -1008,13 +1008,17 @@ int h3_adapter_add(const void* x, long long ldx, const void* y, long long ldy, c
   // the K range over a cluster of CTAs while the row tiles alone leave SMs idle, at least four 64-element stages each
   const int chunks = (K + 63) / 64;
   int splits = 1;
-  const int fit = Rp > 64 ? num_sms() * 7 / 8 : 2 * num_sms();   // CTAs of clusters that are resident together, about
+  // (clusters leave some SMs of their groups unused: 7/8 of the SMs hold one CTA each, about.  Two CTAs an SM, possible
+  // to rank 64, only where that lets all run at once: 4,096 rows of four rank-64 adapters 44 us against 52, but 39
+  // against 35 where one each is enough)
+  const int alone = num_sms() * 7 / 8, fit = Rp > 64 ? alone : num_sms();
   while (splits < 8 && tiles * splits * 2 <= fit && chunks >= splits * 8) splits *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)w.tiles, splits);
   cfg.blockDim = dim3(192);
   const long long per_sm = (tiles * splits + num_sms() - 1) / num_sms();
-  a.stages = ShrinkSmem::stages(Rp, splits, per_sm < 2 ? 1 : splits > 1 && Rp > 64 ? 1 : per_sm < 3 || splits > 1 ? 2 : 3);
+  const int ctas = splits > 1 ? (tiles * splits <= alone ? 1 : 2) : per_sm < 2 ? 1 : per_sm < 3 ? 2 : 3;
+  a.stages = ShrinkSmem::stages(Rp, splits, ctas);
   cfg.dynamicSmemBytes = ShrinkSmem::total(Rp, splits, a.stages);
   cfg.stream = S_(stream);
   cudaLaunchAttribute attr[2];
