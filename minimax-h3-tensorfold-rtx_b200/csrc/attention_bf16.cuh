@@ -119,6 +119,7 @@ struct AttnBf16Args {
   const int* lo;             // spans, or NULL: every key
   const int* hi;
   const float* knorm;        // [key heads][S / 128 tiles]: largest |k|^2 of each 128 keys, or NULL
+  const float* knorm1;       // [key heads][S]: of each key
   const int* order;          // [S / 256 tiles]: query tiles by falling number of key steps, or NULL
   int S, group;              // group: query heads that share a key head
   int* next;                 // units handed out beyond each CTA's first, or NULL: a CTA for every unit
@@ -208,14 +209,14 @@ __device__ __forceinline__ void p_chunk_bf16(const uint32_t (&s)[32], uint64_t s
   }
 }
 
-// Before the attention, for long sequences: the largest |k|^2 of each 128 keys and head (NaN when one is), and the span
-// range of each 128 query rows.  Bound by reading K once: 16 lanes a row.
+// Before the attention, for long sequences: |k|^2 of each key and head, the largest of each 128 (NaN when one is), and the
+// span range of each 128 query rows.  Bound by reading K once: 16 lanes a row.
 struct AttnBf16Prep {
   const __nv_bfloat16* k;
   long long ld, hs;
   int S;
   const int *lo, *hi;
-  float* knorm;
+  float *knorm, *knorm1;
   int2* range;         // [S / 128 tiles]: first and end key of the tile's rows
   int* order;
   int* next;           // to zero
@@ -252,6 +253,8 @@ __global__ void __launch_bounds__(256) attn_bf16_prep_kernel(const AttnBf16Prep 
 #pragma unroll
     for (int o = 8; o; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
     m = max_nan(m, ss);
+    const int t = blockIdx.x * 128 + row0 + 16 * i;
+    if (part == 0 && t < a.S) a.knorm1[(size_t)blockIdx.y * a.S + t] = ss;
   }
   if (part == 0) red[row0] = m;
   __syncthreads();
@@ -382,8 +385,19 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
     }
     u.kk = 0.f;
     if (p.knorm && u.steps > 0) {
+      // exactly the unit's keys, so that its results do not depend, in their rounding, on what lies beside them
+      const int t0 = u.base >> 7, t1 = (kend - 1) >> 7;
+      const float* one = p.knorm1 + (size_t)(u.h / p.group) * p.S;
+      float edge[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int key = (i < 4 ? t0 : t1) * 128 + (i & 3) * 32 + lane;
+        edge[i] = key >= u.base && key < kend ? one[key] : 0.f;
+      }
       const float* kn = p.knorm + (size_t)(u.h / p.group) * ((p.S + 127) >> 7);
-      for (int i = (u.base >> 7) + lane; i <= (kend - 1) >> 7; i += 32) u.kk = max_nan(u.kk, kn[i]);
+      for (int i = t0 + 1 + lane; i < t1; i += 32) u.kk = max_nan(u.kk, kn[i]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) u.kk = max_nan(u.kk, edge[i]);
 #pragma unroll
       for (int o = 16; o; o >>= 1) u.kk = max_nan(u.kk, __shfl_xor_sync(~0u, u.kk, o));
     }

@@ -815,13 +815,14 @@ int h3_attn_fp8_sparse(const void* q, const void* k, const void* v, long long ld
 namespace {
 // workspace of h3_attn_bf16: key norms, span ranges, tile order, units handed out
 struct AttnBf16Ws {
-  size_t knorm, range, order, next, total;
+  size_t knorm, knorm1, range, order, next, total;
 };
 AttnBf16Ws attn_bf16_ws(int S, int Hk) {
   const size_t n = (S + 127) / 128;
   AttnBf16Ws w;
   w.knorm = 0;
-  w.range = align_up((size_t)Hk * n * 4, 16);
+  w.knorm1 = align_up((size_t)Hk * n * 4, 16);
+  w.range = w.knorm1 + align_up((size_t)Hk * S * 4, 16);
   w.order = w.range + align_up(n * 8, 16);
   w.next = w.order + align_up((n + 1) / 2 * 4, 16);
   w.total = w.next + 16;
@@ -884,11 +885,13 @@ int h3_attn_bf16(const void* q, long long ldq, long long hsq, const void* k, lon
     const AttnBf16Ws w = attn_bf16_ws(S, Hk);
     uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
     AttnBf16Prep pr{reinterpret_cast<const __nv_bfloat16*>(k), ldk, hsk, S, span_lo, span_hi,
-                    reinterpret_cast<float*>(ws + w.knorm), reinterpret_cast<int2*>(ws + w.range),
+                    reinterpret_cast<float*>(ws + w.knorm), reinterpret_cast<float*>(ws + w.knorm1),
+                    reinterpret_cast<int2*>(ws + w.range),
                     reinterpret_cast<int*>(ws + w.order), reinterpret_cast<int*>(ws + w.next)};
     attn_bf16_prep_kernel<<<dim3((S + 127) / 128, Hk), 256, 0, S_(stream)>>>(pr);
     if ((rc = check_launch(who))) return rc;
     a.knorm = pr.knorm;
+    a.knorm1 = pr.knorm1;
     a.next = pr.next;
     if (span_lo && a.tile_major && a.rows == 256) {
       cudaError_t e = launch_after(attn_bf16_order_kernel, 1, 1024, 0, S_(stream), pr, a.tiles);

@@ -133,6 +133,55 @@ def test_any_spans(kind):
     device_ok()
 
 
+@pytest.mark.parametrize("kind", ["documents", "frames", "random", "one_key", "none", "every"])
+def test_many_tiles_a_cta(kind):
+    """440 pairs of query tiles, more than run at once: each CTA works through several of differing lengths, some with no
+    keys at all, and what one tile's masked values held must not reach the next."""
+
+    from tfvideo import attention as A
+
+    S, Hq, Hk = 2700, 40, 8
+    rs = np.random.RandomState(3)
+    if kind == "documents":
+        m = A.SpanMask.documents([700, 1, 0, 999, 300], S)                        # the last 700 tokens have no keys
+    elif kind == "frames":
+        m = A.SpanMask.frames([1500, 1100], 90, [100, 0], S)
+    elif kind == "every":
+        m = A.SpanMask.documents([S])
+    else:
+        lo = rs.randint(-5, S, S)
+        n = {"random": rs.randint(-300, 300, S), "one_key": np.full(S, 1), "none": np.full(S, 0)}[kind]
+        n[1024:1536] = 0                                                          # whole tiles without keys
+        m = A.SpanMask(*(torch.from_numpy(x.astype(np.int32)).cuda() for x in (lo, lo + n)))
+    q, k, v = (t.clone() for t in packed(S, Hq, Hk, 21))
+    o = A.bf16(q, k, v, m)
+    check(o, q, k, v, m.lo, m.hi)
+    assert torch.equal(o, A.bf16(q, k, v, m))
+    if kind in ("documents", "frames"):                                           # padding and one head's first request
+        at = 2000 if kind == "documents" else 2600
+        for t in (k, v):
+            t[:, :, at:] = float("nan")
+        v[:, 3, 100, 5] = float("inf")
+        bad = A.bf16(q, k, v, m)
+        seen = (m.lo <= 100) & (m.hi > 100)
+        for h in range(Hq):
+            same = torch.ones((S, 128), dtype=torch.bool, device="cuda")
+            if h // 5 == 3:
+                same[seen, 5] = False
+                assert torch.isposinf(bad[0, h, seen, 5]).all()
+            assert torch.equal(bad[0, h][same], o[0, h][same])
+    device_ok()
+
+
+def test_many_short_heads():
+    from tfvideo import attention as A
+
+    m = A.SpanMask.documents([100, 0, 130, 33], 300)
+    q, k, v = packed(300, 200, 50, 22)
+    check(A.bf16(q, k, v, m), q, k, v, m.lo, m.hi)
+    device_ok()
+
+
 def test_layouts():
     """Head-major memory, separate buffers, unaligned and strided views (copied when TMA cannot read them), shared
     heads as an expanded view: the same bits as contiguous rows."""
