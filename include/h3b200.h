@@ -242,8 +242,9 @@ int h3_attn_fp8_peers(const void* q, const void* k, const void* v, long long ld,
  * Hk key heads in groups of Hq / Hk.  q, k and v are bf16 views with their own token and head strides (multiples of 8
  * elements, 16-byte aligned), element (t, h, d) at t * ld + h * hs + d; out (t, h, d) at out + t * ldo + h * 128 + d,
  * apart from the inputs (H3_ERR_ARG otherwise).  Scores are scaled by 1 / sqrt(128).  S <= 262,144.  workspace: h3_attn_bf16_workspace_bytes(S, Hk) bytes, 16-byte aligned
- * (0, and NULL, for short sequences), one per call in flight: the key norms that let long rows of bounded scores skip
- * their running maximum; NULL is always accepted and only slower.  The reference's backends
+ * (0 for short sequences, which use none), one per call in flight: the key norms that let long rows of bounded scores
+ * skip their running maximum; NULL is always accepted and only slower.  A key that a row does not see can change that
+ * row's rounding, where rows of its 256-row tile see it, but no more.  The reference's backends
  * (tfvideo/attention.py:29-54) attend to the whole sequence. */
 size_t h3_attn_bf16_workspace_bytes(int S, int Hk);
 int h3_attn_bf16(const void* q, long long ldq, long long hsq, const void* k, long long ldk, long long hsk,

@@ -831,7 +831,9 @@ AttnBf16Ws attn_bf16_ws(int S, int Hk) {
 }  // namespace
 
 // (below 2,048 tokens a row has too few key steps to win back the two extra launches)
-size_t h3_attn_bf16_workspace_bytes(int S, int Hk) { return S < 2048 || Hk <= 0 ? 0 : attn_bf16_ws(S, Hk).total; }
+size_t h3_attn_bf16_workspace_bytes(int S, int Hk) {
+  return S < 2048 || S > AttnBf16Smem::MAX_S || Hk <= 0 ? 0 : attn_bf16_ws(S, Hk).total;
+}
 
 int h3_attn_bf16(const void* q, long long ldq, long long hsq, const void* k, long long ldk, long long hsk,
                  const void* v, long long ldv, long long hsv, int S, int Hq, int Hk, const int* span_lo,
@@ -855,6 +857,7 @@ int h3_attn_bf16(const void* q, long long ldq, long long hsq, const void* k, lon
   if (workspace && (!aligned(workspace, 16) || workspace_bytes < h3_attn_bf16_workspace_bytes(S, Hk)))
     return fail(H3_ERR_ARG, "%s: workspace misaligned, or %zu bytes < %zu", who, workspace_bytes,
                 h3_attn_bf16_workspace_bytes(S, Hk));
+  if (!h3_attn_bf16_workspace_bytes(S, Hk)) workspace = nullptr;
   const Rows ro{out, ldo, 128, S, Hq, 128};
   if (meet(ro, {q, ldq, hsq, S, Hq, 128}) || meet(ro, {k, ldk, hsk, S, Hk, 128}) ||
       meet(ro, {v, ldv, hsv, S, Hk, 128}))
@@ -886,14 +889,14 @@ int h3_attn_bf16(const void* q, long long ldq, long long hsq, const void* k, lon
     uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
     AttnBf16Prep pr{reinterpret_cast<const __nv_bfloat16*>(k), ldk, hsk, S, span_lo, span_hi,
                     reinterpret_cast<float*>(ws + w.knorm), reinterpret_cast<float*>(ws + w.knorm1),
-                    reinterpret_cast<int2*>(ws + w.range),
-                    reinterpret_cast<int*>(ws + w.order), reinterpret_cast<int*>(ws + w.next)};
+                    reinterpret_cast<int2*>(ws + w.range), reinterpret_cast<int*>(ws + w.order),
+                    reinterpret_cast<int*>(ws + w.next)};
     attn_bf16_prep_kernel<<<dim3((S + 127) / 128, Hk), 256, 0, S_(stream)>>>(pr);
     if ((rc = check_launch(who))) return rc;
     a.knorm = pr.knorm;
     a.knorm1 = pr.knorm1;
     a.next = pr.next;
-    if (span_lo && a.tile_major && a.rows == 256) {
+    if (span_lo && a.tile_major) {
       cudaError_t e = launch_after(attn_bf16_order_kernel, 1, 1024, 0, S_(stream), pr, a.tiles);
       if (e != cudaSuccess) return fail(H3_ERR_CUDA, "%s: launch: %s", who, cudaGetErrorString(e));
       a.order = pr.order;

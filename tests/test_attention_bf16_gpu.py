@@ -182,6 +182,23 @@ def test_many_short_heads():
     device_ok()
 
 
+def test_a_workspace_where_none_is_needed_is_left_alone():
+    from tfvideo import attention as A
+    from tfvideo import native as N
+
+    S, H = 300, 4
+    q, k, v = packed(S, H, H, 23)
+    out, ws = torch.empty((S, H * 128), dtype=torch.bfloat16, device="cuda"), torch.full((16,), 7, dtype=torch.int32, device="cuda")
+    assert N.attn_bf16_workspace_bytes(S, H) == 0
+    ld, hs = q.stride(2), q.stride(1)
+    rc = N.lib().h3_attn_bf16(q.data_ptr(), ld, hs, k.data_ptr(), ld, hs, v.data_ptr(), ld, hs, S, H, H, None, None,
+                              out.data_ptr(), H * 128, ws.data_ptr(), 0, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    torch.cuda.synchronize()
+    assert (ws == 7).all()
+    assert torch.equal(out.view(S, H, 128).transpose(0, 1)[None], A.bf16(q, k, v))
+
+
 def test_layouts():
     """Head-major memory, separate buffers, unaligned and strided views (copied when TMA cannot read them), shared
     heads as an expanded view: the same bits as contiguous rows."""
