@@ -343,18 +343,20 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
     const int rank = p.tile_major ? n / p.heads : n % p.tiles;
     u.q0 = uniform(p.order ? p.order[rank] : p.tiles - 1 - rank) * p.rows;
   };
-  auto describe = [&](AttnBf16Unit& u) {
+  int lo8[8], hi8[8];   // spans of its rows lane, 32 + lane ..
+  auto spans = [&](const AttnBf16Unit& u) {
     const int q_end = min(u.q0 + p.rows, p.S);
-    int lo[8], hi[8];   // of rows lane, 32 + lane ..
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int query = u.q0 + 32 * i + lane;
-      lo[i] = hi[i] = 0;
+      lo8[i] = hi8[i] = 0;
       if (query < q_end) {
-        lo[i] = p.lo ? p.lo[query] : 0;
-        hi[i] = p.hi ? p.hi[query] : p.S;
+        lo8[i] = p.lo ? p.lo[query] : 0;
+        hi8[i] = p.hi ? p.hi[query] : p.S;
       }
     }
+  };
+  auto describe = [&](AttnBf16Unit& u) {
     u.base = INT_MAX;
     int lo_min[2], hi_max[2];
 #pragma unroll
@@ -362,7 +364,7 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
       int v[4] = {INT_MAX, -1, INT_MAX, -1};
 #pragma unroll
       for (int i = 4 * t; i < 4 * t + 4; ++i) {
-        const int a = max(lo[i], 0), b = min(hi[i], p.S);
+        const int a = max(lo8[i], 0), b = min(hi8[i], p.S);
         if (a < b) {
           v[0] = min(v[0], a);
           v[1] = max(v[1], a);
@@ -404,6 +406,9 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
   };
   AttnBf16Unit first_unit;   // (TMA warp)
   if (warp == 8) {      // the first unit's loads are on their way before the rest is set up
+    wait_primary();     // the preparation's results
+    place(first_unit, blockIdx.x);
+    spans(first_unit);
     if (lane == 0) {
       mbar_init(q_full, 2);
       mbar_init(q_empty, 10);
@@ -421,8 +426,6 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
       fence_barrier_init();
     }
     __syncwarp();
-    wait_primary();   // the preparation's results
-    place(first_unit, blockIdx.x);
     load_q(first_unit);
     describe(first_unit);
     for (int j = 0; j < min(first_unit.steps, 2); ++j) {
@@ -500,6 +503,7 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
         u.q0 = -1;
         if (n < all) {
           place(u, n);
+          spans(u);
           describe(u);
         }
       }
