@@ -238,13 +238,14 @@ int h3_attn_fp8_peers(const void* q, const void* k, const void* v, long long ld,
 /* bf16 attention under per-token key spans: token i attends to the keys [span_lo[i], span_hi[i]) of its head, softmax
  * over those alone (device int32 [S], clipped to [0, S); both NULL: every key).  Packed requests, a prefix with causal
  * or frame-causal tokens behind it and windows are all spans.  A token with an empty span gets zeros.  Keys and values
- * outside a token's span never reach its row, whatever they hold (NaN and infinities included).  Hq query heads share
- * Hk key heads in groups of Hq / Hk.  q, k and v are bf16 views with their own token and head strides (multiples of 8
- * elements, 16-byte aligned), element (t, h, d) at t * ld + h * hs + d; out (t, h, d) at out + t * ldo + h * 128 + d,
- * apart from the inputs (H3_ERR_ARG otherwise).  Scores are scaled by 1 / sqrt(128).  S <= 262,144.  workspace: h3_attn_bf16_workspace_bytes(S, Hk) bytes, 16-byte aligned
- * (0 for short sequences, which use none), one per call in flight: the key norms that let long rows of bounded scores
- * skip their running maximum; NULL is always accepted and only slower.  A key that a row does not see can change that
- * row's rounding, where rows of its 256-row tile see it, but no more.  The reference's backends
+ * outside a token's span never reach its row, whatever they hold (NaN and infinities included); where rows of its
+ * 256-row tile see such a key, it can change the row's rounding, but no more.  Values up to 2^29 (the sums of a long
+ * row of larger ones may overflow).  Hq query heads share Hk key heads in groups of Hq / Hk.  q, k and v are bf16 views
+ * with their own token and head strides (multiples of 8 elements, 16-byte aligned), element (t, h, d) at t * ld +
+ * h * hs + d; out (t, h, d) at out + t * ldo + h * 128 + d, apart from the inputs (H3_ERR_ARG otherwise).  Scores are
+ * scaled by 1 / sqrt(128).  S <= 262,144.  workspace: h3_attn_bf16_workspace_bytes(S, Hk) bytes, 16-byte aligned (0 for
+ * short sequences, which use none), one per call in flight: the key norms that let long rows of bounded scores skip
+ * their running maximum, and the list of tiles; NULL is always accepted and only slower.  The reference's backends
  * (tfvideo/attention.py:29-54) attend to the whole sequence. */
 size_t h3_attn_bf16_workspace_bytes(int S, int Hk);
 int h3_attn_bf16(const void* q, long long ldq, long long hsq, const void* k, long long ldk, long long hsk,

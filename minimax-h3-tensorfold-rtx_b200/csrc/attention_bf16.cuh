@@ -7,18 +7,22 @@
 // maximum m and sum l in 32 bits.  A row without keys gives zeros.  P is rounded to bf16 for the PV MMA (both operands
 // of that MMA have one type, V's); l sums the unrounded P.
 //
-// One CTA = two 128-row query tiles (A, B) of one head over the same 128-key steps.  TMEM: S_A, S_B, O_A, O_B of 128
-// columns each, P written over S.  Warps 0-3: softmax of A, 4-7: of B, a thread per query row with its 128 scores in
-// registers; warp 8: TMA; warps 9 and 10: the MMAs of A and of B; warp 11: guards masked V rows (below).  One tile's
-// MMAs run under the other's softmax.  (One warp issuing both tiles' MMAs was the bottleneck itself: a wait and a
-// commit cost it about 200 cycles each, and P lay ready for 700 of a step's 3,260 cycles.)
+// A unit of work = two 128-row query tiles (A, B) of one head over the same 128-key steps.  TMEM: S_A, S_B, O_A, O_B of
+// 128 columns each, P written over S.  Warps 0-3: softmax of A, 4-7: of B, a thread per query row; warp 8: TMA and the
+// next unit; warps 9 and 10: the MMAs of A and of B; warp 11: guards masked V rows (below).  One tile's MMAs run under
+// the other's softmax.  A CTA takes units from a counter, so that a unit's loads and its first S run under the end of
+// the one before (a CTA for each unit: 8 us of start and end, 162 us against 145 for packed clips of 1 to 2,019 tokens,
+// 40 heads, 4.6 units an SM).
 //
-// A step of both tiles is 4 x 512 cycles of MMA at the bf16 rate, and measures 2,920 cycles: each tile's own chain (S to
-// P to PV and the next S) is what is left once the two take turns.  Exponentials are 2 x 1,024 cycles at 16 a cycle, 5
-// pairs in 16 on the FMA pipe instead.  At 37,760 tokens in two requests, 40 heads: 13.0 ms, 1.12 PFLOP/s, with the SM
-// clock held at 1.5-1.6 GHz by the power limit (a plain bf16 GEMM sustains 1.39 under it).
+// A step of both tiles is 4 x 512 cycles of MMA at the bf16 rate, and measures 2,570: S to P takes 1,490, P to the next S
+// 1,070 (PV of 64 keys, QK, and 300 of waiting and issuing), which is as long as two turns of the tensor core with
+// their 250 cycles of changing hands.  Exponentials are 2 x 1,024 cycles at 16 a cycle, 5 pairs in 16 on the FMA pipe
+// instead.  Measured beside this: 16 softmax warps, two threads a row (147 us for those clips: the same chunk takes
+// 270 cycles a warp with two warps as 316 with one); one warp for both tiles' MMAs (150 us); P handed over whole (147),
+// by quarters (147) or three quarters first (168).  At 37,760 tokens in two requests, 40 heads: 12.1 ms, 1.21 PFLOP/s,
+// with the SM clock held at 1.5-1.6 GHz by the power limit (a plain bf16 GEMM sustains 1.39 under it).
 //
-// Masked keys.  Steps run over the union of the CTA's spans and start at its first key, so documents begin on a step.
+// Masked keys.  Steps run over the union of the unit's spans and start at its first key, so documents begin on a step.
 // Scores of masked keys become -inf before the maximum, whatever K holds there.  V needs more: 0 x NaN is NaN inside
 // the MMA, and another request's rows or the memory behind the last one may hold anything.  In a step that hides some
 // key from some row, warp 11 sets non-finite elements of the V tile to zero and notes the step; the epilogue adds
@@ -161,8 +165,8 @@ constexpr int kAttnBf16Threads = 384;
 // relative rounding does not depend on the factor.
 constexpr float kTauBf16 = 8.0f;
 // Scores are bounded by |q| |k|; while twice that bound is below this (log2 units), a row keeps the maximum of its
-// first step for good: P and l then stay below 2^98, and no later step looks for a maximum (13.5 ms against 14.4, with
-// one MMA warp, at the size above).
+// first step for good: P and l then stay below 2^98 (and O below fp32's range for values to 2^29), and no later step
+// looks for a maximum: 13.5 ms against 14.4, with one MMA warp, at the size above.
 constexpr float kBoundBf16 = 80.0f;
 // pairs of each 32-key chunk whose exp2 runs on the FMA pipe (bit i: keys 2i, 2i + 1)
 constexpr uint32_t kPolyPairsBf16 = 0x2492u;
@@ -555,11 +559,13 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
           const int n = j + 1, g = g0 + j;
           // (also for steps this tile has no part in: a ring slot is free once both warps have let go of it)
           if (j >= 0 && !(ok = __all_sync(~0u, mbar_wait(&v_ok[g % L::VST], (g / L::VST) & 1, 311)))) break;
-          if (n < steps && !(ok = __all_sync(~0u, mbar_wait(&k_full[(g + 1) % L::KST], ((g + 1) / L::KST) & 1, 312)))) break;
+          if (n < steps && !(ok = __all_sync(~0u, mbar_wait(&k_full[(g + 1) % L::KST], ((g + 1) / L::KST) & 1, 312))))
+            break;
           const bool pv = j >= first && j < last, qk = n >= first && n < last;
           // The warps take turns, A first.  Left to themselves the two tiles' MMAs interleave and finish together, and
-          // both softmaxes then wait for both: 4,160 cycles a step, against 2,920 in turns.  (Passing the turn on before
-          // the last MMAs of S are issued, or waiting for P before the turn, settles into unequal halves: 3,220 cycles.)
+          // both softmaxes then wait for both: 4,160 cycles a step, against 2,920 in turns at that time.  (Passing the
+          // turn on before the last MMAs of S are issued: 150 us against 145 for the clips; waiting for P before the
+          // turn: 146.)
           if (t + r0 + n > 0 && !(ok = __all_sync(~0u, mbar_wait(&turn[t], (r0 + n - 1 + t) & 1, 316 + t)))) break;
           if (pv) {
             // O of the unit before is in registers
