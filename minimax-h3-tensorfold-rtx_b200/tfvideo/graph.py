@@ -6,6 +6,8 @@ per block can be recorded once and replayed.  The reference removes its per-call
 the scale read-back into one sync per forward (tfvideo/minimax_h3.py:220-235, tfvideo/linear.py:189-216).  The graph
 reads its inputs from its own static tensors: copy the step's latents into ``graph.x`` and its timestep embedding into
 ``graph.t_emb``, call ``replay()``, and read the result from ``graph.x`` (updated in place, as EngineBlock does).
+The engine's mask and adapters of the time of capture are part of the step and stay so, whatever the engine is given
+later; their tensors may be changed in place.
 
 Single-GPU engines only: the Ulysses path's collectives are not recorded here.
 """
@@ -31,6 +33,7 @@ class StepGraph:
         else:
             self.rope = rope_freqs.detach().to(device=x.device, dtype=torch.float32).contiguous()
         self.mod_segments = mod_segments
+        self._captured = (engine.attn_mask, engine.adapters, engine.adapter_rows)   # the graph reads their memory
         # one eager forward on a scratch copy when the run has none yet, so the captured forward is a delayed-scale
         # one; it also fills the engine's buffers and its row-index cache (nothing is allocated during capture)
         side = torch.cuda.Stream(device=x.device)

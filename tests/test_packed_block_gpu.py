@@ -238,3 +238,25 @@ def test_step_graph_of_a_packed_batch(act):
         out = graph.replay()
         assert torch.equal(out, eager[k]), f"replay {k}"
     device_ok()
+
+
+def test_a_captured_step_keeps_its_mask_and_adapters():
+    from tfvideo import attention as A
+    from tfvideo import graph as G
+
+    eng, cfg, w, x, t_emb, segs, p, m, rows, sets = setup("gelu", layers=2)
+    eng.attn_mask = A.SpanMask(m.lo.clone(), m.hi.clone())
+    eng.set_adapters(sets, rows.clone())
+    eng.forward(x.clone(), t_emb, segs, p)
+    ref = eng.forward(x.clone(), t_emb, segs, p).clone()
+    eng.end_run()
+    eng.forward(x.clone(), t_emb, segs, p)
+    graph = G.StepGraph(eng, x, t_emb, segs, p)
+    eng.set_adapters({}, None)
+    eng.attn_mask = None
+    sets.clear()
+    waste = [torch.full((n,), -1, dtype=torch.int32, device="cuda") for n in (S, 512, 1 << 12, 1 << 16, 1 << 20) * 8]
+    graph.x.copy_(x)
+    assert torch.equal(graph.replay(), ref)
+    del waste
+    device_ok()
