@@ -259,7 +259,7 @@ class AdapterSet:
     def __init__(self, pairs, scales=None, device="cuda"):
         if not pairs:
             raise ValueError("AdapterSet: no adapters")
-        K, N = pairs[0][0].shape[1], pairs[0][1].shape[0]
+        K, N = pairs[0][0].shape[-1], pairs[0][1].shape[0]
         for a, b in pairs:
             if a.dim() != 2 or b.dim() != 2 or a.shape[1] != K or b.shape[0] != N or a.shape[0] != b.shape[1]:
                 raise ValueError(f"AdapterSet: A {tuple(a.shape)} and B {tuple(b.shape)} are not [r, {K}] and [{N}, r]")

@@ -199,6 +199,24 @@ def test_a_workspace_where_none_is_needed_is_left_alone():
     assert torch.equal(out.view(S, H, 128).transpose(0, 1)[None], A.bf16(q, k, v))
 
 
+def test_without_a_workspace():
+    """The C entry takes none for any length: every row then keeps a running maximum, and no CTA has a second tile."""
+
+    from tfvideo import attention as A
+    from tfvideo import native as N
+
+    S, H = 2500, 24
+    q, k, v = packed(S, H, H, 24)
+    m = A.SpanMask.documents([900, 0, 1500], S)
+    out = torch.empty((S, H * 128), dtype=torch.bfloat16, device="cuda")
+    ld, hs = q.stride(2), q.stride(1)
+    rc = N.lib().h3_attn_bf16(q.data_ptr(), ld, hs, k.data_ptr(), ld, hs, v.data_ptr(), ld, hs, S, H, H, m.lo.data_ptr(),
+                              m.hi.data_ptr(), out.data_ptr(), H * 128, None, 0, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    check(out.view(S, H, 128).transpose(0, 1)[None], q, k, v, m.lo, m.hi)
+    device_ok()
+
+
 def test_layouts():
     """Head-major memory, separate buffers, unaligned and strided views (copied when TMA cannot read them), shared
     heads as an expanded view: the same bits as contiguous rows."""

@@ -213,7 +213,7 @@ def test_adapters_refuse_bad_arguments():
                 dict(out=b(1, 64).expand(10, 64)), dict()):                 # the last: CPU tensors
         with pytest.raises(ValueError):
             L.adapter_add(**{**good, **bad})
-    for pairs, scales in (([], None), ([(b(4, 32), b(64, 5))], None), ([(b(4, 32), b(64, 4)), (b(4, 40), b(64, 4))], None),
+    for pairs, scales in (([], None), ([(b(4), b(64, 4))], None), ([(b(4, 32), b(64, 5))], None), ([(b(4, 32), b(64, 4)), (b(4, 40), b(64, 4))], None),
                           ([(b(130, 32), b(64, 130))], None), ([(b(4, 30), b(64, 4))], None), ([(b(4, 32), b(64, 4))], [1, 2])):
         with pytest.raises(ValueError):
             L.AdapterSet(pairs, scales, device="cpu")
