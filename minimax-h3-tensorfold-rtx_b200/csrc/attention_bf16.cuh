@@ -697,33 +697,40 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(q_empty);
-      for (int j = first; j < last; ++j, ++ns) {
+      auto written = [&](int half) {   // P of 64 keys
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * t + half]);
+      };
+      for (int j = first; ok && j < last;) {
+        // nearly every step of a long row: bounded scores, every key visible, 32 scores at a time with the next on their
+        // way (P's words lie over scores that have been read)
+        if (bounded && base + 128 * j >= lo_top && !__any_sync(~0u, m_used == -INFINITY)) {
+          const int end = min(last, (hi_low - base) >> 7);
+          const float nm = -m_used;
+#pragma unroll 1
+          for (; j < end; ++j, ++ns) {
+            if (!(ok = __all_sync(~0u, mbar_wait(&s_full[t], ns & 1, 330 + t)))) break;
+            tc_fence_after();
+            uint32_t s[2][32];
+            tmem_ld32(s_col, s[0]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              tmem_ld_wait();
+              if (c < 3) tmem_ld32(s_col + 32 * (c + 1), s[(c + 1) & 1]);
+              uint32_t pw[16];
+              p_chunk_bf16<true>(s[c & 1], scale2, nm, pw, l2a, l2b);
+              tmem_st16(s_col + 16 * c, pw);
+              if (c & 1) written(c >> 1);
+            }
+          }
+          if (!ok || j >= last) break;
+        }
         const int kb = base + 128 * j;
         if (!(ok = __all_sync(~0u, mbar_wait(&s_full[t], ns & 1, 330 + t)))) break;
         tc_fence_after();
-        auto written = [&](int half) {   // P of 64 keys
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[2 * t + half]);
-        };
         const bool masked = lo_top > kb || hi_low < kb + 128;
-        if (bounded && !masked && !__any_sync(~0u, m_used == -INFINITY)) {
-          // nearly every step of a long row: 32 scores at a time, the next on their way (P's words lie over scores that
-          // have been read)
-          uint32_t s[2][32];
-          tmem_ld32(s_col, s[0]);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            tmem_ld_wait();
-            if (c < 3) tmem_ld32(s_col + 32 * (c + 1), s[(c + 1) & 1]);
-            uint32_t pw[16];
-            p_chunk_bf16<true>(s[c & 1], scale2, -m_used, pw, l2a, l2b);
-            tmem_st16(s_col + 16 * c, pw);
-            if (c & 1) written(c >> 1);
-          }
-          continue;
-        }
         // 64 scores at a time, twice: for the maximum, and for P
         uint32_t s[2][32];
         auto scores = [&](int half) {
@@ -784,6 +791,7 @@ __global__ void __launch_bounds__(kAttnBf16Threads, 1)
           }
           written(half);
         }
+        ++j, ++ns;
       }
       // ---- epilogue: O / l -> bf16, this thread's row
       if (ok && any) ok = __all_sync(~0u, mbar_wait(&o_done[t], no & 1, 332));
