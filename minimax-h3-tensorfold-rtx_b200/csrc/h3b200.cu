@@ -998,12 +998,26 @@ int h3_adapter_add(const void* x, long long ldx, const void* y, long long ldy, c
     a.tile = tile;
     a.total = counters;
     a.perm = perm;
-    if (w.blocks > 1) {   // (one block sets the counters itself)
-      cudaError_t e = cudaMemsetAsync(counters, 0, 8, S_(stream));
-      if (e != cudaSuccess) return fail(H3_ERR_CUDA, "%s: cudaMemsetAsync: %s", who, cudaGetErrorString(e));
+    PlanArgs plan{rows, M, n, tile, counters, counters + 1, perm, w.blocks > 1 && w.blocks <= kPlanCluster};
+    if (plan.cluster) {   // a launch less: such blocks set the counters themselves
+      cudaLaunchAttribute one;
+      one.id = cudaLaunchAttributeClusterDimension;
+      one.val.clusterDim = {(unsigned)w.blocks, 1, 1};
+      cudaLaunchConfig_t pc = {};
+      pc.gridDim = dim3((unsigned)w.blocks);
+      pc.blockDim = dim3(1024);
+      pc.stream = S_(stream);
+      pc.attrs = &one;
+      pc.numAttrs = 1;
+      cudaError_t e = cudaLaunchKernelEx(&pc, adapter_plan_kernel, plan);
+      if (e != cudaSuccess) return fail(H3_ERR_CUDA, "%s: cluster launch: %s", who, cudaGetErrorString(e));
+    } else {
+      if (w.blocks > 1) {   // (one block sets them too)
+        cudaError_t e = cudaMemsetAsync(counters, 0, 8, S_(stream));
+        if (e != cudaSuccess) return fail(H3_ERR_CUDA, "%s: cudaMemsetAsync: %s", who, cudaGetErrorString(e));
+      }
+      adapter_plan_kernel<<<(unsigned)w.blocks, 1024, 0, S_(stream)>>>(plan);
     }
-    adapter_plan_kernel<<<(unsigned)w.blocks, 1024, 0, S_(stream)>>>(
-        PlanArgs{rows, M, n, tile, counters, counters + 1, perm});
     if ((rc = check_launch(who))) return rc;
   }
   // tiles there will be, about
