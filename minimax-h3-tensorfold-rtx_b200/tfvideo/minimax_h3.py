@@ -166,7 +166,7 @@ class MiniMaxH3Engine:
         self._delayed_now = False
         self._buf = None
         self._idx_key = self._idx = None
-        self._rope_key = self._rope = None
+        self._rope_key = self._rope = self._rope_ref = None
         self.clipped = torch.zeros((), dtype=torch.int32, device=self.device)
         self.timer = None                  # a profiling.StageTimer to time each stage of each block
         self.attn_mask = None              # attention.TileMask (fp8) or attention.SpanMask (bf16) when set
@@ -209,7 +209,7 @@ class MiniMaxH3Engine:
 
         if self.on_forward is not None:
             self.on_forward(self, S, transformer_options or {})
-        self._rope_key = None
+        self._rope_key = self._rope = self._rope_ref = None
         delayed = self.delayed_scales and self._forwards > 0
         if delayed and self.sp is not None:
             amax = self.slots[:, 0].contiguous()
@@ -296,10 +296,10 @@ class MiniMaxH3Engine:
         if isinstance(rope_freqs, K.AxialPositions):
             p = self.rope_positions(rope_freqs, S)
             return K.rope_axes(p.pos, p.dims, p.theta)
-        key = (id(rope_freqs), rope_freqs.data_ptr(), rope_freqs._version)
-        if key != self._rope_key:
+        key = self._rope_version(rope_freqs)
+        if self._rope_ref is not rope_freqs or key != self._rope_key:
             self._rope = rope_freqs.reshape(S, -1, 2, 2).to(device=self.device, dtype=torch.float32).contiguous()
-            self._rope_key = key
+            self._rope_key, self._rope_ref = key, rope_freqs
         return self._rope
 
     def rope_positions(self, p: "K.AxialPositions", S: int) -> "K.AxialPositions":
@@ -307,11 +307,18 @@ class MiniMaxH3Engine:
 
         if len(p) != S:
             raise ValueError(f"AxialPositions holds {len(p)} tokens, the sequence has {S}")
-        key = (id(p), p.pos.data_ptr(), p.pos._version)
-        if key != self._rope_key:
-            self._rope, self._rope_ref = p.to(self.device), p
-            self._rope_key = key
+        key = self._rope_version(p.pos)
+        if self._rope_ref is not p or key != self._rope_key:
+            self._rope = p.to(self.device)
+            self._rope_key, self._rope_ref = key, p
         return self._rope
+
+    @staticmethod
+    def _rope_version(t: torch.Tensor) -> tuple:
+        """What tells a change of a table or of positions from one block of a forward to the next (their object is held
+        beside it, so no other takes its id).  Tensors made in inference mode count no versions."""
+
+        return t.data_ptr(), None if t.is_inference() else t._version
 
     def _qknorm_rope(self, b: Block, q, k, ld: int, n: int, H: int, rope_freqs, S: int, t0: int) -> None:
         """q, k RMSNorm + RoPE in place for tokens t0 .. t0 + n (rows of ld elements): from the positions when given,

@@ -1,0 +1,53 @@
+"""What an engine keeps between the blocks of a forward: tables and positions, without a GPU."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+
+def engine():
+    from tfvideo import minimax_h3 as M
+
+    return M.MiniMaxH3Engine([], device="cpu", attn="bf16")
+
+
+def table(S=6):
+    return torch.randn((1, S, 1, 8, 2, 2), generator=torch.Generator().manual_seed(1))
+
+
+def test_positions_and_tables_of_inference_mode():
+    """Tensors made in inference mode count no versions; a sampler's usual ones."""
+
+    from tfvideo import kernels as K
+
+    eng = engine()
+    with torch.inference_mode():
+        pos = torch.arange(12, dtype=torch.int32).view(6, 2)
+        p, t = K.AxialPositions(pos, (8, 8)), table()
+        assert t.is_inference() and p.pos.is_inference()
+        assert torch.equal(eng.rope_positions(p, 6).pos, pos) and eng.rope_positions(p, 6) is eng.rope_positions(p, 6)
+        assert torch.equal(eng.rope_table(t, 6), t.view(6, 8, 2, 2)) and eng.rope_table(t, 6) is eng.rope_table(t, 6)
+    assert torch.equal(eng.rope_positions(p, 6).pos, pos)            # outside it too
+    assert torch.equal(eng.rope_table(t, 6), t.view(6, 8, 2, 2))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_tables_are_kept_by_object_and_version(dtype):
+    """Kept while the same object is handed in unchanged; one changed in place, another in its memory, or one that was
+    refused is not taken for it."""
+
+    eng = engine()
+    t = table().to(dtype)
+    ref = lambda x: x.float().reshape(6, 8, 2, 2)      # noqa: E731
+    first = eng.rope_table(t, 6)
+    assert torch.equal(first, ref(t)) and eng.rope_table(t, 6) is first
+    t.mul_(2)
+    assert torch.equal(eng.rope_table(t, 6), ref(t))
+    for k in range(4):                                 # ids and addresses of freed tables come again
+        other = (table() + k).to(dtype)
+        assert torch.equal(eng.rope_table(other, 6), ref(other))
+        del other
+    with pytest.raises(RuntimeError):
+        eng.rope_table(t[:, :5], 6)
+    assert torch.equal(eng.rope_table(t, 6), ref(t))
