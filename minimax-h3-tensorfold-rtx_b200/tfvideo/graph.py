@@ -6,6 +6,8 @@ per block can be recorded once and replayed.  The reference removes its per-call
 the scale read-back into one sync per forward (tfvideo/minimax_h3.py:220-235, tfvideo/linear.py:189-216).  The graph
 reads its inputs from its own static tensors: copy the step's latents into ``graph.x`` and its timestep embedding into
 ``graph.t_emb``, call ``replay()``, and read the result from ``graph.x`` (updated in place, as EngineBlock does).
+``graph.rope`` is the rotation table or the AxialPositions that replays read: the caller's own memory where it lies on
+the device (a table in contiguous fp32), a copy there otherwise; either may be changed in place between replays.
 The engine's mask and adapters of the time of capture are part of the step and stay so, whatever the engine is given
 later; their tensors may be changed in place.
 
@@ -29,7 +31,7 @@ class StepGraph:
         self.x = x.detach().clone()
         self.t_emb = t_emb.detach().to(device=x.device, dtype=torch.float32).clone()
         if isinstance(rope_freqs, AxialPositions):
-            self.rope = AxialPositions(rope_freqs.pos.detach().to(x.device).clone(), rope_freqs.dims, rope_freqs.theta)
+            self.rope = AxialPositions(rope_freqs.pos.detach().to(x.device), rope_freqs.dims, rope_freqs.theta)
         else:
             self.rope = rope_freqs.detach().to(device=x.device, dtype=torch.float32).contiguous()
         self.mod_segments = mod_segments

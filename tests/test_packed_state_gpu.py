@@ -38,3 +38,28 @@ def test_blocks_and_captured_steps_in_inference_mode(use_table):
         graph.x.copy_(x)
         assert torch.equal(graph.replay(), ref)
     device_ok()
+
+
+@pytest.mark.parametrize("device", ["cuda", "cpu"])
+def test_a_captured_step_follows_positions_changed_in_place(device):
+    """The caller's own tensor where it is on the device, ``graph.rope.pos`` in any case."""
+
+    from tfvideo import graph as G
+
+    eng, cfg, w, x, t_emb, segs, p, m, rows, sets = setup("gelu", layers=2, adapters=False)
+    eng.attn_mask = m
+    p = p.to(device)
+    moved = type(p)(p.pos.roll(7, 0), p.dims, p.theta)
+    eng.forward(x.clone(), t_emb, segs, p)
+    refs = [eng.forward(x.clone(), t_emb, segs, q).clone() for q in (p, moved)]
+    assert not torch.equal(*refs)
+    eng.end_run()
+    eng.forward(x.clone(), t_emb, segs, p)
+    graph = G.StepGraph(eng, x, t_emb, segs, p)
+    if device == "cuda":
+        assert graph.rope.pos.data_ptr() == p.pos.data_ptr()
+    for k, q in enumerate((p.pos.clone(), moved.pos)):
+        (p.pos if device == "cuda" else graph.rope.pos).copy_(q)
+        graph.x.copy_(x)
+        assert torch.equal(graph.replay(), refs[k]), f"replay {k}"
+    device_ok()
