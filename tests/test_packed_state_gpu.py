@@ -63,3 +63,54 @@ def test_a_captured_step_follows_positions_changed_in_place(device):
         graph.x.copy_(x)
         assert torch.equal(graph.replay(), refs[k]), f"replay {k}"
     device_ok()
+
+
+def test_a_captured_step_keeps_buffers_weights_and_rows_index():
+    """Between replays: a forward of another length (the engine drops its buffers), other weights, a mask and adapters
+    that are given other tensors; freed memory is written over each time."""
+
+    from tfvideo import graph as G
+    from tfvideo import minimax_h3 as M
+
+    eng, cfg, w, x, t_emb, segs, p, m, rows, sets = setup("swiglu", layers=2)
+    short = [(0, 128, 3)]
+    x2, p2 = x[:128].clone(), p.rows(0, 128)
+
+    def other_length():
+        mask, ads, r = eng.attn_mask, eng.adapters, eng.adapter_rows
+        eng.attn_mask, eng.adapters, eng.adapter_rows = None, {}, None
+        eng.forward(x2.clone(), t_emb, short, p2)
+        eng.attn_mask, eng.adapters, eng.adapter_rows = mask, ads, r
+
+    def waste():
+        keep = [torch.full((1 << k,), -1, dtype=torch.int8, device="cuda") for k in range(8, 24) for _ in range(8)]
+        keep.append([torch.full((1 << k,), -1, dtype=torch.int32) for k in range(6, 16) for _ in range(8)])
+        torch.cuda.synchronize()
+
+    eng.attn_mask = m
+    eng.set_adapters(sets, rows)
+    refs = []
+    for k in range(4):
+        if k == 2:
+            other_length()
+        refs.append(eng.forward(x.clone(), t_emb, segs, p).clone())
+    eng.end_run()
+    eng.forward(x.clone(), t_emb, segs, p)
+    graph = G.StepGraph(eng, x, t_emb, list(segs), p)     # (a list no forward has seen)
+    assert torch.equal(graph.replay(), refs[1])
+    other_length()
+    waste()
+    graph.x.copy_(x)
+    assert torch.equal(graph.replay(), refs[2])
+    spare = M.MiniMaxH3Engine.from_weights(M.synthetic_weights(cfg, seed=9, device="cuda"), cfg, device="cuda", attn="bf16")
+    eng.replace_blocks(spare.blocks, slots=spare.slots)
+    m.lo, m.hi = m.lo * 0, m.hi * 0
+    for ad in sets.values():
+        ad.A, ad.B, ad.scale = ad.A * 0, ad.B * 0, ad.scale * 0
+    eng.set_adapters({}, None)
+    eng.attn_mask, eng._idx, eng._idx_key, eng._idx_ref = None, None, None, None
+    eng.release_vram()
+    waste()
+    graph.x.copy_(x)
+    assert torch.equal(graph.replay(), refs[3])
+    device_ok()
