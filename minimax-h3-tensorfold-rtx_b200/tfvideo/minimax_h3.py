@@ -166,7 +166,7 @@ class MiniMaxH3Engine:
         self._delayed_now = False
         self._buf = None
         self._idx_key = self._idx = None
-        self._rope_key = self._rope = self._rope_ref = None
+        self._rope_key = self._rope = self._rope_ref = self._rope_made = None
         self.clipped = torch.zeros((), dtype=torch.int32, device=self.device)
         self.timer = None                  # a profiling.StageTimer to time each stage of each block
         self.attn_mask = None              # attention.TileMask (fp8) or attention.SpanMask (bf16) when set
@@ -209,7 +209,7 @@ class MiniMaxH3Engine:
 
         if self.on_forward is not None:
             self.on_forward(self, S, transformer_options or {})
-        self._rope_key = self._rope = self._rope_ref = None
+        self._rope_key = self._rope = self._rope_ref = self._rope_made = None
         delayed = self.delayed_scales and self._forwards > 0
         if delayed and self.sp is not None:
             amax = self.slots[:, 0].contiguous()
@@ -269,7 +269,7 @@ class MiniMaxH3Engine:
         return ad
 
     def release_vram(self):
-        self._buf = None
+        self._buf = self._rope_made = None
         torch.cuda.empty_cache()
 
     def row_index(self, mod_segments, S: int) -> torch.Tensor:
@@ -290,12 +290,14 @@ class MiniMaxH3Engine:
         return self._idx
 
     def rope_table(self, rope_freqs, S: int) -> torch.Tensor:
-        """fp32 [S, rot/2, 2, 2] from ComfyUI's [1, S, 1, rot/2, 2, 2] rotation table (cached within a forward), or
-        made from a kernels.AxialPositions."""
+        """fp32 [S, rot/2, 2, 2] from ComfyUI's [1, S, 1, rot/2, 2, 2] rotation table, or made from a
+        kernels.AxialPositions (either cached within a forward)."""
 
         if isinstance(rope_freqs, K.AxialPositions):
             p = self.rope_positions(rope_freqs, S)
-            return K.rope_axes(p.pos, p.dims, p.theta)
+            if self._rope_made is None or self._rope_made[0] is not p:
+                self._rope_made = p, K.rope_axes(p.pos, p.dims, p.theta)
+            return self._rope_made[1]
         key = self._rope_version(rope_freqs)
         if self._rope_ref is not rope_freqs or key != self._rope_key:
             self._rope = rope_freqs.reshape(S, -1, 2, 2).to(device=self.device, dtype=torch.float32).contiguous()

@@ -51,3 +51,28 @@ def test_tables_are_kept_by_object_and_version(dtype):
     with pytest.raises(RuntimeError):
         eng.rope_table(t[:, :5], 6)
     assert torch.equal(eng.rope_table(t, 6), ref(t))
+
+
+def test_an_override_table_is_made_once_a_forward(monkeypatch):
+    """Attention overrides of every block are handed one table; positions changed in place, or others, make a new one."""
+
+    from tfvideo import kernels as K
+
+    made = []
+
+    def rope_axes(pos, dims, theta):
+        made.append(pos.clone())
+        return torch.full((pos.shape[0], 8, 2, 2), float(len(made)))
+
+    monkeypatch.setattr(K, "rope_axes", rope_axes)
+    eng = engine()
+    p = K.AxialPositions(torch.arange(12, dtype=torch.int32).view(6, 2), (8, 8))
+    first = eng.rope_table(p, 6)
+    assert eng.rope_table(p, 6) is first and eng.rope_positions(p, 6).pos is p.pos and eng.rope_table(p, 6) is first
+    p.pos.add_(1)
+    assert eng.rope_table(p, 6) is not first and len(made) == 2 and torch.equal(made[1], p.pos)
+    q = K.AxialPositions(p.pos, (8, 8), 50.0)
+    assert eng.rope_table(q, 6) is not eng.rope_table(p, 6) and len(made) == 4
+    eng._rope_key = None                               # as a new forward does
+    t = table()
+    assert torch.equal(eng.rope_table(t, 6), t.view(6, 8, 2, 2))

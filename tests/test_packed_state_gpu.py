@@ -114,3 +114,27 @@ def test_a_captured_step_keeps_buffers_weights_and_rows_index():
     graph.x.copy_(x)
     assert torch.equal(graph.replay(), refs[3])
     device_ok()
+
+
+def test_overrides_of_a_forward_share_one_table():
+    from tfvideo import minimax_h3 as M
+
+    eng, cfg, w, x, t_emb, segs, p, m, rows, sets = setup("gelu", layers=2, adapters=False)
+    blocks = [M.EngineBlock(eng, i) for i in range(2)]
+    seen = []
+
+    def override(h, rope_freqs, transformer_options):
+        seen.append(rope_freqs.clone())
+        at.append(rope_freqs.data_ptr())
+        return torch.zeros_like(h)
+
+    for moved in range(2):
+        if moved:
+            p.pos.copy_(p.pos.roll(3, 0))
+        at, y = [], x.clone()
+        for b in blocks:
+            y = b(y, t_emb, segs, p, attention=override)
+        assert at[0] == at[1]
+        assert torch.equal(seen[-1], p.table()) and torch.equal(seen[-2], p.table())
+    assert not torch.equal(seen[0], seen[2])
+    device_ok()
