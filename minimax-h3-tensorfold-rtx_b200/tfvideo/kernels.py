@@ -27,11 +27,9 @@ HEAD_DIM = 128
 
 
 @lru_cache(maxsize=64)
-def _axes(what: str, dims: tuple, theta) -> tuple:
-    """Validated (dims, theta per axis, rot, the two as H3Positions holds them)."""
+def _axes(what: str, dims: tuple, theta: tuple) -> tuple:
+    """Validated (dims, theta per axis, rot, the two as H3Positions holds them) of plain numbers."""
 
-    dims = tuple(int(d) for d in dims)
-    theta = tuple(float(t) for t in theta) if isinstance(theta, tuple) else (float(theta),) * len(dims)
     if not 1 <= len(dims) <= 4 or len(theta) != len(dims):
         raise ValueError(f"{what}: 1 to 4 axes and one theta for each or for all, got dims {dims}, theta {theta}")
     if any(d <= 0 or d % 2 for d in dims) or sum(dims) > HEAD_DIM:
@@ -43,7 +41,9 @@ def _axes(what: str, dims: tuple, theta) -> tuple:
 
 
 def _check_positions(what: str, pos: torch.Tensor, dims, theta) -> tuple:
-    axes = _axes(what, tuple(dims), tuple(theta) if isinstance(theta, (list, tuple)) else theta)
+    # (as plain numbers: a tensor among them would be known by its identity, whatever it comes to hold)
+    dims = tuple(map(int, dims))
+    axes = _axes(what, dims, tuple(map(float, theta)) if isinstance(theta, (list, tuple)) else (float(theta),) * len(dims))
     if pos.dim() != 2 or pos.dtype not in N.POS_TYPES or pos.shape[1] != len(axes[0]):
         raise ValueError(f"{what}: pos must be an int32, int64 or fp32 [S, {len(axes[0])}] tensor, got "
                          f"{tuple(pos.shape)} {pos.dtype}")

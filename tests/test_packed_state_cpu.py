@@ -1,4 +1,4 @@
-"""What an engine keeps between the blocks of a forward: tables and positions, without a GPU."""
+"""What the packed-batch operators and an engine keep between calls (tables, positions, checked arguments), without a GPU."""
 
 from __future__ import annotations
 
@@ -76,3 +76,26 @@ def test_an_override_table_is_made_once_a_forward(monkeypatch):
     eng._rope_key = None                               # as a new forward does
     t = table()
     assert torch.equal(eng.rope_table(t, 6), t.view(6, 8, 2, 2))
+
+
+def test_theta_and_dims_are_taken_by_their_values():
+    """Tensors and numpy numbers in place of plain ones: as they are when the call is made."""
+
+    import numpy as np
+    from tfvideo import kernels as K
+
+    pos = torch.zeros((10, 2), dtype=torch.int32)
+    theta, dim = torch.tensor(10000.0), torch.tensor(16)
+    for t in (theta, (theta, theta), [theta, 10000.0]):
+        theta.fill_(10000.0), dim.fill_(16)
+        p = K.AxialPositions(pos, (dim, 16), t)
+        assert p.theta == (10000.0, 10000.0) and p.dims == (16, 16) and p.rot == 32
+        theta.fill_(50.0), dim.fill_(32)
+        p = K.AxialPositions(pos, (dim, 16), t)
+        assert p.theta[0] == 50.0 and p.dims == (32, 16) and all(type(x) is float for x in p.theta)
+        axes = K._check_positions("rope_axes", pos, (dim, 16), t)
+        assert axes[3][0] == 32 and axes[4][0] == 50.0
+    p = K.AxialPositions(pos, np.array([16, 24]), np.float32(256))
+    assert p.dims == (16, 24) and p.theta == (256.0, 256.0)
+    with pytest.raises(ValueError, match="theta"):
+        K.AxialPositions(pos, (16, 16), (10000.0,))
