@@ -566,6 +566,7 @@ __global__ void __launch_bounds__(448)
         kind = any ? 2 : !a.inplace;
       }
       if (!ok) break;
+      __syncwarp();   // every lane's rows_s before lane 0 lets the other warps read them
       if (lane == 0) {
         unit_s[b] = unit < units ? unit : -1;
         kind_s[b] = kind;
