@@ -25,7 +25,7 @@ namespace h3 {
 struct AdapterArgs {
   const int* rows;      // [M]
   const float* scale;   // [n], or NULL: 1
-  __nv_bfloat16* t;     // [tiles, 128, Rp]
+  __nv_bfloat16* t;     // [M, Rp]: a tile's rows from its first place in perm on (without a plan, from its first row)
   const __nv_bfloat16 *x, *y;
   __nv_bfloat16* out;
   long long ldx, ldy, ldo;
@@ -383,9 +383,11 @@ __global__ void __launch_bounds__(192)
           uint32_t w[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) w[e] = pack_bf16(__uint_as_float(v[2 * e]) * sc, __uint_as_float(v[2 * e + 1]) * sc);
-          uint4* d = reinterpret_cast<uint4*>(a.t + ((size_t)blockIdx.x * 128 + row) * a.Rp + c);
-          d[0] = make_uint4(w[0], w[1], w[2], w[3]);
-          d[1] = make_uint4(w[4], w[5], w[6], w[7]);
+          if (row < tile.count) {   // (the rows behind are the next tile's)
+            uint4* d = reinterpret_cast<uint4*>(a.t + ((size_t)tile.begin + row) * a.Rp + c);
+            d[0] = make_uint4(w[0], w[1], w[2], w[3]);
+            d[1] = make_uint4(w[4], w[5], w[6], w[7]);
+          }
         }
       }
     }
@@ -398,6 +400,7 @@ __global__ void __launch_bounds__(192)
     const float sc = a.scale ? a.scale[tile.adapter] : 1.0f;
     for (int i = threadIdx.x; i < per * pieces; i += 192) {
       const int row = blockIdx.y * per + i / pieces, c = (i % pieces) * 8;
+      if (row >= tile.count) break;
       float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       for (int s = 0; s < splits; ++s) {
         const uint32_t at = cluster_addr(red + row * L::red_row(a.Rp) + c * 4, s);
@@ -405,7 +408,7 @@ __global__ void __launch_bounds__(192)
         f[0] += u.x; f[1] += u.y; f[2] += u.z; f[3] += u.w;
         f[4] += v.x; f[5] += v.y; f[6] += v.z; f[7] += v.w;
       }
-      *reinterpret_cast<uint4*>(a.t + ((size_t)blockIdx.x * 128 + row) * a.Rp + c) =
+      *reinterpret_cast<uint4*>(a.t + ((size_t)tile.begin + row) * a.Rp + c) =
           make_uint4(pack_bf16(f[0] * sc, f[1] * sc), pack_bf16(f[2] * sc, f[3] * sc), pack_bf16(f[4] * sc, f[5] * sc),
                      pack_bf16(f[6] * sc, f[7] * sc));
     }
@@ -583,8 +586,8 @@ __global__ void __launch_bounds__(448)
         const int st = nt % nts;
         if (!(ok = __all_sync(~0u, mbar_wait(&t_empty[st], ((nt / nts) & 1) ^ 1, 452)))) break;
         mbar_arrive_expect_tx(&t_full[st], kc * L::SUB);
-        const int t0 = unit_s[b] / strips * 128;
-        for (int c = 0; c < kc; ++c) tma_load_3d(ts + (st * kc + c) * L::SUB, &tmT, 64 * c, t0, 0, &t_full[st]);
+        // (with rows of the next tiles, whose products are not used; zeros past the last)
+        for (int c = 0; c < kc; ++c) tma_load_3d(ts + (st * kc + c) * L::SUB, &tmT, 64 * c, tile.begin, 0, &t_full[st]);
         ++nt;
       }
       for (int x = x0; ok && x < x1 && kind > 0; ++x) {

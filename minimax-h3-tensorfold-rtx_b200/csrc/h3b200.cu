@@ -931,7 +931,7 @@ AdapterWs adapter_ws(int M, int R, int n) {
   w.tile = 16;
   w.perm = w.tile + (n == 1 ? 0 : (size_t)w.tiles * 16);
   w.t = align_up(w.perm + (n == 1 ? 0 : (size_t)M * 4), 16);
-  w.total = w.t + (size_t)w.tiles * 128 * ((R + 15) / 16 * 16) * 2;
+  w.total = w.t + (size_t)M * ((R + 15) / 16 * 16) * 2;
   return w;
 }
 }  // namespace
@@ -968,7 +968,7 @@ int h3_adapter_add(const void* x, long long ldx, const void* y, long long ldy, c
   if ((rc = make_map_bf16(&ta, A, K, R, n, K, (long long)R * K, Rp, who))) return rc;
   if ((rc = make_map_bf16(&ty, y, N, M, 1, ldy, 0, 128, who))) return rc;
   uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
-  if ((rc = make_map_bf16(&tt, ws + w.t, Rp, w.tiles * 128, 1, Rp, 0, 128, who))) return rc;
+  if ((rc = make_map_bf16(&tt, ws + w.t, Rp, M, 1, Rp, 0, 128, who))) return rc;
   if ((rc = make_map_bf16(&tb, B, R, N, n, R, (long long)N * R, 128, who))) return rc;
   if ((rc = make_map_bf16(&to, out, N, M, 1, ldo, 0, 32, who))) return rc;
   if ((rc = smem_optin(adapter_shrink_kernel, 232448, &g_optin_shrink, who))) return rc;

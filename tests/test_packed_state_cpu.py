@@ -99,3 +99,19 @@ def test_theta_and_dims_are_taken_by_their_values():
     assert p.dims == (16, 24) and p.theta == (256.0, 256.0)
     with pytest.raises(ValueError, match="theta"):
         K.AxialPositions(pos, (16, 16), (10000.0,))
+
+
+@pytest.mark.parametrize("M", [1, 10, 333, 4096, 37_760])
+@pytest.mark.parametrize("R", [8, 64, 128])
+@pytest.mark.parametrize("n", [1, 2, 100, 1000, 1 << 20])
+def test_adapter_workspace_goes_by_the_rows(M, R, n):
+    """A x of every row (its rank rounded up to 16, bf16), and 20 bytes a row of lists at the most, however many adapters
+    are registered."""
+
+    from tfvideo import native
+    if not native.LIB_PATH.exists():
+        from build import build
+        build()
+    size = native.lib().h3_adapter_workspace_bytes(M, R, n)
+    t = M * ((R + 15) // 16 * 16) * 2
+    assert t <= size <= t + 20 * M + 64

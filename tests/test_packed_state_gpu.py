@@ -138,3 +138,25 @@ def test_overrides_of_a_forward_share_one_table():
         assert torch.equal(seen[-1], p.table()) and torch.equal(seen[-2], p.table())
     assert not torch.equal(seen[0], seen[2])
     device_ok()
+
+
+@pytest.mark.parametrize("M,R,n", [(700, 16, 64), (4500, 40, 2000), (9000, 128, 3)])
+def test_adapter_calls_write_nothing_behind_their_workspace(M, R, n):
+    """A tile's part of the workspace ends with its rows: calls whose workspace has a guard behind it, and whose memory
+    held NaN before, give what others do."""
+
+    from tfvideo import linear as L
+    from tfvideo import native as N
+    from test_adapter_gpu import check, make
+
+    x, y, A, B, rows, scale = make(M, 136, 264, R, n, seed=M, kind="any")
+    ref = L.adapter_add(y, x, A, B, rows, scale, out=torch.empty_like(y))
+    check(ref, x, y, A, B, rows, scale)
+    size = N.adapter_workspace_bytes(M, R, n)
+    for fill in (0xFF, 0x7F):
+        ws = torch.full((size + 4096,), fill, dtype=torch.uint8, device="cuda")
+        out = torch.empty_like(y)
+        N.launch(0, "h3_adapter_add", 3, x.data_ptr(), 136, y.data_ptr(), 264, A.data_ptr(), B.data_ptr(),
+                 scale.data_ptr(), rows.data_ptr(), M, 136, 264, R, n, out.data_ptr(), 264, ws.data_ptr(), size)
+        assert torch.equal(out, ref) and (ws[size:] == fill).all()
+    device_ok()
