@@ -241,23 +241,22 @@ class MiniMaxH3Engine:
         """Low-rank adapters beside the block linears, a different one for each request of the packed sequence:
         ``adapters[(block, name)]`` is the linear.AdapterSet of block linear ``name`` (qkv, out, fc1, fc2; fc1 of a SwiGLU
         model with [gate | up] outputs), ``rows`` int32 [S] each token's adapter in those sets (outside them: none).  They
-        stay until ``set_adapters({}, None)``; ``rows`` is read on the device, so it may be changed in place.  Against
-        merged weights (store.load_or_convert): no re-conversion, and as many sets at once as there are requests."""
+        stay until ``set_adapters({}, None)``; the sets and ``rows`` are read on the device in every forward, so they may be
+        changed in place.  Against merged weights (store.load_or_convert): no re-conversion, and as many sets at once as
+        there are requests."""
 
         if adapters and self.sp is not None:
             raise ValueError("set_adapters: sequence-parallel engines run without adapters; merge them instead")
         if adapters and (not torch.is_tensor(rows) or rows.dim() != 1 or rows.dtype != torch.int32
                          or not rows.is_contiguous()):
             raise ValueError("set_adapters: rows must be a contiguous int32 [S] tensor")
-        laid_out = {}
         for (i, name), ad in adapters.items():
             if not 0 <= i < len(self.blocks) or name not in LIN_NAMES:
                 raise ValueError(f"set_adapters: no linear {name!r} in block {i}")
             lin = self.blocks[i].lins[name]
             if (ad.n, ad.k) != (lin.n, lin.k):
                 raise ValueError(f"set_adapters: block {i} {name} is [{lin.n}, {lin.k}], its adapters [{ad.n}, {ad.k}]")
-            laid_out[(i, name)] = ad.interleaved16() if lin.interleaved else ad
-        self.adapters = laid_out
+        self.adapters = dict(adapters)
         self.adapter_rows = rows.to(self.device) if adapters else None
 
     def _adapter(self, i: int, name: str, S: int):
@@ -586,8 +585,8 @@ class MiniMaxH3Engine:
             u = buf.projection(n, cfg.fc1_out, self.device)
             with maybe(T, "gemm_store"):
                 l1.gemm(buf.h4, buf.h4sf, n, N.H3Epilogue(kind=N.H3_EPI_STORE, out=u.data_ptr(), ldo=cfg.fc1_out))
-            with maybe(T, "adapters"):
-                ad1.add(u, h, self.adapter_rows)
+            with maybe(T, "adapters"):   # (B laid out anew each time, so that it may be changed in place)
+                (ad1.interleaved16() if l1.interleaved else ad1).add(u, h, self.adapter_rows)
             with maybe(T, "act+quant"):
                 N.act(u, a, N.ACT_SWIGLU16 if l1.interleaved else act_kind, s2)
         elif delayed:

@@ -160,3 +160,48 @@ def test_adapter_calls_write_nothing_behind_their_workspace(M, R, n):
                  scale.data_ptr(), rows.data_ptr(), M, 136, 264, R, n, out.data_ptr(), 264, ws.data_ptr(), size)
         assert torch.equal(out, ref) and (ws[size:] == fill).all()
     device_ok()
+
+
+@pytest.mark.parametrize("act", ["gelu", "swiglu"])
+def test_adapters_changed_in_place(act):
+    """Weights and scales of each linear's set, changed in place after set_adapters: forwards and replays use them.  The
+    changes are by powers of two, which bf16 takes back without a rounding."""
+
+    from tfvideo import graph as G
+    from tfvideo import linear as L
+
+    eng, cfg, w, x, t_emb, segs, p, m, rows, sets = setup(act)
+    eng.attn_mask = m
+
+    def forwards(ads):
+        eng.set_adapters(ads, rows)
+        eng.end_run()
+        eng.forward(x.clone(), t_emb, segs, p)
+        return eng.forward(x.clone(), t_emb, segs, p).clone()
+
+    def copy(ad):
+        c = L.AdapterSet.__new__(L.AdapterSet)
+        c.n, c.k, c.count, c.A, c.B, c.scale = ad.n, ad.k, ad.count, ad.A.clone(), ad.B.clone(), ad.scale.clone()
+        return c
+
+    forwards(sets)
+    eng.end_run()
+    eng.forward(x.clone(), t_emb, segs, p)
+    graph = G.StepGraph(eng, x, t_emb, segs, p)
+    for name in ("qkv", "out", "fc1", "fc2"):
+        for what in ("A", "B", "scale"):
+            before = forwards({k: copy(ad) for k, ad in sets.items()})
+            getattr(sets[0, name], what).mul_(-2)
+            ref = forwards({k: copy(ad) for k, ad in sets.items()})
+            assert not torch.equal(ref, before)
+            eng.set_adapters(sets, rows)               # (as they are now; the next change is made behind it)
+            getattr(sets[0, name], what).mul_(-0.5)
+            eng.end_run()
+            eng.forward(x.clone(), t_emb, segs, p)
+            assert torch.equal(eng.forward(x.clone(), t_emb, segs, p), before), (name, what)
+            getattr(sets[0, name], what).mul_(-2)
+            eng.end_run()
+            eng.forward(x.clone(), t_emb, segs, p)
+            graph.x.copy_(x)
+            assert torch.equal(graph.replay(), ref), (name, what)
+    device_ok()
