@@ -171,7 +171,7 @@ class MiniMaxH3Engine:
         self.timer = None                  # a profiling.StageTimer to time each stage of each block
         self.attn_mask = None              # attention.TileMask (fp8) or attention.SpanMask (bf16) when set
         self.adapters = {}                 # (block, linear name) -> linear.AdapterSet (set_adapters)
-        self.adapter_rows = None           # int32 [S]: each token's adapter
+        self.adapter_rows = None           # int32 [S] on the device: each token's adapter (set_adapters)
         self.qkv_parts = 4                 # Ulysses: row parts of the qkv GEMM (all but the last sent by copy engines)
         self.copy_streams = 7              # Ulysses: side streams for those copies (one per destination rank at 8)
         self.part_sender = "auto"          # Ulysses: "copy" (copy engines), "push" (a push kernel beside the GEMM),
@@ -242,8 +242,9 @@ class MiniMaxH3Engine:
         ``adapters[(block, name)]`` is the linear.AdapterSet of block linear ``name`` (qkv, out, fc1, fc2; fc1 of a SwiGLU
         model with [gate | up] outputs), ``rows`` int32 [S] each token's adapter in those sets (outside them: none).  They
         stay until ``set_adapters({}, None)``; the sets and ``rows`` are read on the device in every forward, so they may be
-        changed in place.  Against merged weights (store.load_or_convert): no re-conversion, and as many sets at once as
-        there are requests."""
+        changed in place (``rows`` given on another device are copied: ``engine.adapter_rows`` is what forwards read).
+        Against merged weights (store.load_or_convert): no re-conversion, and as many sets at once as there are requests.
+        """
 
         if adapters and self.sp is not None:
             raise ValueError("set_adapters: sequence-parallel engines run without adapters; merge them instead")

@@ -205,3 +205,28 @@ def test_adapters_changed_in_place(act):
             graph.x.copy_(x)
             assert torch.equal(graph.replay(), ref), (name, what)
     device_ok()
+
+
+def test_rows_given_on_the_host():
+    """A copy of them is what forwards read: ``engine.adapter_rows``, which may be changed in place."""
+
+    eng, cfg, w, x, t_emb, segs, p, m, rows, sets = setup("gelu")
+    eng.attn_mask = m
+
+    def second():
+        eng.end_run()
+        eng.forward(x.clone(), t_emb, segs, p)
+        return eng.forward(x.clone(), t_emb, segs, p).clone()
+
+    eng.set_adapters(sets, rows)
+    assert eng.adapter_rows is rows
+    ref = second()
+    rows.copy_(rows.roll(50))
+    moved = second()
+    assert not torch.equal(moved, ref)
+    host = rows.roll(-50).cpu()
+    eng.set_adapters(sets, host)
+    assert torch.equal(second(), ref)
+    eng.adapter_rows.copy_(rows)
+    assert torch.equal(second(), moved)
+    device_ok()
