@@ -193,7 +193,8 @@ def bf16_tokens(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Te
                          f"{tuple(out.shape)}: bf16 [S, H, {HEAD_DIM}] rows and [S, Hq * {HEAD_DIM}], query heads a "
                          "multiple of the key heads")
     (S, Hq, _), Hk = q.shape, k.shape[1]
-    _bf16_launch(S, Hq, Hk, q, q.stride(), k, k.stride(), v, v.stride(), out, out.stride(0), mask)
+    ldo = out.stride(0) if S > 1 else out.shape[1]      # (one row: any stride)
+    _bf16_launch(S, Hq, Hk, q, q.stride(), k, k.stride(), v, v.stride(), out, ldo, mask)
     return out
 
 

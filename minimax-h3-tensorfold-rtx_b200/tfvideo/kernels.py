@@ -92,6 +92,8 @@ def qknorm_rope_axes(q: torch.Tensor, k: torch.Tensor, qw: torch.Tensor, kw: tor
         ld, hs, ds = t.stride()
         at = t.data_ptr()
         if ds != 1 or ld & 3 or hs & 3 or at & 7:
+            ld, hs = ld if t.shape[0] > 1 else 0, hs if t.shape[1] > 1 else 0   # (of one entry: any)
+        if ds != 1 or ld & 3 or hs & 3 or at & 7:
             raise ValueError("qknorm_rope_axes: q, k and their outputs need a contiguous head dim and 8-byte aligned rows, "
                              f"got strides {t.stride()}")
         st += (at, ld, hs)

@@ -227,14 +227,18 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tens
     if K & 7 or cols & 7 or R & 7 or R > 128 or n > 1 << 20:
         raise ValueError("adapter_add: K, N and R must be multiples of 8, R at most 128 and n at most 2^20, got "
                          f"K={K} N={cols} R={R} n={n}")
+    lds = []
     for name, t in (("y", y), ("out", out)) if out is not y else (("y", y),):
         ld, cs = t.stride()
+        if M == 1:          # (a dimension of one entry has any stride)
+            ld = cols
         if (cols > 1 and cs != 1) or ld & 7 or (M > 1 and ld < cols) or t.data_ptr() & 15:
             raise ValueError(f"adapter_add: {name} needs 16-byte aligned contiguous rows, got strides {t.stride()}")
+        lds.append(ld)
     ldx, cs = x.stride()
     if cs != 1 or ldx & 7 or ldx < K or x.data_ptr() & 15:
         x = N.aligned16(x)
-        ldx = x.stride(0)
+        ldx = K
     A, B, rows = N.aligned16(A), N.aligned16(B), rows.contiguous()
     if scale is None:
         dev = N.one_device("adapter_add", y, x, A, B, rows, out)
@@ -244,9 +248,9 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tens
     if M and cols and n and K and R:
         size = N.adapter_workspace_bytes(M, R, n)
         ws = x.new_empty(size // 2)
-        N.launch(dev, "h3_adapter_add", 2 if n == 1 else 3, x.data_ptr(), ldx, y.data_ptr(), y.stride(0), A.data_ptr(),
+        N.launch(dev, "h3_adapter_add", 2 if n == 1 else 3, x.data_ptr(), ldx, y.data_ptr(), lds[0], A.data_ptr(),
                  B.data_ptr(), None if scale is None else scale.data_ptr(), rows.data_ptr(), M, K, cols, R, n,
-                 out.data_ptr(), out.stride(0), ws.data_ptr(), size)
+                 out.data_ptr(), lds[-1], ws.data_ptr(), size)
     elif out is not y:
         out.copy_(y)
     return out
