@@ -462,8 +462,11 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 // relative-error least-squares fit on [-1/2, 1/2]; max relative error 7.5e-5, below the e4m3 rounding P gets next
 // by three orders of magnitude).  n comes from the magic-number rounding x + (1.5 * 2^23 + 127): the sum's low
 // mantissa bits hold 127 + n, which shifted into the exponent field is the fp32 2^n.  x is clamped to >= -126.
-__device__ __forceinline__ uint64_t exp2_poly_clamped(uint64_t x) {   // x >= -126 (or NaN)
+__device__ __forceinline__ uint64_t exp2_poly_pair(uint64_t x2) {
   constexpr float kMagic = 12582912.0f + 127.0f;
+  float a, b;
+  f32x2_unpack(x2, a, b);
+  const uint64_t x = f32x2_pack(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
   const uint64_t t = add2(x, f32x2_splat(kMagic));
   const uint64_t n = add2(t, f32x2_splat(-kMagic));
   const uint64_t g = fma2(n, f32x2_splat(-1.0f), x);
@@ -473,11 +476,6 @@ __device__ __forceinline__ uint64_t exp2_poly_clamped(uint64_t x) {   // x >= -1
   float t0, t1;
   f32x2_unpack(t, t0, t1);
   return mul2(p, f32x2_pack(__uint_as_float(__float_as_uint(t0) << 23), __uint_as_float(__float_as_uint(t1) << 23)));
-}
-__device__ __forceinline__ uint64_t exp2_poly_pair(uint64_t x2) {
-  float a, b;
-  f32x2_unpack(x2, a, b);
-  return exp2_poly_clamped(f32x2_pack(fmaxf(a, -126.0f), fmaxf(b, -126.0f)));
 }
 __device__ __forceinline__ uint64_t exp2_mufu_pair(uint64_t x2) {
   float a, b;

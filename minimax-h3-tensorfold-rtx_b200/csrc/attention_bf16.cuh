@@ -178,7 +178,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // NaN when eithe
 }
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1u); }
 
-// 2^x for a pair whose results are normal numbers: exp2_poly_clamped's polynomial, without its clamp, and the exponent
+// 2^x for a pair whose results are normal numbers: exp2_poly_pair's polynomial, without its clamp, and the exponent
 // raised by an integer addition.
 __device__ __forceinline__ uint64_t exp2_poly_normal(uint64_t x) {
   constexpr float kMagic = 12582912.0f;                                     // 1.5 * 2^23: the sum's low bits are round(x)

@@ -38,10 +38,10 @@ __device__ __forceinline__ void fence_barrier_init() {
 // elect.sync inside the instruction sequence picks the one lane that issues.  The operands then stay in warp-uniform
 // registers: issuing the same instructions from a lane-0 branch instead costs tens of cycles each (a tcgen05.mma
 // from a lane-0 branch takes ~60 cycles to issue, from the whole warp ~7), which starves the tensor pipe.
+#define H3_ELECT "elect.sync rx|e, 0xffffffff;\n\t"
 // A value that all lanes hold, such as a warp's index or one read from shared memory, as the compiler can know it: an
 // operand that it takes for a lane's own costs a move to a uniform register at every issue.
 __device__ __forceinline__ int uniform(int x) { return __reduce_max_sync(~0u, x); }
-#define H3_ELECT "elect.sync rx|e, 0xffffffff;\n\t"
 // warp-wide: one arrival that also expects `bytes` of transaction data
 __device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t* bar, uint32_t bytes) {
   asm volatile("{\n\t.reg .pred e;\n\t.reg .b32 rx;\n\t" H3_ELECT
