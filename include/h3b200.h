@@ -116,7 +116,8 @@ int h3_nvfp4_quant(const void* x, long long ldx, int cblk, long long blk_stride,
 int h3_gate_add(void* x, int ldx, const void* y, int ldy, const float* mod, const int* idx, int S, int D, int part,
                 void* stream);
 /* act_kind 0: gelu_tanh(u) (u [M, F]); 1: silu(gate) * up (u = [gate | up] [M, 2F]) (replaces kernels.swiglu,
- * tfvideo/kernels.py:66-84); 2: the same from 16 gate and 16 up columns in turn (F % 16 == 0); bf16 out [M, F]; amax (nullable) += max |out|.  F % 8 == 0. */
+ * tfvideo/kernels.py:66-84); 2: the same from 16 gate and 16 up columns in turn (F % 16 == 0); bf16 out [M, F]; amax
+ * (nullable) += max |out|.  F % 8 == 0. */
 int h3_act(const void* u, int ldu, void* out, int ldo, int M, int F, int act_kind, float* amax, void* stream);
 /* mod[m, j] = ada_b[j] + t_emb[m] . ada_w[j] (fp32 [M, J]) (replaces MiniMaxH3Engine.modulation,
  * tfvideo/minimax_h3.py:265-269). */
@@ -239,14 +240,19 @@ int h3_attn_fp8_peers(const void* q, const void* k, const void* v, long long ld,
  * over those alone (device int32 [S], clipped to [0, S); both NULL: every key).  Packed requests, a prefix with causal
  * or frame-causal tokens behind it and windows are all spans.  A token with an empty span gets zeros.  Keys and values
  * outside a token's span never reach its row, whatever they hold (NaN and infinities included); where rows of its
- * 256-row tile see such a key, it can change the row's rounding, but no more.  Values up to 2^29 (the sums of a long
- * row of larger ones may overflow).  Hq query heads share Hk key heads in groups of Hq / Hk.  q, k and v are bf16 views
- * with their own token and head strides (multiples of 8 elements, 16-byte aligned), element (t, h, d) at t * ld +
- * h * hs + d; out (t, h, d) at out + t * ldo + h * 128 + d, apart from the inputs (H3_ERR_ARG otherwise).  Scores are
- * scaled by 1 / sqrt(128).  S <= 262,144.  workspace: h3_attn_bf16_workspace_bytes(S, Hk) bytes, 16-byte aligned (0 for
- * short sequences, which use none), one per call in flight: the key norms that let long rows of bounded scores skip
- * their running maximum, and the list of tiles; NULL is always accepted and only slower.  The reference's backends
- * (tfvideo/attention.py:29-54) attend to the whole sequence. */
+ * 256-row tile see such a key, it can change the row's rounding, but no more.  Hq query heads share
+ * Hk key heads in groups of Hq / Hk.  q, k and v are bf16 views with their own token and head strides (multiples of 8
+ * elements, 16-byte aligned), element (t, h, d) at t * ld + h * hs + d; out (t, h, d) at out + t * ldo + h * 128 + d,
+ * apart from the inputs (H3_ERR_ARG otherwise).  Scores are scaled by 1 / sqrt(128).  S <= 262,144.
+ * Scores, statistics of the softmax and sums are in 32 bits.  A key's weight exp(score - maximum) is rounded to bf16 (by
+ * at most 2^-8 of it) for the product with V and divided by the sum of unrounded ones.  Rows of bounded scores in calls
+ * with a workspace take some of their weights from a polynomial good to 7.5e-5, and keep the maximum of the first keys
+ * they see (a step of 128), so that later weights reach 2^80: with values above 2^29 their sums can overflow where the
+ * result would not.
+ * workspace: h3_attn_bf16_workspace_bytes(S, Hk) bytes, 16-byte aligned (0 for short sequences, which use none), one per
+ * call in flight: the key norms that let long rows of bounded scores skip their running maximum, and the list of tiles;
+ * NULL is always accepted and only slower.  The reference's backends (tfvideo/attention.py:29-54) attend to the whole
+ * sequence. */
 size_t h3_attn_bf16_workspace_bytes(int S, int Hk);
 int h3_attn_bf16(const void* q, long long ldq, long long hsq, const void* k, long long ldk, long long hsk,
                  const void* v, long long ldv, long long hsv, int S, int Hq, int Hk, const int* span_lo,

@@ -12,8 +12,8 @@
 // A tile whose rows follow one another moves by TMA boxes, any other by 16-byte asynchronous copies and stores of
 // single rows (TMA's gather4 took 90 cycles for each four rows, ten times too slow).  A row meets its own adapter's
 // weights only, so another request's never reach it, non-finite ones included; rows without an adapter are copied (or
-// left, in place) bit for bit.  With one adapter there is no plan: tiles are the rows
-// in order, and rows without the adapter are left out in the epilogue.
+// left, in place) bit for bit.  With one adapter there is no plan: tiles are the rows in order, and rows without the
+// adapter are left out in the epilogue.
 #pragma once
 
 #include "attention_bf16.cuh"

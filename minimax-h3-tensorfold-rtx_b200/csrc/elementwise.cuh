@@ -286,7 +286,8 @@ __device__ __forceinline__ float gelu_tanh_f(float u) {
 __device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + expf(-g)) * u; }
 
 // act = gelu_tanh(u) (act_kind 0, u [M, F]) or silu(gate) * up (act_kind 1, u = [gate | up] [M, 2F]; act_kind 2,
-// u [M, 2F] alternating 16 gate and 16 up columns, as a 16-interleaved fc1 writes them); bf16 out [M, F].  `amax` (nullable) receives max |act|.  tfvideo/kernels.py:66-84.
+// u [M, 2F] alternating 16 gate and 16 up columns, as a 16-interleaved fc1 writes them); bf16 out [M, F].  `amax`
+// (nullable) receives max |act|.  tfvideo/kernels.py:66-84.
 __global__ void __launch_bounds__(256) act_kernel(const __nv_bfloat16* u, int ldu, __nv_bfloat16* out, int ldo, int M,
                                                   int F, int act_kind, float* amax) {
   const int vec = F >> 3;

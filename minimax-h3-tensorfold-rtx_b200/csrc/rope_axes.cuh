@@ -167,7 +167,8 @@ __device__ __forceinline__ void qk_rows(const QkNormAxesArgs& a, const QkRows& t
 
 // FEW: at most seven heads, as many of k as of q (one GPU's share of the heads): all of a token's rows are on their way
 // before the angles, where the groups after the first would each wait for memory again.  (launch bounds: 80 registers,
-// three blocks an SM; unbounded or four blocks measured 411 and 307 us against 264 at 37,760 tokens, 40 heads)
+// three blocks an SM, 44 bytes spilled, 4 with FEW; unbounded or four blocks measured 411 and 307 us against 264 at
+// 37,760 tokens, 40 heads)
 template <int TYPE, bool FEW>
 __global__ void __launch_bounds__(256, 3) qknorm_rope_axes_kernel(const __grid_constant__ QkNormAxesArgs a,
                                                                      const __grid_constant__ RopePos r) {

@@ -182,7 +182,7 @@ def fp8_sparse(mask: TileMask):
 def bf16_tokens(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
                 mask: SpanMask | None = None) -> torch.Tensor:
     """Low-level form: q [S, Hq, 128], k and v [S, Hk, 128] bf16 views (token and head strides multiples of 8,
-    16-byte aligned); out [S, Hq * 128] bf16, row stride a multiple of 8."""
+    16-byte aligned); out [S, Hq * 128] bf16, row stride a multiple of 8.  Values and roundings as for ``bf16``."""
 
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] or k.shape[1] == 0 \
             or q.shape[1] % k.shape[1] or q.shape[2] != HEAD_DIM or k.shape[2] != HEAD_DIM \
@@ -230,6 +230,10 @@ def _tma_rows(t: torch.Tensor):
 
 
 def bf16(q, k, v, mask: SpanMask | None = None):
+    """q [1, H, S, 128], k and v [1, Hk, S, 128] bf16 (any strides; H a multiple of Hk), each token attending to its span
+    of ``mask`` (None: to every key).  Scores and sums are in 32 bits; a key's weight is rounded to bf16 for the product
+    with V.  Values up to 2^29: sums of larger ones may overflow in long rows (2,048 tokens and more)."""
+
     qs, ks = q.shape, k.shape
     if len(qs) != 4 or len(ks) != 4 or qs[0] != 1 or ks[0] != 1 or qs[3] != HEAD_DIM or ks[3] != HEAD_DIM \
             or v.shape != ks or not q.dtype == k.dtype == v.dtype == torch.bfloat16:

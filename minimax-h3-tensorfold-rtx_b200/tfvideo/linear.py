@@ -207,8 +207,9 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tens
                 scale: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """y[m] + B[a] (scale[a] A[a] x[m]) with a = rows[m], for bf16 x [M, K], y [M, N], A [n, R, K], B [n, N, R] (lower
     ranks padded with zeros), scale fp32 [n] (None: 1) and rows int32 [M], in any order; a row whose entry is outside
-    [0, n) has no adapter and keeps y's bits.  In place on y, unless ``out`` names other memory (apart from
-    y); either may be x itself.  K, N and R multiples of 8, R <= 128."""
+    [0, n) has no adapter and keeps y's bits.  Sums in 32 bits; scale[a] A[a] x[m] is rounded to bf16 once, before B[a].
+    In place on y, unless ``out`` names other memory (apart from y); either may be x itself.  K, N and R multiples of 8,
+    R <= 128."""
 
     out = y if out is None else out
     bf16 = torch.bfloat16
